@@ -17,6 +17,7 @@
 // gemm_tc.cu; the two cluster barriers (after set-up, before the tensor memory is freed) are reached by every
 // thread on every path.
 #include "gemm_tc_pair.cuh"
+#include "group_units.cuh"
 #include "umma.cuh"
 
 #include <stdlib.h>
@@ -121,61 +122,8 @@ __device__ __forceinline__ PairUnit pair_unit(int u, int tiles_m, int tiles, int
 // experts of 1,792 x 4,096, both products on the one-SM kernel's tiles of 64 and 128 / here: 560 / 417, 414 / 352, 331 / 330, 326 /
 // 317 us, of which 287 are the weights at the copy rate.  (Of 512 experts of 512 x 2,048 with 8 a token: 8,192 tokens 283 / 265,
 // 16,384 410 / 431, where the list below is too short.)
-// Rows come in tiles of 32 that belong to one group (an expert) each, negative groups are skipped.  A unit of
-// tokens is up to eight neighbouring tiles of one group, multiplied at their own width with that group's weight rows.  Every CTA
-// lists the units when it starts: one warp walks the tiles 32 at a time.  A unit is its first tile and, from bit 24 on, its tiles.
-__device__ __forceinline__ uint32_t group_unit_at(const int* tile_group, int n_tiles, int t) {
-    const int g = tile_group[t];
-    int c = 1;
-    while (c < PBN / P_GROUP_TILE && t + c < n_tiles && tile_group[t + c] == g) ++c;
-    return (uint32_t)t | (uint32_t)c << 24;
-}
-// All 32 lanes.  Writes the first P_LIST units and returns how many there are.  The groups of two stretches of 32 tiles are on their
-// way while one is looked at; where the runs of a stretch and of the next begin is a mask of 64 bits.  (With the loads of every
-// stretch, and of every unit's eight tiles, waited for where they were wanted, 2,048 tokens on 6 of 64 experts took 8 us longer a
-// product, 16,384 on 8 of 512 65.)
-__device__ __forceinline__ int group_units(const int* tile_group, int n_tiles, uint32_t* list) {
-    constexpr int MOST = PBN / P_GROUP_TILE;
-    const int lane = threadIdx.x & 31;
-    auto at = [&](int t) { return t < n_tiles ? tile_group[t] : -1; };
-    auto begins_of = [&](int g, int before) {
-        const int left = __shfl_up_sync(0xffffffffu, g, 1);
-        return __ballot_sync(0xffffffffu, g != (lane ? left : before));
-    };
-    int found = 0, run = 0, g = at(lane), next = at(32 + lane), after = at(64 + lane);      // run: where the one that reaches in began
-    uint32_t begins = begins_of(g, -1);
-    for (int t0 = 0; t0 < n_tiles; t0 += 32) {
-        const int further = at(t0 + 96 + lane);
-        const uint32_t begins_next = begins_of(next, __shfl_sync(0xffffffffu, g, 31));
-        const uint32_t mine = begins & (0xffffffffu >> (31 - lane));
-        const int t = t0 + lane, from = mine ? t0 + 31 - __clz(mine) : run;
-        const uint32_t units = __ballot_sync(0xffffffffu, g >= 0 && (t - from) % MOST == 0);
-        const int place = found + __popc(units & ((1u << lane) - 1u));
-        const int left = __ffsll((long long)(((unsigned long long)begins_next << 32 | begins) >> (lane + 1)));      // tiles of the run from t on
-        if ((units >> lane & 1u) && place < P_LIST) list[place] = (uint32_t)t | (uint32_t)(left == 0 || left > MOST ? MOST : left) << 24;
-        found += __popc(units);
-        run = __shfl_sync(0xffffffffu, from, 31);
-        g = next;
-        next = after;
-        after = further;
-        begins = begins_next;
-    }
-    return found;
-}
-// Unit i of the list or, where there are more than it holds, counted on from the last one that this thread asked for: a role asks
-// for ascending units, so that it walks the tiles once.  A sort of rows by group makes at most (tiles + 7 groups) / 8 units:
-// 440 hold 3,000 tiles of 64 groups and 1,700 of 256.
-struct GroupWalk { int i; uint32_t unit; };
-__device__ __forceinline__ uint32_t group_unit(const int* tile_group, int n_tiles, const uint32_t* list, int i, GroupWalk& walk) {
-    if (i < P_LIST) return list[i];
-    if (walk.i < P_LIST) walk = GroupWalk{P_LIST - 1, list[P_LIST - 1]};
-    for (; walk.i < i; ++walk.i) {
-        int t = (int)(walk.unit & 0xffffffu) + (int)(walk.unit >> 24);
-        while (tile_group[t] < 0) ++t;
-        walk.unit = group_unit_at(tile_group, n_tiles, t);
-    }
-    return walk.unit;
-}
+// Rows come in tiles of 32 that belong to one group (an expert) each; a unit of tokens (group_units.cuh) is up to eight neighbouring
+// tiles, multiplied at their own width with their group's weight rows.
 
 template <typename TO, bool ACT, bool GROUPED>     // ACT: the epilogue applies the plain activation `plain_act`
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1)
@@ -228,7 +176,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if (GROUPED) {
         if (warp == 2) {
             fb_pdl_wait();                       // which weights a tile wants is the work of the kernels before this one
-            const int found = group_units(tile_group, n_tiles, list);
+            const int found = group_units<P_LIST>(tile_group, n_tiles, PBN / P_GROUP_TILE, list);
             if (lane == 0) *group_count = found;
         }
         __syncthreads();
@@ -250,7 +198,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         if constexpr (GROUPED) {
             PairUnit w;
             const int i = u / tiles_n;
-            const uint32_t unit = group_unit(tile_group, n_tiles, list, i, walk);
+            const uint32_t unit = group_unit<P_LIST>(tile_group, n_tiles, PBN / P_GROUP_TILE, list, i, walk);
             w.m0 = (int)(unit & 0xffffffu) * P_GROUP_TILE;
             w.nt = u - i * tiles_n;
             w.split = 0;

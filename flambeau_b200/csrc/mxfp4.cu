@@ -1,0 +1,243 @@
+// Rows into four bits and back, and the tiles that the product reads (formats in mxfp4.cuh).
+//
+// A block's scale is the smallest power of two, not below 2^-127, under which its largest magnitude stays below 7, where rounding
+// still ends at 6: with amax = m 2^e, 1 <= m < 2, it is 2^(e - 2), or 2^(e - 1) where m >= 1.75.  Codes are the nearest of the grid,
+// ties to the even code (of 6 and less: scales end at 2^125,
+// so that every number of a block is a finite float32, and magnitudes above 6 times that become it); both follow from bits and from products with powers of two, so they are the same on any machine.  A block
+// with an infinity or a NaN gets scale 255 and decodes to NaN.
+//
+// Bound by memory: 2 or 4 bytes in, 17/32 out.  Four threads share a block, eight numbers each; a warp reads 512 bytes (bfloat16) in
+// a row.
+#include "mxfp4.cuh"
+
+namespace {
+
+// Eight numbers of a row from column c on; zeros beyond K.
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+// VEC: rows start on 16-byte borders (and their strides keep them there).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+quantize_kernel(const T* __restrict__ x, long ldx, long rows, int K, int blocks, uint8_t* __restrict__ codes,
+                uint8_t* __restrict__ scales) {
+    fb_pdl_launch_dependents();
+    fb_pdl_wait();
+    const long quarters = rows * blocks * 4;                             // a quarter: eight numbers
+    const long step = (long)gridDim.x * 256;
+    for (long base = (long)blockIdx.x * 256; base < quarters; base += step) {     // (whole warps stay together for the shuffles)
+        const long q = base + threadIdx.x;
+        const bool mine = q < quarters;
+        const long row = mine ? q / (blocks * 4) : 0;
+        const int c = mine ? 8 * (int)(q - row * (blocks * 4)) : 0;
+        float v[8];
+        const T* p = x + row * ldx + c;
+        if (VEC && mine && c + 8 <= K) {
+            load8(p, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = mine && c + i < K ? fb_to_float(p[i]) : 0.0f;
+        }
+        uint32_t top = 0;                                                // the largest magnitude's bits (NaN above infinity)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int s = min(MX_LAST_SCALE, max(0, (int)(top >> 23) - 2 + ((top & 0x7fffffu) >= 0x600000u ? 1 : 0)));
+        const bool finite = top < 0x7f800000u;
+        const float inv = __uint_as_float((uint32_t)(254 - s) << 23);    // 2^(127 - s)
+        uint32_t out = 0;
+        if (finite) {
+            asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+                "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+                : "=r"(out)
+                : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
+                  "f"(v[6] * inv), "f"(v[7] * inv));
+        }
+        if (mine) {
+            reinterpret_cast<uint32_t*>(codes)[q] = out;                 // (quarters of a row follow one another)
+            if ((q & 3) == 0) scales[q >> 2] = finite ? (uint8_t)s : 255;
+        }
+    }
+}
+
+__device__ __forceinline__ float code_value(uint32_t code, float scale) {
+    const uint32_t m = code & 7u;
+    const float v = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+    return copysignf(v, code & 8u ? -1.0f : 1.0f) * scale;
+}
+__device__ __forceinline__ float scale_value(uint32_t s) {
+    return __uint_as_float(s == 255u ? 0x7fc00000u : s == 0 ? 0x00400000u : s << 23);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long rows, int K, int blocks,
+                  T* __restrict__ out, long ldo) {
+    fb_pdl_launch_dependents();
+    fb_pdl_wait();
+    const long quarters = rows * blocks * 4, step = (long)gridDim.x * 256;
+    for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < quarters; q += step) {
+        const long row = q / (blocks * 4);
+        const int c = 8 * (int)(q - row * (blocks * 4));
+        const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[q];
+        const float scale = scale_value(scales[q >> 2]);
+        T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fb_from_float<T>(code_value(w >> (4 * i) & 15u, scale));
+        T* p = out + row * ldo + c;
+        if (VEC && c + 8 <= K) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(v) / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(v)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < K) p[i] = v[i];
+        }
+    }
+}
+
+// The two kernels that write the tiles let no kernel behind them in before they end: the product asks for its first weights ahead of
+// its wait for the kernel before it, and that kernel may have come in early itself.
+// shifts[g] = how far the scales of matrix g have to be lowered (one block a matrix; scales of 255 do not count).
+__global__ void __launch_bounds__(1024)
+shift_kernel(const uint8_t* __restrict__ scales, long per_group, int* __restrict__ shifts) {
+    fb_pdl_wait();
+    __shared__ float scratch[32];
+    const uint8_t* s = scales + (size_t)blockIdx.x * per_group;
+    int top = 0;
+    for (long i = threadIdx.x; i < per_group; i += 1024) {
+        const int v = s[i];
+        if (v != 255) top = max(top, v);
+    }
+    const float all = fb_block_max((float)top, scratch);
+    if (threadIdx.x == 0) shifts[blockIdx.x] = max(0, (int)all - MX_TOP_SCALE);
+}
+
+// A thread a row and block of 32 columns: its 16 bytes of codes in the tiles' order, its scale lowered by the matrix's shift.
+__global__ void __launch_bounds__(128)
+tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int N, int blocks, int tiles_k,
+             const int* __restrict__ shifts, uint8_t* __restrict__ tiles) {
+    fb_pdl_wait();
+    const int row = threadIdx.x, b = blockIdx.x, n = blockIdx.y * MX_ROWS + row, group = blockIdx.z;
+    const size_t tile = ((size_t)group * gridDim.y + blockIdx.y) * tiles_k + b / 4;
+    uint8_t* dst = tiles + tile * MX_TILE_BYTES;
+    uint32_t w[4] = {0, 0, 0, 0};
+    int s = 0;
+    if (n < N && b < blocks) {
+        const size_t at = ((size_t)group * N + n) * blocks + b;
+        const uint4 c = reinterpret_cast<const uint4*>(codes)[at];
+        const uint32_t in[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[i] |= mx_place(in[i] >> (8 * j) & 15u, j) | mx_place(in[i] >> (8 * j + 4) & 15u, j) << 16;
+        s = scales[at];
+        if (s != 255) {
+            s -= shifts[group];
+            if (s < 0) {                 // below 2^-127 of the largest scale that the product takes: nothing is left of it
+                s = 0;
+                w[0] = w[1] = w[2] = w[3] = 0;
+            }
+        }
+    }
+    reinterpret_cast<uint4*>(dst)[(b & 3) * MX_ROWS + row] = make_uint4(w[0], w[1], w[2], w[3]);
+    dst[MX_CODE_BYTES + row * 4 + (b & 3)] = (uint8_t)s;
+}
+
+// Rows of bfloat16 numbers into rows that start on 16-byte borders.
+__global__ void __launch_bounds__(256)
+align_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, int M, int K, __nv_bfloat16* __restrict__ out, long ldo) {
+    fb_pdl_launch_dependents();
+    fb_pdl_wait();
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)M * K; i += (long)gridDim.x * 256) {
+        const long m = i / K, k = i - m * K;
+        out[m * ldo + k] = x[m * ldx + k];
+    }
+}
+
+int grid_of(long threads, int per_block) {
+    const long blocks = (threads + per_block - 1) / per_block, most = 8L * fb_sm_count();
+    return (int)(blocks < most ? blocks : most);
+}
+
+}  // namespace
+
+// codes [rows, 16 ceil(K / 32)] and scales [rows, ceil(K / 32)] (contiguous) of x [rows, K], float32 or bfloat16 with rows ldx
+// elements apart; the columns behind K of a row's last block count as zeros.
+FB_API int fb_quantize_mxfp4(const void* x, int dtype, long long ldx, long long rows, int K, void* codes, void* scales,
+                             cudaStream_t stream) {
+    FB_REQUIRE(rows >= 0 && K > 0 && K <= (1 << 30), "quantize_mxfp4: bad sizes");
+    FB_REQUIRE(ldx >= K || rows <= 1, "quantize_mxfp4: a row stride is shorter than its row");
+    FB_REQUIRE(((uintptr_t)codes & 15) == 0, "quantize_mxfp4: codes must be 16-byte aligned");
+    if (rows == 0) return 0;
+    const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+    FB_DISPATCH_DTYPE(dtype, T, {
+        const bool vec = ((uintptr_t)x & 15) == 0 && (rows == 1 || ldx * sizeof(T) % 16 == 0);
+        auto kernel = vec ? quantize_kernel<T, true> : quantize_kernel<T, false>;
+        fb_launch(kernel, dim3(grid_of((long)rows * blocks * 4, 256)), dim3(256), 0, stream, (const T*)x, (long)ldx, (long)rows, K,
+                  blocks, (uint8_t*)codes, (uint8_t*)scales);
+    });
+    return fb_check_launch("quantize_mxfp4");
+}
+
+// out [rows, K], float32 or bfloat16: the numbers that codes and scales stand for (bfloat16 holds them exactly;
+// 4 and 6 times 2^127, which fb_quantize_mxfp4 never writes, are infinite in both).
+FB_API int fb_dequantize_mxfp4(const void* codes, const void* scales, long long rows, int K, void* out, int dtype, long long ldo,
+                               cudaStream_t stream) {
+    FB_REQUIRE(rows >= 0 && K > 0 && K <= (1 << 30), "dequantize_mxfp4: bad sizes");
+    FB_REQUIRE(ldo >= K || rows <= 1, "dequantize_mxfp4: a row stride is shorter than its row");
+    FB_REQUIRE(((uintptr_t)codes & 15) == 0, "dequantize_mxfp4: codes must be 16-byte aligned");
+    if (rows == 0) return 0;
+    const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
+    FB_DISPATCH_DTYPE(dtype, T, {
+        const bool vec = ((uintptr_t)out & 15) == 0 && (rows == 1 || ldo * sizeof(T) % 16 == 0);
+        auto kernel = vec ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
+        fb_launch(kernel, dim3(grid_of((long)rows * blocks * 4, 256)), dim3(256), 0, stream, (const uint8_t*)codes,
+                  (const uint8_t*)scales, (long)rows, K, blocks, (T*)out, (long)ldo);
+    });
+    return fb_check_launch("dequantize_mxfp4");
+}
+
+// Bytes of one matrix [N, K] in tiles.
+FB_API long long fb_mxfp4_tile_bytes(int N, int K) {
+    return (long long)((N + MX_ROWS - 1) / MX_ROWS) * ((K + MX_COLS - 1) / MX_COLS) * MX_TILE_BYTES;
+}
+
+// `groups` matrices [N, K] from rows (codes, scales as fb_quantize_mxfp4 writes them) into tiles, and shifts[groups] (int32).
+FB_API int fb_mxfp4_tiles(const void* codes, const void* scales, int groups, int N, int K, void* tiles, int* shifts,
+                          cudaStream_t stream) {
+    FB_REQUIRE(groups > 0 && N > 0 && K > 0 && groups <= 65535 && N <= 65535 * MX_ROWS, "mxfp4_tiles: bad sizes");
+    FB_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)tiles & 15) == 0, "mxfp4_tiles: operands must be 16-byte aligned");
+    const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK, tiles_k = (K + MX_COLS - 1) / MX_COLS;
+    fb_launch(shift_kernel, dim3(groups), dim3(1024), 0, stream, (const uint8_t*)scales, (long)N * blocks, shifts);
+    fb_launch(tiles_kernel, dim3(4 * tiles_k, (N + MX_ROWS - 1) / MX_ROWS, groups), dim3(128), 0, stream, (const uint8_t*)codes,
+              (const uint8_t*)scales, N, blocks, tiles_k, shifts, (uint8_t*)tiles);
+    return fb_check_launch("mxfp4_tiles");
+}
+
+// out[m, k] = x[m, k], rows of `out` ldo elements apart (what lies between them is left as it is).
+FB_API int fb_align_rows(const void* x, long long ldx, int M, int K, void* out, long long ldo, cudaStream_t stream) {
+    FB_REQUIRE(M >= 0 && K > 0 && (ldx >= K || M <= 1) && ldo >= K, "align_rows: bad sizes");
+    if (M == 0) return 0;
+    fb_launch(align_rows_kernel, dim3(grid_of((long)M * K, 256)), dim3(256), 0, stream, (const __nv_bfloat16*)x, (long)ldx, M, K,
+              (__nv_bfloat16*)out, (long)ldo);
+    return fb_check_launch("align_rows");
+}

@@ -101,6 +101,7 @@ int fb_tensor_map_bf16_uncached(CUtensorMap* out, const void* ptr, long rows, lo
 
 // An output of a product: [slabs][rows][cols] of float32 or bfloat16 (row stride ld, slab stride slab_stride, in
 // elements), written in boxes of box_rows x box_cols elements of one slab as they lie in shared memory (no swizzle).
+// A row that ends inside 16 bytes is not taken: measured, the store fills the 16 bytes up, beyond the row.
 // Not cached: outputs are workspace views that differ from call to call more often than not, and the encoder takes
 // no memory.  Returns 1 if such a map cannot be made for these strides and this address (the caller then stores
 // without it), 0 if it was made, a negative code after fb_fail() if the driver refused it.
@@ -111,7 +112,7 @@ int fb_tensor_map_out(CUtensorMap* out, void* ptr, int elem_bytes, long rows, lo
     if (slabs < 1) slabs = 1;
     if (slabs == 1) slab_stride = rows * ld;
     const bool ok = ((uintptr_t)ptr & 15) == 0 && (ld * elem_bytes) % 16 == 0 && (slab_stride * elem_bytes) % 16 == 0 &&
-                    (box_cols * elem_bytes) % 16 == 0 && box_cols <= 256 && box_rows <= 256 && rows > 0 && cols > 0;
+                    (cols * elem_bytes) % 16 == 0 && (box_cols * elem_bytes) % 16 == 0 && box_cols <= 256 && box_rows <= 256 && rows > 0 && cols > 0;
     if (!ok) return 1;
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)slabs};
     const cuuint64_t strides[2] = {(cuuint64_t)ld * elem_bytes, (cuuint64_t)slab_stride * elem_bytes};

@@ -598,6 +598,11 @@ class _SplitScratch:
         return hit
 
 
+class PackedWeight:
+    """A linear map's weight that is no tensor: `linear`, `linear_slabs`, `linear_add`, `gated_linear`, `activated_linear`,
+    `grouped_linear` and `grouped_gated_linear` call its method instead of a kernel for tensors (Mxfp4Weight)."""
+
+
 def tc_supported(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> bool:
     """Whether the tcgen05 product takes these operands: bfloat16, 16-byte aligned, row strides of 8 elements."""
     return (a.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and out.dtype in _CODES
@@ -715,6 +720,8 @@ def gemm_tc_act(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, status: tor
 def linear_slabs(a: torch.Tensor, w: torch.Tensor, slabs: torch.Tensor, ctx) -> int:
     """slabs[0] + ... + slabs[k-1] = a @ w^T; returns k.  The tensor-core kernel leaves the split-K shares for the
     next kernel to add; every other path writes the whole product into slabs[0]."""
+    if isinstance(w, PackedWeight):
+        return w.linear_slabs(a, slabs, ctx)
     out = slabs[0]
     if slabs.shape[0] > 1 and tc_supported(a, w, out):
         return gemm_tc(a, w, out, ctx.runtime.status, slabs=slabs)
@@ -804,6 +811,9 @@ def grouped_gated_linear(a: torch.Tensor, row_index, w: torch.Tensor, tile_group
     and up rows alternating): on the tcgen05 kernel with the activation in its epilogue for bfloat16 operands, else
     the float32-FMA grouped product followed by the activation kernel.  row_share / row_pair (with row_index): the
     fetched row is multiplied by row_share[row_pair[m]] on its way (see gather_rows)."""
+    if isinstance(w, PackedWeight):
+        w.grouped(a, row_index, tile_group, tile, out, ctx, gate=activation, row_share=row_share, row_pair=row_pair)
+        return
     if grouped_tc_supported(a, w, out):
         with ctx.ws.scope():
             side = a
@@ -830,6 +840,9 @@ def grouped_linear(a: torch.Tensor, row_index, w: torch.Tensor, tile_group: torc
     experts over rows that were sorted by expert and padded to whole tiles.  bfloat16 operands go to the tcgen05
     kernel (rows that have to be fetched through row_index are first laid side by side, since tensor-map copies
     take whole tiles of consecutive rows); everything else to the float32-FMA kernel, which fetches by index."""
+    if isinstance(w, PackedWeight):
+        w.grouped(a, row_index, tile_group, tile, out, ctx, activation_name, row_share=row_share, row_pair=row_pair)
+        return
     if ctx is not None and grouped_tc_supported(a, w, out):
         if row_index is not None:
             with ctx.ws.scope():
@@ -854,13 +867,53 @@ def grouped_linear(a: torch.Tensor, row_index, w: torch.Tensor, tile_group: torc
 
 def linear(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, ctx=None) -> None:
     """out = a @ w^T with the kernel that fits the dtypes and the shape: the tcgen05 kernels for bfloat16 and for
-    float32 operands they can fetch by TMA, the float32-FMA kernel for everything else."""
+    float32 operands they can fetch by TMA, the float32-FMA kernel for everything else; four-bit weights (Mxfp4Weight)
+    multiply bfloat16 rows on a tcgen05 kernel of their own."""
+    if isinstance(w, PackedWeight):
+        w.linear(a, out, ctx)
+        return
     if ctx is not None and tc_supported(a, w, out):
         gemm_tc(a, w, out, ctx.runtime.status)
     elif getattr(ctx, "ws", None) is not None and f32_tc_supported(a, w, out):
         gemm_f32_tc(a, w, out, ctx.runtime.status, ctx.ws)
     else:
         gemm_simt(a, w, out)
+
+
+def linear_add(a: torch.Tensor, w, acc: torch.Tensor, ctx, max_slabs: int = 1) -> bool:
+    """acc += a @ w^T in float32 where the product's own epilogue can do the add; False, with nothing done, where it cannot
+    (see gemm_tc_add)."""
+    if isinstance(w, PackedWeight):
+        return w.linear_add(a, acc, ctx)
+    return gemm_tc_add(a, w, acc, ctx.runtime.status, max_slabs)
+
+
+def gated_linear(a: torch.Tensor, w, out: torch.Tensor, activation, ctx) -> None:
+    """out[M, N/2] = act(g) * u where (g_0, u_0, g_1, u_1, ...) = a @ w^T: w stacks gate and up rows alternately.  In the
+    product's epilogue for bfloat16 operands and four-bit weights, else by a product and the activation kernel."""
+    if isinstance(w, PackedWeight):
+        w.gated_linear(a, out, activation, ctx)
+    elif tc_supported(a, w, out):
+        gemm_tc_gated(a, w, out, ctx.runtime.status, activation)
+    else:
+        with ctx.ws.scope():
+            z = ctx.ws.alloc((a.shape[0], w.shape[0]), out.dtype)
+            linear(a, w, z, ctx)
+            gate_mul(z, out, activation=activation)
+
+
+def activated_linear(a: torch.Tensor, w, out: torch.Tensor, activation_name: str, ctx) -> None:
+    """out[M, N] = act(a @ w^T) with a plain activation (PLAIN_ACTIVATIONS): in the product's epilogue for bfloat16 operands
+    and four-bit weights, else by a product and the activation kernel."""
+    if isinstance(w, PackedWeight):
+        w.activated_linear(a, out, activation_name, ctx)
+    elif tc_supported(a, w, out):
+        gemm_tc_act(a, w, out, ctx.runtime.status, activation_name)
+    else:
+        with ctx.ws.scope():
+            z = ctx.ws.alloc((a.shape[0], w.shape[0]), torch.float32)
+            linear(a, w, z, ctx)
+            activation(z, out, activation_name)
 
 
 class _AttentionScratch:
@@ -1549,3 +1602,204 @@ def hc_step(streams: torch.Tensor, y, n_partials: int, partial_stride: int, mix,
                            dtype_code(norm_weight) if norm_weight is not None else 0, float(eps), float(weight_offset),
                            _ptr(out), dtype_code(out) if out is not None else 0, _ptr(rows), 1 if write_back else 0,
                            n_out, D, _stream()), "hc_step")
+
+
+# ---------------------------------------------------------------------------
+# four-bit weights
+# ---------------------------------------------------------------------------
+# Blocks of 32 numbers along a row share a power-of-two scale (microscaled E2M1, csrc/mxfp4.cuh): a number is a sign and one of the
+# magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6, times 2^(S - 127), S being its block's byte (255: the block is not a number).  As rows they
+# are codes uint8 [..., 16 * blocks], element 2 i of a block in the low half of byte i, and scales uint8 [..., blocks], blocks =
+# ceil(columns / 32).
+
+MXFP4_BLOCK = 32          # numbers that share a scale
+
+
+def quantize_mxfp4(x: torch.Tensor) -> tuple:
+    """(codes, scales) of x [..., columns], float32 or bfloat16 (a 2-d x may have rows apart, more dimensions are contiguous).
+
+    A block's scale is the smallest power of two, not below 2^-127, under which its largest magnitude stays below 7 (where
+    rounding still ends at 6), but at most 2^125, so that every number is a finite float32; numbers go to the nearest of the grid, ties to the even code.  A block with an infinity or a NaN
+    becomes NaN as a whole.  The columns behind the last one of a row's last block count as zeros."""
+    _cuda(x)
+    code = dtype_code(x)
+    if x.dim() < 2 or x.shape[-1] < 1:
+        raise KernelError(f"quantize_mxfp4: rows wanted, not a tensor of shape {tuple(x.shape)}")
+    if x.dim() > 2 and not x.is_contiguous():
+        raise KernelError("quantize_mxfp4: more than two dimensions must be contiguous")
+    flat = x if x.dim() == 2 else x.view(-1, x.shape[-1])
+    rows, columns = flat.shape
+    stride = _rows(flat) if rows > 1 or flat.stride(1) != 1 else columns
+    blocks = -(-columns // MXFP4_BLOCK)
+    codes = torch.empty((*x.shape[:-1], 16 * blocks), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device)
+    check(lib().fb_quantize_mxfp4(flat.data_ptr(), code, stride, rows, columns, codes.data_ptr(), scales.data_ptr(), _stream()),
+          "quantize_mxfp4")
+    return codes, scales
+
+
+def _mxfp4_blocks(codes: torch.Tensor, scales: torch.Tensor, columns: int, what: str) -> int:
+    """The number of blocks of a row."""
+    _cuda(codes, scales)
+    blocks = -(-int(columns) // MXFP4_BLOCK)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or columns < 1 or codes.dim() < 2 \
+            or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * blocks or scales.shape[-1] != blocks:
+        raise KernelError(f"{what}: uint8 codes [..., {16 * blocks}] and scales [..., {blocks}] wanted for {columns} columns, not "
+                          f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+    if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
+        raise KernelError(f"{what}: codes and scales must be contiguous, codes on a 16-byte border")
+    return blocks
+
+
+def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, columns: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The numbers that codes and scales stand for, [..., columns] in float32 or bfloat16 (which holds them exactly)."""
+    blocks = _mxfp4_blocks(codes, scales, columns, "dequantize_mxfp4")
+    out = torch.empty((*codes.shape[:-1], columns), dtype=dtype, device=codes.device)
+    code = dtype_code(out)
+    check(lib().fb_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), scales.numel() // blocks, int(columns), out.data_ptr(), code,
+                                    int(columns), _stream()), "dequantize_mxfp4")
+    return out
+
+
+class Mxfp4Weight(PackedWeight):
+    """A linear map's weight [outputs, inputs], or several of one size [groups, outputs, inputs], in four bits, laid out for the
+    products once (the codes and scales that it is made from are not kept).
+
+    `shape`, `dtype` (of the rows that it multiplies), `device`, `nbytes` are those of a weight tensor.  Every number of such a
+    weight is a bfloat16 number: the products give what bfloat16 products with `dequantize_mxfp4`'s numbers give, up to the order of
+    their float32 sums.  (Numbers below 2^-127 of 3 times a matrix's largest scale, where that is above 2, count as zeros.)"""
+    dtype = torch.bfloat16
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, inputs: int):
+        _mxfp4_blocks(codes, scales, inputs, "mxfp4 weight")
+        if codes.dim() not in (2, 3):
+            raise KernelError(f"mxfp4 weight: [outputs, inputs] or [groups, outputs, inputs] wanted, not {codes.dim()} dimensions")
+        self.shape = torch.Size((*codes.shape[:-1], int(inputs)))
+        groups = codes.shape[0] if codes.dim() == 3 else 1
+        outputs = codes.shape[-2]
+        if groups < 1 or outputs < 1:
+            raise KernelError("mxfp4 weight: no outputs")
+        self.device = codes.device
+        self.tiles = torch.empty(groups * lib().fb_mxfp4_tile_bytes(outputs, int(inputs)), dtype=torch.uint8, device=codes.device)
+        self.shifts = torch.empty(groups, dtype=torch.int32, device=codes.device)
+        check(lib().fb_mxfp4_tiles(codes.data_ptr(), scales.data_ptr(), groups, outputs, int(inputs), self.tiles.data_ptr(),
+                                   self.shifts.data_ptr(), _stream()), "mxfp4_tiles")
+
+    @classmethod
+    def from_dense(cls, weight: torch.Tensor) -> "Mxfp4Weight":
+        """The weight tensor (float32 or bfloat16), quantised."""
+        return cls(*quantize_mxfp4(weight.contiguous()), weight.shape[-1])
+
+    @property
+    def nbytes(self) -> int:
+        return self.tiles.numel() + 4 * self.shifts.numel()
+
+    def dim(self) -> int:
+        return len(self.shape)
+
+    def _matrix(self, a: torch.Tensor, out: torch.Tensor, columns: int, what: str) -> tuple:
+        if self.dim() != 2:
+            raise KernelError(f"{what}: one matrix wanted, not {tuple(self.shape)}")
+        return self._operands(a, out, columns, what)
+
+    def _operands(self, a: torch.Tensor, out: torch.Tensor, columns: int, what: str) -> tuple:
+        """Checks what a product takes: a [M, K] bfloat16, out [M, columns] float32 or bfloat16, rows dense.  (M, N, K)."""
+        _cuda(a, out)
+        N, K = self.shape[-2:]
+        if a.dim() != 2 or out.dim() != 2 or a.shape[1] != K or out.shape[1] != columns or out.shape[0] != a.shape[0]:
+            raise KernelError(f"{what}: shapes a{tuple(a.shape)} w{tuple(self.shape)} out{tuple(out.shape)} do not agree")
+        if a.dtype != torch.bfloat16:
+            raise KernelError(f"{what}: four-bit weights multiply bfloat16 rows, not {a.dtype}")
+        if a.device != self.device or out.device != self.device:
+            raise KernelError(f"{what}: the weight is on {self.device}, the rows on {a.device}, the output on {out.device}")
+        dtype_code(out)
+        _rows(out)
+        return a.shape[0], N, K
+
+    @staticmethod
+    def _aligned(a: torch.Tensor, ws) -> torch.Tensor:
+        """a, or a copy of it in the arena where its rows do not start on 16-byte borders."""
+        if _rows(a) % 8 == 0 and a.data_ptr() % 16 == 0:
+            return a
+        M, K = a.shape
+        side = ws.alloc((M, -(-K // 8) * 8), a.dtype)
+        check(lib().fb_align_rows(a.data_ptr(), _rows(a), M, K, side.data_ptr(), side.stride(0), _stream()), "align_rows")
+        return side[:, :K]
+
+    def _product(self, a, out, ctx, columns: int, what: str, gate=(0, 0.0, 0.0), plain_act: int = 0, accumulate: bool = False,
+                 slabs=None) -> int:
+        M, N, K = self._matrix(a, out, columns, what)
+        ws, used = ctx.ws, ctypes.c_int(1)
+        counters = ws.counters
+        with ws.scope():
+            a = self._aligned(a, ws)
+            floats, partials = 0, None
+            if slabs is None:
+                floats = lib().fb_gemm_mxfp4_scratch_floats(M, N, K, counters.numel())
+                partials = ws.alloc((floats,), torch.float32) if floats > 0 else None
+            check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self.tiles.data_ptr(), self.shifts.data_ptr(), out.data_ptr(),
+                                      dtype_code(out), _rows(out), slabs.stride(0) if slabs is not None else 0,
+                                      slabs.shape[0] if slabs is not None else 0, ctypes.byref(used), M, N, K, *gate, plain_act,
+                                      1 if accumulate else 0, _ptr(partials), floats, counters.data_ptr(), counters.numel(),
+                                      ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
+        return used.value
+
+    def linear(self, a, out, ctx) -> None:
+        self._product(a, out, ctx, self.shape[-2], "linear")
+
+    def linear_slabs(self, a, slabs, ctx) -> int:
+        if slabs.dim() != 3 or slabs.dtype != torch.float32 or slabs.shape[0] < 1:
+            raise KernelError("linear_slabs: float32 slabs [shares, rows, outputs] wanted")
+        if slabs.shape[0] == 1:
+            self.linear(a, slabs[0], ctx)
+            return 1
+        return self._product(a, slabs[0], ctx, self.shape[-2], "linear_slabs", slabs=slabs)
+
+    def linear_add(self, a, acc, ctx) -> bool:
+        if acc.dtype != torch.float32:
+            raise KernelError("linear_add: a float32 output wanted")
+        # up to 128 rows the shares of K are better left to the next norm, which fetches the stream anyway
+        if a.shape[0] <= 128:
+            return False
+        self._product(a, acc[:a.shape[0]], ctx, self.shape[-2], "linear_add", accumulate=True)
+        return True
+
+    def gated_linear(self, a, out, activation, ctx) -> None:
+        if self.shape[-2] % 2:
+            raise KernelError("gated_linear: gate and up rows alternate, their number is even")
+        self._product(a, out, ctx, self.shape[-2] // 2, "gated_linear", gate=gate_arguments(activation))
+
+    def activated_linear(self, a, out, activation_name, ctx) -> None:
+        self._product(a, out, ctx, self.shape[-2], "activated_linear", plain_act=plain_activation_code(activation_name))
+
+    def grouped(self, a, row_index, tile_group, tile: int, out, ctx, activation_name=None, gate=None, row_share=None,
+                row_pair=None) -> None:
+        """grouped_linear, or with `gate` grouped_gated_linear."""
+        what = "grouped product"
+        if ctx is None:
+            raise KernelError(f"{what}: four-bit weights need the step's scratch (ctx)")
+        _cuda(a, row_index, tile_group, out)
+        _i32(tile_group, "tile_group")
+        N, K = self.shape[-2:]
+        M = out.shape[0]
+        if self.dim() != 3 or (gate is not None and N % 2):
+            raise KernelError(f"{what}: weights [groups, outputs, inputs] wanted, with a gate an even number of outputs")
+        if tile < 16 or tile > 128 or tile % 16 or M % tile or tile_group.numel() * tile < M or not tile_group.is_contiguous():
+            raise KernelError(f"{what}: {M} rows are not whole tiles of {tile} (a multiple of 16 up to 128) with a group each")
+        ws = ctx.ws
+        with ws.scope():
+            if row_index is not None:
+                if row_index.numel() < M or a.shape[1] != K:
+                    raise KernelError(f"{what}: shapes do not agree")
+                side = ws.alloc((M, K), a.dtype)
+                gather_rows(a, row_index, side, row_share, row_pair, tile_group, tile)
+                a = side
+            elif row_share is not None:
+                raise KernelError(f"{what}: shares of rows go with an index of rows")
+            self._operands(a, out, N // 2 if gate is not None else N, what)
+            a = self._aligned(a, ws)
+            gate_args = gate_arguments(gate) if gate is not None else (0, 0.0, 0.0)
+            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), self.tiles.data_ptr(), self.shifts.data_ptr(),
+                                              self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(), dtype_code(out),
+                                              _rows(out), M, N, K, *gate_args, plain_activation_code(activation_name),
+                                              ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4_grouped", (M, N, K))
