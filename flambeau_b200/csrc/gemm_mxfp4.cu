@@ -1,63 +1,131 @@
 // out[M,N] = X[M,K] * W[N,K]^T with X in bfloat16 and W in four bits (mxfp4.cuh) on the 5th-generation tensor cores.
 //
-// Every number of W is a bfloat16 number, so the product is that of two bfloat16 matrices, summed in float32: nothing is rounded
-// that a bfloat16 weight would not have rounded.  What is gained is memory: 17 bits for every four of a bfloat16 weight.
+// tcgen05.mma.kind::mxf8f6f4 multiplies 8-bit numbers whose blocks of 32 along K carry power-of-two scales, and sums in float32.
+// A four-bit weight is such a number as it is.  A row's bfloat16 numbers become two e4m3 numbers each, the second what the first left
+// (mxfp4.cuh: what is lost is below 2^-22 of a block's largest number, far below what bfloat16 itself has rounded), so the
+// product is that of bfloat16 rows with the weights' numbers, summed in float32; only infinities among the rows end as NaN.
 //
-// Layout.  One CTA owns 128 output features x up to 192 tokens ("swap-AB": the weight is the 128-row operand of tcgen05.mma, the
-// tokens its N dimension).  A stage is 128 of K: one bulk copy brings a weight tile of 8,704 bytes as it lies in memory, two TMA copies
-// (128-byte swizzle) the tokens.  Eight warps decode: a thread a feature, 128 numbers a stage as 64 pairs into tensor memory, where
-// the MMA takes its A operand from.  The decoded weights never pass through shared memory: at 88 bytes a cycle for writing and as
-// many for reading, which memory speed would ask for, its 128 bytes a cycle would be the bound.  The two groups of four warps
-// take the stages in turn.
+// Why this instruction, on one SM, for 128 features x 128 of K (a tile of 8,704 bytes, which HBM brings every 370 cycles): kind::f16
+// takes 8 instructions of 70 cycles at least, whatever the number of tokens up to 128, and its weights have to be decoded to
+// bfloat16 (19 instructions for eight: shifts, masks, multiplications); this kind takes 4 of 35 cycles up to 32 tokens (N = 64: both
+// parts side by side), and decoding is moving bits (7 instructions for eight), since the scales go to the tensor core as
+// they are.
 //
-// Warps: 0 weight copies, 1 MMA, 2 token copies, 3 tensor memory, 4..11 decode, 12.. epilogue (a thread a feature; two warps a lane
-// quarter in the wide form).  full[s]: the stage's tokens (bytes) and its decoded weights (128 arrivals) are there; done[s]: its
-// MMAs are.  Two accumulators, so that the epilogue of one unit overlaps the products of the next.
+// Layout.  A CTA owns 128 output features x a tile of tokens ("swap-AB": the weight is the 128-row operand, the tokens are N).  A stage
+// is 128 of K: one bulk copy brings a weight tile as it lies in memory, groups of four warps take the stages in turn and decode, a
+// thread a feature, into tensor memory, where the MMA takes its A operand and both operands' scales from; the rows' parts, made
+// once for all CTAs by a kernel of their own, come by TMA (K-major, 128-byte swizzle), their scales by tcgen05.cp.  Up to 64 tokens the
+// two parts are N's two halves, which the epilogue adds; with more they are two instructions into one accumulator.
 //
-// Shares of K go to slabs that the next kernel adds, or meet in scratch, where the CTA that arrives last (a counter a tile, no
-// waiting) adds them in order.  Grouped form (routed experts): a unit is a run of neighbouring row tiles of one group.
+// The narrow form (up to 32 tokens: decoding, experts' few rows): the tiles of all row tiles form one line that the CTAs cut into
+// equal stretches.  The wide form sends its output through shared memory.  Shares of K go to slabs that the next kernel adds, or
+// meet in scratch, where the CTA that arrives last (a counter a row tile, no waiting) adds them in order.  Grouped (routed
+// experts): row tiles of one group each; a unit is a run of neighbouring ones.
 //
-// Every mbarrier wait is bounded as in gemm_tc.cu.
+// full[s]: a stage's rows and its decoded weights are there; done[s]: its MMAs are.  Two accumulators, so that the epilogue of one
+// unit overlaps the products of the next.  Every mbarrier wait is bounded as in gemm_tc.cu.
 #include "group_units.cuh"
 #include "mxfp4.cuh"
 #include "tensor_map.cuh"
 #include "umma.cuh"
 
+#include <map>
+#include <mutex>
+#include <tuple>
+
 namespace {
 
-constexpr int XBM = MX_ROWS;                      // output features per CTA
-constexpr int XBK = MX_COLS;                      // K per stage
-constexpr int A_COLS = XBK / 2;                   // tensor-memory columns of a stage's weights
-constexpr int MAX_W = 16, MAX_R = 4;              // most stages of packed weights / of tokens and decoded weights
-constexpr int X_LIST = 256;                       // units of the grouped form that are kept in shared memory
+constexpr int A_COLS = MX_COLS / 4;               // tensor-memory columns of a stage's weights, then of their scales
+constexpr int SFA_COLS = 4;
+constexpr int MAX_W = 16, MAX_R = 8;              // most stages of packed weights / of rows and decoded weights
+constexpr int LIST = 512;                         // units of the grouped form that are kept in shared memory
 constexpr int OUT_TOKENS = 16;
-constexpr int OUT_BYTES = OUT_TOKENS * XBM * 4;   // a staged box of the output
-constexpr int CONTROL = 512 + 4 * X_LIST;         // barriers and flags, the list
+constexpr int OUT_BYTES = OUT_TOKENS * MX_ROWS * 4;       // a staged box of the output
+constexpr int CONTROL = 512 + 4 * LIST;           // barriers and flags, the list
+constexpr int NARROW_TOKENS = 32, WIDE_TOKENS = 128;      // most tokens of a tile of either form
+constexpr int SIDE_BY_SIDE = 64;                  // most tokens whose two parts are one operand
+constexpr int ATOM = 512;                         // scales of 128 rows for a stage, as tcgen05.cp brings them to tensor memory
+constexpr int EPI = 256;                          // threads of the epilogue
+constexpr int TMEM = 512, SMEM = 227 * 1024;
 
-// The narrow form (up to 32 tokens: decoding) leaves room for two CTAs an SM, so that one kernel's first weights are on their way
-// while the kernel before it drains; the wide form has the SM to itself and sends its output through shared memory.
-template <bool WIDE> struct Form {
-    static constexpr int EPI_WARPS = WIDE ? 8 : 4;
-    static constexpr int THREADS = 32 * (12 + EPI_WARPS);
-    static constexpr int MOST_TOKENS = WIDE ? 192 : 32;
-    static constexpr int TMEM = WIDE ? 512 : 256;
-    static constexpr int SMEM = WIDE ? 227 * 1024 : 113 * 1024;
+// TOK: most tokens of a tile.  R stages of rows and decoded weights, GROUPS of four decoding warps: a stage is 1,500 cycles on its way
+// from the first look at its weights to the end of its MMAs, of which a group works on it for half, so that it takes
+// four groups and eight stages to keep up with memory where the MMAs are short.
+template <int TOK> struct Form {
+    static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow form cuts the line of tiles, and stores directly)
+    static constexpr int R = TOK <= NARROW_TOKENS ? 8 : 4;
+    static constexpr int GROUPS = TOK <= NARROW_TOKENS ? 4 : 3;
+    static constexpr int EPI_WARP = 4 + 4 * GROUPS, THREADS = 32 * EPI_WARP + EPI;
+    static constexpr int ATOMS = TOK <= SIDE_BY_SIDE ? 1 : 2 * ((TOK + 127) / 128);
+    static constexpr int ACC_COLS = TOK <= SIDE_BY_SIDE ? 2 * TOK : TOK;
+    static constexpr int RING_COLS = (A_COLS + SFA_COLS + 4 * ATOMS + 7) / 8 * 8;      // [weights | their scales | the rows' scales]
+    static constexpr int STAGE_BYTES = (TOK * 256 + ATOMS * ATOM + 1023) / 1024 * 1024;
     static constexpr int OUT = WIDE ? 4 * OUT_BYTES : 0;
-    static constexpr int RING = SMEM - 1024 - CONTROL - OUT;          // for both rings of stages
+    static constexpr int RING = SMEM - 1024 - CONTROL - OUT;             // for the rings of stages
+    static constexpr int FIT = (RING - R * STAGE_BYTES) / MX_TILE_BYTES;
+    static constexpr int WS = FIT < MAX_W ? FIT : MAX_W;
+    static_assert(2 * ACC_COLS + R * RING_COLS <= TMEM, "tensor memory");
+    static_assert(GROUPS <= R && WS >= GROUPS + R, "a wait names a phase by its parity: see the decoding warps");
 };
 
 struct MxArgs {
     const uint8_t* W; long w_group; const int* shifts;    // tiles, bytes of one group's, what each group's results are raised by
+    MxRows rows;                                          // what X's parts, which come by map_x, are made from
+    const uint8_t* x_scales; long scale_rows;             // their scales
     void* out; long ldo, slab_stride;
-    int o_bf16, accumulate, boxed;
-    float* partials; int* counters;
-    int M, N, K, kb, bn, acc_cols, tiles_m, tiles_n, splits, n_units, ws, ring;
+    int o_bf16, accumulate, boxed, slabs;
+    float* partials; int* counters; int max_segments;
+    int M, N, K, kb, bn, atoms, tiles_m, tiles_n, splits;
+    long items;                                           // narrow, not grouped: tiles_n * kb; wide, not grouped: units
     const int* tile_group; int tile, n_tiles;
     FbGate gate; int plain_act;
     int* status;
 };
 
-struct MxUnit { int m0, n_tok, nt, group, split, kb0, n_kb, id; };
+// What a CTA works on at a time: a row tile of a group's matrix, tiles kb0 .. kb0 + n_kb along K, over n_tok rows from m0 on.
+struct Unit { int m0, n_tok, nt, group, kb0, n_kb, share, shares, id; };
+
+__device__ __forceinline__ void mma_mx(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], [%1], %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+}
+// e4m3 x e4m3 -> f32 under E8M0 scales, M = 128; the k-th block of 32 of a stage takes byte k of the scales' words.
+__device__ __forceinline__ uint32_t mx_idesc(int n) { return ((uint32_t)(n >> 3) << 17) | (1u << 23) | (8u << 24); }
+__device__ __forceinline__ constexpr uint32_t mx_block(int k) { return ((uint32_t)k << 4) | ((uint32_t)k << 29); }
+// 512 bytes of scales, [lane i][j] words of row 32 j + i, into four columns, the same in every quarter of the lanes; in order with the
+// MMAs of the same thread.
+__device__ __forceinline__ uint64_t scales_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)8 << 16 | (uint64_t)8 << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint4& v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// mbar_wait whose tries may sleep for long: twenty warps that ask again and again take issue slots from those that work.
+__device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, int* status) {
+    constexpr uint32_t HINT_NS = 1000000;
+    unsigned long long t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(bar), "r"(parity), "r"(HINT_NS) : "memory");
+        if (ok) return true;
+        if (t0 == 0) t0 = global_ns();
+        else if (global_ns() - t0 > FB_WAIT_LIMIT_NS) {
+            atomicOr(status, FB_STATUS_WAIT_TIMEOUT);
+            return false;
+        }
+    }
+}
 
 __device__ __forceinline__ void store_box(const void* map, uint32_t src, int x, int y, int z, bool add) {
     if (add)
@@ -69,88 +137,118 @@ __device__ __forceinline__ void store_box(const void* map, uint32_t src, int x, 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-template <bool WIDE>
-__global__ void __launch_bounds__(Form<WIDE>::THREADS, WIDE ? 1 : 2)
+// g sigmoid(g) u by the approximate exponential and reciprocal (relative errors of 2^-22 and 2^-23; the exponential's argument is
+// rounded to 2^-24 of itself): within 3e-7 (2 + |g|) of the result.  The exact ones made the epilogue of 160 tokens longer than the
+// products of K = 4,096.
+__device__ __forceinline__ float silu_times(float g, float u) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * g));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));          // (e = inf: 0)
+    return g * r * u;
+}
+
+template <int TOK, bool GROUPED>
+__global__ void __launch_bounds__(Form<TOK>::THREADS, 1)
 gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_o,
                   const __grid_constant__ MxArgs a) {
-    using F = Form<WIDE>;
-    constexpr int EPI = 32 * F::EPI_WARPS;
+    using F = Form<TOK>;
+    constexpr bool WIDE = F::WIDE;
+    constexpr int WS = F::WS, R = F::R, G = F::GROUPS, EPI_WARP = F::EPI_WARP;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const int WS = a.ws, R = a.ring;
-    const uint32_t atom_bytes = (uint32_t)a.bn * 128, x_bytes = 2 * atom_bytes;
-    uint8_t* w_base = smem + (size_t)R * x_bytes;                        // [token stages | weight stages | output boxes | control]
+    uint8_t* w_base = smem + R * F::STAGE_BYTES;                         // [stages of rows | weight stages | output boxes | control]
     uint8_t* out_stage = smem + F::RING;
     uint64_t* bars = (uint64_t*)(out_stage + F::OUT);
-    uint64_t *w_full = bars, *w_empty = w_full + MAX_W, *full = w_empty + MAX_W, *done = full + MAX_R, *acc_full = done + MAX_R,
-             *acc_empty = acc_full + 2;
+    uint64_t *w_full = bars, *w_empty = w_full + MAX_W, *x_full = w_empty + MAX_W, *full = x_full + MAX_R, *done = full + MAX_R,
+             *acc_full = done + MAX_R, *acc_empty = acc_full + 2;
     uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
     int* flag = (int*)(tmem_slot + 1);           // what the epilogue decided together
     int* bail = flag + 1;                        // a bounded wait ran out somewhere in this CTA
     int* unit_count = bail + 1;
     uint32_t* list = (uint32_t*)((uint8_t*)bars + 512);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(smem_u32(bar), parity, a.status); };
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_long(smem_u32(bar), parity, a.status); };
     auto bailed = [&]() { return *(volatile int*)bail != 0; };
-    const bool grouped = a.tile_group != nullptr;
-    const int most = grouped ? a.bn / a.tile : 1;
+    const int most = GROUPED ? a.bn / a.tile : 1;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MAX_W; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 128); }
-        for (int s = 0; s < MAX_R; ++s) { mbar_init(smem_u32(&full[s]), 129); mbar_init(smem_u32(&done[s]), 1); }
+        for (int s = 0; s < MAX_W; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4); }
+        for (int s = 0; s < R; ++s) {
+            mbar_init(smem_u32(&x_full[s]), 1);
+            mbar_init(smem_u32(&full[s]), 4);
+            mbar_init(smem_u32(&done[s]), 1);
+        }
         for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&acc_full[s]), 1); mbar_init(smem_u32(&acc_empty[s]), EPI); }
         *bail = 0;
         mbar_fence_init();
     }
-    if (warp == 3) tmem_alloc(tmem_slot, F::TMEM);
+    if (warp == 3) tmem_alloc(tmem_slot, TMEM);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     fb_pdl_launch_dependents();                  // (behind the allocation: see umma.cuh)
-    const uint32_t tmem = *tmem_slot;
-    int n_units = a.n_units, stride = gridDim.x;
-    if (grouped) {
-        if (warp == 12) {
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const uint32_t ring = tmem + 2 * F::ACC_COLS;
+
+    // The CTA's part of the work: items first .. last of the line.  Narrow, not grouped: an item is a tile along K of a row tile; else a
+    // unit, and the CTAs take turns.
+    constexpr bool LINE = !WIDE && !GROUPED;
+    long first = blockIdx.x, last = a.items;
+    if constexpr (GROUPED) {
+        if (warp == EPI_WARP) {
             fb_pdl_wait();                       // which weights a tile wants is the work of the kernels before this one
-            const int found = group_units<X_LIST>(a.tile_group, a.n_tiles, most, list);
+            const int found = group_units<LIST>(a.tile_group, a.n_tiles, most, list);
             if (lane == 0) *unit_count = found;
         }
         __syncthreads();
-        n_units = *unit_count * a.tiles_n;
+        last = (long)*unit_count * a.tiles_n;
+    } else if constexpr (LINE) {
+        first = blockIdx.x * a.items / gridDim.x;
+        last = (blockIdx.x + 1) * a.items / gridDim.x;
     }
     GroupWalk walk = {0, 0u};
-    auto unit_of = [&](int u) {
-        MxUnit w;
-        if (grouped) {                           // feature tiles vary fastest: the CTAs that run together share few units' rows
-            const int i = u / a.tiles_n;
-            const uint32_t unit = group_unit<X_LIST>(a.tile_group, a.n_tiles, most, list, i, walk);
-            const int t = (int)(unit & 0xffffffu);
+    auto unit_at = [&](long item) {              // (asked for ascending items only)
+        Unit w;
+        if constexpr (GROUPED) {                 // feature tiles vary fastest: the CTAs that run together share few units' rows
+            const int i = (int)(item / a.tiles_n);
+            const uint32_t entry = group_unit<LIST>(a.tile_group, a.n_tiles, most, list, i, walk);
+            const int t = (int)(entry & 0xffffffu);
             w.m0 = t * a.tile;
-            w.n_tok = (int)(unit >> 24) * a.tile;
+            w.n_tok = (int)(entry >> 24) * a.tile;
             w.group = a.tile_group[t];
-            w.nt = u - i * a.tiles_n;
-            w.id = 0; w.split = 0; w.kb0 = 0; w.n_kb = a.kb;
-        } else {                                 // token tiles vary fastest: the CTAs that run together share weight tiles
-            const int tiles = a.tiles_m * a.tiles_n;
-            w.split = u / tiles;
-            w.id = u - w.split * tiles;
+            w.nt = (int)(item - (long)i * a.tiles_n);
+            w.kb0 = 0; w.n_kb = a.kb; w.share = 0; w.shares = 1; w.id = 0;
+        } else if constexpr (WIDE) {             // token tiles vary fastest: the CTAs that run together share weight tiles
+            const long tiles = (long)a.tiles_m * a.tiles_n;
+            w.share = (int)(item / tiles);
+            w.shares = a.splits;
+            w.id = (int)(item - w.share * tiles);
             w.m0 = w.id % a.tiles_m * a.bn;
             w.nt = w.id / a.tiles_m;
             w.n_tok = a.bn;
             w.group = 0;
-            w.kb0 = (int)((long)w.split * a.kb / a.splits);
-            w.n_kb = (int)((long)(w.split + 1) * a.kb / a.splits) - w.kb0;
+            w.kb0 = (int)((long)w.share * a.kb / a.splits);
+            w.n_kb = (int)((long)(w.share + 1) * a.kb / a.splits) - w.kb0;
+        } else {
+            w.nt = (int)(item / a.kb);
+            w.kb0 = (int)(item - (long)w.nt * a.kb);
+            w.n_kb = (int)(last - item < a.kb - w.kb0 ? last - item : a.kb - w.kb0);
+            w.m0 = 0; w.n_tok = a.bn; w.group = 0; w.id = w.nt;
+            const long from = (long)w.nt * a.kb, begin = ((from + 1) * gridDim.x - 1) / a.items;
+            w.share = (int)(blockIdx.x - begin);
+            w.shares = (int)(((from + a.kb) * gridDim.x - 1) / a.items - begin) + 1;
         }
         return w;
     };
+    auto after = [&](long item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
 
     if (warp == 0) {
         // ---------------- weights: no other kernel writes them, so they are requested at once ----------------
         if (elect_one()) {
             int s = 0;
             uint32_t phase = 1;
-            for (int u = blockIdx.x; u < n_units && !bailed(); u += stride) {
-                const MxUnit w = unit_of(u);
+            for (long u = first; u < last && !bailed();) {
+                const Unit w = unit_at(u);
                 const uint8_t* src = a.W + (size_t)w.group * a.w_group + ((size_t)w.nt * a.kb + w.kb0) * MX_TILE_BYTES;
                 for (int i = 0; i < w.n_kb; ++i, src += MX_TILE_BYTES) {
                     if (!wait(&w_empty[s], phase)) { *bail = 1; break; }
@@ -158,168 +256,246 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES), src, MX_TILE_BYTES, smem_u32(&w_full[s]));
                     if (++s == WS) { s = 0; phase ^= 1u; }
                 }
+                u = after(u, w);
             }
         }
         __syncwarp();
     } else if (warp == 2) {
-        // ---------------- tokens ----------------
+        // ---------------- the rows' parts and their scales ----------------
         if (elect_one()) {
             fb_pdl_wait();
             int s = 0;
             uint32_t phase = 1;
-            for (int u = blockIdx.x; u < n_units && !bailed(); u += stride) {
-                const MxUnit w = unit_of(u);
-                const int boxes = grouped ? w.n_tok / a.tile : 1, box = grouped ? a.tile : a.bn;
+            for (long u = first; u < last && !bailed();) {
+                const Unit w = unit_at(u);
+                const int boxes = GROUPED ? w.n_tok / a.tile : 1, box = GROUPED ? a.tile : a.bn;
                 for (int i = 0; i < w.n_kb; ++i) {
                     if (!wait(&done[s], phase)) { *bail = 1; break; }
-                    mbar_expect_tx(smem_u32(&full[s]), (uint32_t)w.n_tok * 256);
-                    const uint32_t dst = smem_u32(smem) + (uint32_t)s * x_bytes;
+                    const uint32_t bar = smem_u32(&x_full[s]), dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES);
+                    const uint32_t scale_bytes = GROUPED ? (uint32_t)w.n_tok * 4 : (uint32_t)a.atoms * ATOM;
+                    mbar_expect_tx(bar, (uint32_t)w.n_tok * 2 * 128 + scale_bytes);
                     for (int b = 0; b < boxes; ++b) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)          // (rows beyond M and columns beyond K arrive as zeros)
-                            tma_load_2d(dst + h * atom_bytes + (uint32_t)(b * box) * 128, &map_x, smem_u32(&full[s]),
-                                        (w.kb0 + i) * XBK + h * 64, w.m0 + b * box);
+                        for (int p = 0; p < 2; ++p)          // (rows beyond M are the other part's, or zeros: nobody stores them)
+                            tma_load_2d(dst + (uint32_t)(p * w.n_tok + b * box) * 128, &map_x, bar, (w.kb0 + i) * 64, p * a.M + w.m0 + b * box);
                     }
+                    const size_t at = GROUPED ? ((size_t)(w.kb0 + i) * a.scale_rows + w.m0) * 4
+                                              : ((size_t)(w.kb0 + i) * a.tiles_m + w.m0 / a.bn) * (a.atoms * ATOM);
+                    bulk_copy_g2s(dst + TOK * 256, a.x_scales + at, scale_bytes, bar);
                     if (++s == R) { s = 0; phase ^= 1u; }
                 }
+                u = after(u, w);
             }
         }
         __syncwarp();
     } else if (warp == 1) {
         // ---------------- MMA ----------------
+        // (What an instruction's operands are made of is brought to uniform registers first.  Where a stage's place in the ring is counted
+        // out, that takes 300 cycles a stage of four instructions; with four places as constants it is done once, and a stage
+        // takes 140 with its wait and commit, 57 to 260 of them MMAs.)
         if (elect_one()) {
             int s = 0, j = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < n_units && ok && !bailed(); u += stride, ++j) {
-                const MxUnit w = unit_of(u);
-                const uint32_t idesc = umma_idesc(w.n_tok);
+            const uint32_t x_base = smem_u32(smem), full_base = smem_u32(full), done_base = smem_u32(done);
+            const uint64_t desc = umma_desc(x_base), desc_scales = scales_desc(x_base + TOK * 256);
+            for (long u = first; u < last && ok && !bailed(); ++j) {
+                const Unit w = unit_at(u);
+                const bool both = w.n_tok <= SIDE_BY_SIDE;               // both parts in one operand
                 const int b = j & 1;
+                const uint32_t idesc = mx_idesc(both ? 2 * w.n_tok : w.n_tok), second = (uint32_t)w.n_tok * 8;      // (128 bytes, in sixteens)
+                const uint32_t sfb_second = (uint32_t)(w.n_tok + 127) / 128 * 4;
                 ok = wait(&acc_empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u);        // (the epilogue has drained it, two units ago)
                 if (!ok) break;
                 tmem_fence_after();
-                const uint32_t d = tmem + (uint32_t)(b * a.acc_cols);
-                for (int i = 0; i < w.n_kb; ++i) {
-                    ok = wait(&full[s], phase);
-                    if (!ok) break;
+                const uint32_t d = tmem + (uint32_t)(b * F::ACC_COLS);
+                auto stage = [&](int at, bool fresh) {                   // the stage in place `at` of the ring
+                    if (!wait_long(full_base + 8 * at, phase, a.status)) return false;
                     tmem_fence_after();
-                    const uint32_t A = tmem + (uint32_t)(2 * a.acc_cols + s * A_COLS);
-                    const uint64_t x = umma_desc(smem_u32(smem) + (uint32_t)s * x_bytes);
+                    const uint32_t A = ring + (uint32_t)(at * F::RING_COLS), sfb = A + A_COLS + SFA_COLS;
+                    const uint64_t x = desc + (uint64_t)(at * (F::STAGE_BYTES / 16));
+                    if constexpr (!GROUPED) {
 #pragma unroll
-                    for (int k = 0; k < XBK / UMMA_K; ++k)
-                        umma_bf16_ts(d, A + (uint32_t)(k * (UMMA_K / 2)), x + (uint64_t)((k >> 2) * (atom_bytes >> 4) + (k & 3) * 2),
-                                     idesc, (i > 0 || k > 0) ? 1u : 0u);
-                    umma_commit(smem_u32(&done[s]));
-                    if (++s == R) { s = 0; phase ^= 1u; }
+                        for (int t = 0; t < F::ATOMS; ++t)
+                            if (t == 0 || t < a.atoms) copy_scales(sfb + 4 * t, desc_scales + (uint64_t)((at * F::STAGE_BYTES + t * ATOM) / 16));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_mx(d, A + 8 * k, x + 2 * k, idesc + mx_block(k), A + A_COLS, sfb, fresh && k == 0 ? 0u : 1u);
+                    if (TOK > SIDE_BY_SIDE && !both) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma_mx(d, A + 8 * k, x + second + 2 * k, idesc + mx_block(k), A + A_COLS, sfb + sfb_second, 1u);
+                    }
+                    umma_commit(done_base + 8 * at);
+                    return true;
+                };
+                for (int i = 0; i < w.n_kb && ok;) {
+                    static_assert(R == 4 || R == 8, "blocks of four places");
+                    if (s == 0 && i + 4 <= w.n_kb) {
+                        ok = stage(0, i == 0) && stage(1, false) && stage(2, false) && stage(3, false);
+                        s = 4; i += 4;
+                    } else if (R == 8 && s == 4 && i + 4 <= w.n_kb) {
+                        ok = stage(4, i == 0) && stage(5, false) && stage(6, false) && stage(7, false);
+                        s = 8; i += 4;
+                    } else {
+                        ok = stage(s, i == 0);
+                        ++s; ++i;
+                    }
+                    if (s == R) { s = 0; phase ^= 1u; }
                 }
                 if (ok) umma_commit(smem_u32(&acc_full[b]));
+                u = after(u, w);
             }
             if (!ok) *bail = 1;
         }
         __syncwarp();
-    } else if (warp >= 4 && warp < 12) {
-        // ---------------- decode: a thread a feature; the group's stages are it = ab, ab + 2, ... ----------------
-        // (A wait names a phase by its parity alone.  A group comes to a slot of the rings at every second turn or at every one; it
-        // cannot be two turns off: it has seen the MMAs of stage it - 2 - R done, and so every earlier stage decoded, and WS > R + 2.)
-        const int quarter = warp & 3, row = quarter * 32 + lane, ab = (warp - 4) >> 2;
-        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(2 * a.acc_cols);
-        uint32_t it = 0, w_phase = 0, r_phase = 1;
-        int ws = 0, r = 0;
+    } else if (warp >= 4 && warp < EPI_WARP) {
+        // ---------------- decode: a thread a feature; the group's stages are it = group, group + G, ... ----------------
+        // (A wait names a phase by its parity alone, and a group does not come to every slot in every round of a ring.  It has seen the
+        // MMAs of stage it - G - R done, so with G <= R no slot of that ring is two rounds behind, and with WS >= G + R none
+        // of the weights'; x_full is looked at behind done, by which the round before it has arrived.)
+        const int quarter = warp & 3, row = quarter * 32 + lane, group = (warp - 4) >> 2;
+        const uint32_t lanes = ring + ((uint32_t)(quarter * 32) << 16);
+        int ws = group, r = group;
+        uint32_t w_phase = 0, r_phase = 0, it = 0;       // it: stages ahead of the unit, modulo G
         bool ok = true;
-        for (int u = blockIdx.x; u < n_units && ok && !bailed(); u += stride) {
-            const int n = unit_of(u).n_kb;
-            for (int i = 0; i < n; ++i, ++it) {
-                if ((int)(it & 1u) == ab) {
-                    ok = wait(&w_full[ws], w_phase);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    const uint8_t* src = w_base + (size_t)ws * MX_TILE_BYTES;
-                    const uint32_t scales = *reinterpret_cast<const uint32_t*>(src + MX_CODE_BYTES + row * 4);
-                    uint4 c[4];
+        for (long u = first; u < last && ok && !bailed();) {
+            const Unit w = unit_at(u);
+            int i = group - (int)it;                                     // the group's first stage of the unit
+            if (i < 0) i += G;
+            for (; i < w.n_kb; i += G) {
+                ok = wait(&w_full[ws], w_phase);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                const uint8_t* src = w_base + (size_t)ws * MX_TILE_BYTES;
+                const uint4 scales = *reinterpret_cast<const uint4*>(src + MX_CODE_BYTES + lane * 16);
+                uint4 c[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) c[q] = *reinterpret_cast<const uint4*>(src + (q * MX_ROWS + row) * 16);
-                    ok = wait(&done[r], r_phase);                        // the MMAs that read this buffer are done
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    tmem_fence_after();
-                    const uint32_t dst = lanes + (uint32_t)(r * A_COLS);
+                for (int q = 0; q < 4; ++q) c[q] = *reinterpret_cast<const uint4*>(src + (q * MX_ROWS + row) * 16);
+                ok = wait(&done[r], r_phase ^ 1u);                   // the MMAs that read this buffer are done
+                if (ok) ok = wait(&x_full[r], r_phase);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tmem_fence_after();
+                const uint32_t dst = lanes + (uint32_t)(r * F::RING_COLS);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const uint32_t scale = mx_scale(scales >> (8 * q) & 255u);
-                        uint32_t v[16];
-                        mx_decode(c[q].x, scale, v);
-                        mx_decode(c[q].y, scale, v + 4);
-                        mx_decode(c[q].z, scale, v + 8);
-                        mx_decode(c[q].w, scale, v + 12);
-                        tmem_st16(dst + (uint32_t)(q * 16), v);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v[16];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t in[4] = {c[2 * h + q].x, c[2 * h + q].y, c[2 * h + q].z, c[2 * h + q].w};
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) mx_decode(in[p], v[8 * q + 2 * p], v[8 * q + 2 * p + 1]);
                     }
-                    // (behind the stores, which need every number of the row: see gemm_f32_tc.cu)
-                    mbar_arrive(smem_u32(&w_empty[ws]));
-                    tmem_wait_st();
-                    tmem_fence_before();
-                    mbar_arrive(smem_u32(&full[r]));
+                    tmem_st16(dst + 16 * h, v);
                 }
-                if (++ws == WS) { ws = 0; w_phase ^= 1u; }
-                if (++r == R) { r = 0; r_phase ^= 1u; }
+                tmem_st4(dst + A_COLS, scales);
+                if (GROUPED) {                                       // the rows' scales: lane l of word j has row 32 j + l
+                    const uint32_t* sx = reinterpret_cast<const uint32_t*>(smem + r * F::STAGE_BYTES + TOK * 256);
+                    const uint32_t sfb = dst + A_COLS + SFA_COLS;
+                    auto word = [&](int q) { return q < w.n_tok ? sx[q] : 0u; };
+                    if (w.n_tok <= SIDE_BY_SIDE) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int q = j * 32 + lane;
+                            v[j] = q < w.n_tok ? sx[q] : mx_second_scales(word(q - w.n_tok));
+                        }
+                        tmem_st4(sfb, make_uint4(v[0], v[1], v[2], v[3]));
+                    } else {
+                        const int second = (w.n_tok + 127) / 128 * 4;
+                        for (int j = 0; j < second; j += 4) {
+                            uint32_t v[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) v[q] = word((j + q) * 32 + lane);
+                            tmem_st4(sfb + j, make_uint4(v[0], v[1], v[2], v[3]));
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) v[q] = mx_second_scales(v[q]);
+                            tmem_st4(sfb + second + j, make_uint4(v[0], v[1], v[2], v[3]));
+                        }
+                    }
+                }
+                // (behind the stores, which need every number of the row: see gemm_f32_tc.cu)
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&w_empty[ws]));
+                tmem_wait_st();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&full[r]));
+                if ((ws += G) >= WS) { ws -= WS; w_phase ^= 1u; }
+                if ((r += G) >= R) { r -= R; r_phase ^= 1u; }
             }
+            it = (it + (uint32_t)w.n_kb) % G;
+            u = after(u, w);
         }
         if (!ok) *bail = 1;
-    } else if (warp >= 12) {
-        // ---------------- epilogue: lanes are features ----------------
+    } else if (warp >= EPI_WARP) {
+        // ---------------- epilogue: lanes are features, the two groups of four warps take 16 tokens in turn ----------------
         fb_pdl_wait();
-        const int quarter = warp & 3, half = (warp - 12) >> 2, row = quarter * 32 + lane;
+        const int quarter = warp & 3, half = (warp - EPI_WARP) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 32 * EPI_WARP;
         const bool leader = quarter == 0 && lane == 0;
-        constexpr int STEP = OUT_TOKENS * (F::EPI_WARPS / 4);
-        const bool join = a.splits > 1 && a.slab_stride == 0;
+        constexpr int STEP = OUT_TOKENS * 2;
         uint32_t boxes = 0;                      // boxes this group of warps has staged: the buffers take turns
         int j = 0;
-        for (int u = blockIdx.x; u < n_units; u += stride, ++j) {
-            const MxUnit w = unit_of(u);
-            const int b = j & 1, n0 = w.nt * XBM, n = n0 + row;
+        for (long u = first; u < last; ++j) {
+            const Unit w = unit_at(u);
+            const bool both = w.n_tok <= SIDE_BY_SIDE, join = !GROUPED && w.shares > 1 && a.slabs == 0;
+            const int b = j & 1, n0 = w.nt * MX_ROWS, n = n0 + row;
             const int rows = min(w.n_tok, a.M - w.m0);                   // (grouped: whole tiles)
             const float* from = nullptr;                                 // where shares are joined: the first one of this tile
             if (bailed() || !wait(&acc_full[b], (uint32_t)(j >> 1) & 1u)) *bail = 1;
             asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
-            if (threadIdx.x == 12 * 32) *flag = bailed() ? 2 : 0;        // one thread decides for all: they meet at barriers below
+            if (tid == 0) *flag = bailed() ? 2 : 0;                      // one thread decides for all: they meet at barriers below
             asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
             if (*flag == 2) break;
             tmem_fence_after();
-            const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * a.acc_cols);
+            const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * F::ACC_COLS);
+            auto sums = [&](int c, float (&v)[16]) {
+                tmem_ld16(acc + (uint32_t)c, v);
+                if (both) {
+                    float second[16];
+                    tmem_ld16(acc + (uint32_t)(w.n_tok + c), second);
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) v[q] += second[q];
+                }
+            };
             if (join) {
-                float* mine = a.partials + ((size_t)w.id * a.splits + w.split) * (size_t)(a.bn * XBM) + row;
+                float* mine = a.partials + ((size_t)w.id * a.max_segments + w.share) * (size_t)(a.bn * MX_ROWS) + row;
                 for (int c = half * OUT_TOKENS; c < rows; c += STEP) {
                     float v[16];
-                    tmem_ld16(acc + (uint32_t)c, v);
+                    sums(c, v);
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) mine[(size_t)(c + q) * XBM] = v[q];
+                    for (int q = 0; q < 16; ++q)
+                        if (c + q < rows) mine[(size_t)(c + q) * MX_ROWS] = v[q];
                 }
                 __threadfence();
                 asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
-                if (threadIdx.x == 12 * 32) {
-                    const bool last = atomicAdd(&a.counters[w.id], 1) == a.splits - 1;
-                    if (last) a.counters[w.id] = 0;                      // ready for the next launch
-                    *flag = last;
+                if (tid == 0) {
+                    const bool is_last = atomicAdd(&a.counters[w.id], 1) == w.shares - 1;
+                    if (is_last) a.counters[w.id] = 0;                   // ready for the next launch
+                    *flag = is_last;
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
                 if (*flag == 1) {
                     __threadfence();
-                    from = a.partials + (size_t)w.id * a.splits * (size_t)(a.bn * XBM) + row;
+                    from = a.partials + (size_t)w.id * a.max_segments * (size_t)(a.bn * MX_ROWS) + row;
                 }
             }
             if (!join || from) {
                 const int shift = a.shifts[w.group];
                 const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
+                const int slab = a.slabs ? w.share : 0;
 #pragma unroll 1
                 for (int c = half * OUT_TOKENS; c < rows; c += STEP) {
                     float v[16];
                     if (from) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) v[q] = 0.0f;
-                        for (int s = 0; s < a.splits; ++s) {
-                            const float* p = from + ((size_t)s * a.bn + c) * XBM;
+                        for (int s = 0; s < w.shares; ++s) {
+                            const float* p = from + ((size_t)s * a.bn + c) * MX_ROWS;
 #pragma unroll
-                            for (int q = 0; q < 16; ++q) v[q] += __ldcg(p + q * XBM);
+                            for (int q = 0; q < 16; ++q)
+                                if (c + q < rows) v[q] += __ldcg(p + q * MX_ROWS);
                         }
                     } else {
-                        tmem_ld16(acc + (uint32_t)c, v);
+                        sums(c, v);
                     }
                     if (shift > 0) {
 #pragma unroll
@@ -331,15 +507,20 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     }
                     // gated: features alternate gate, up; the even lane has act(gate) * up of column n / 2
                     bool writes = n < a.N;
-                    int col = n, width = XBM, at = row;
+                    int col = n, width = MX_ROWS, at = row;
                     if (a.gate.act) {
+                        float up[16];
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            const float up = __shfl_xor_sync(0xffffffffu, v[q], 1);
-                            v[q] = fb_gate_times(a.gate, v[q], up);
+                        for (int q = 0; q < 16; ++q) up[q] = __shfl_xor_sync(0xffffffffu, v[q], 1);
+                        if (a.gate.act == FB_ACT_SILU) {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) v[q] = silu_times(v[q], up[q]);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) v[q] = fb_gate_times(a.gate, v[q], up[q]);
                         }
                         writes = !(lane & 1) && n + 1 < a.N;
-                        col = n >> 1; width = XBM / 2; at = row >> 1;
+                        col = n >> 1; width = MX_ROWS / 2; at = row >> 1;
                     }
                     if (WIDE && a.boxed) {
                         // the values go to shared memory as [token][feature], and one thread sends the box on its way (what lies
@@ -359,25 +540,31 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
-                        if (leader) store_box(&map_o, smem_u32(box), a.gate.act ? n0 / 2 : n0, w.m0 + c, join ? 0 : w.split, a.accumulate != 0);
+                        if (leader) store_box(&map_o, smem_u32(box), a.gate.act ? n0 / 2 : n0, w.m0 + c, slab, a.accumulate != 0);
                     } else if (writes) {
-                        const size_t first = (size_t)w.split * a.slab_stride + (size_t)(w.m0 + c) * a.ldo + col;
+                        const size_t begin = (size_t)slab * a.slab_stride + (size_t)(w.m0 + c) * a.ldo + col;
                         if (a.o_bf16) {
-                            __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + first;
+                            __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + begin;
 #pragma unroll
                             for (int q = 0; q < 16; ++q)
                                 if (c + q < rows) p[(size_t)q * a.ldo] = __float2bfloat16_rn(v[q]);
                         } else {
-                            float* p = reinterpret_cast<float*>(a.out) + first;
+                            float* p = reinterpret_cast<float*>(a.out) + begin;
 #pragma unroll
                             for (int q = 0; q < 16; ++q)
                                 if (c + q < rows) p[(size_t)q * a.ldo] = a.accumulate ? p[(size_t)q * a.ldo] + v[q] : v[q];
+                            if (!WIDE && a.slabs && w.share == w.shares - 1)         // shares that this row tile does not have
+                                for (int s = w.shares; s < a.slabs; ++s) {
+                                    p += a.slab_stride;
+                                    for (int q = 0; q < 16 && c + q < rows; ++q) p[(size_t)q * a.ldo] = 0.0f;
+                                }
                         }
                     }
                 }
             }
             tmem_fence_before();
             mbar_arrive(smem_u32(&acc_empty[b]));
+            u = after(u, w);
         }
         if (WIDE && leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");        // the boxes it sent are in memory
     }
@@ -385,33 +572,62 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     __syncthreads();
     if (warp == 3) {
         tmem_fence_after();
-        tmem_dealloc(tmem, F::TMEM);
+        tmem_dealloc(tmem, TMEM);
     }
 }
 
-struct MxPlan { int bn, splits; bool wide; };
+// ---- narrow: how the line of tiles is cut ----
+int segments_of(long tiles_n, long kb, long grid) {           // the most stretches that a row tile is cut into
+    const long items = tiles_n * kb;
+    long most = 1;
+    for (long nt = 0; nt < tiles_n; ++nt) {
+        const long first = ((nt * kb + 1) * grid - 1) / items, last = ((nt * kb + kb) * grid - 1) / items;
+        if (last - first + 1 > most) most = last - first + 1;
+    }
+    return (int)most;
+}
+// CTAs, one an SM, each with a few tiles at least, and the most stretches that they cut a row tile into: as many CTAs as leave no
+// more than `limit`.
+constexpr int ANY = 1 << 30, LEAST_ITEMS = 4;
+struct Cut { int grid, segments; };
+Cut cut_of(int tiles_n, int kb, int limit) {
+    static std::map<std::tuple<int, int, int, int>, Cut> known;              // (counting through the tiles takes microseconds)
+    static std::mutex mu;
+    const std::tuple<int, int, int, int> key{tiles_n, kb, limit, fb_sm_count()};
+    std::lock_guard<std::mutex> lock(mu);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    const long most = ((long)tiles_n * kb + LEAST_ITEMS - 1) / LEAST_ITEMS, slots = fb_sm_count();
+    long grid = most < slots ? most : slots;
+    int segments = segments_of(tiles_n, kb, grid);
+    while (segments > limit && grid > 1) segments = segments_of(tiles_n, kb, --grid);
+    if (known.size() > 4096) known.clear();
+    return known[key] = Cut{(int)grid, segments};
+}
+int narrow_tokens(int M) { return (M + 7) / 8 * 8; }
 
-// Token tiles and shares of K: the cheapest of the choices in cycles of an SM.  A stage costs its MMAs (4 cycles a token) or its
+// ---- wide: token tiles and shares of K ----
+struct Plan { int bn, splits; };
+constexpr int MORE_TILES = 2;
+// The cheapest of the choices in cycles of an SM.  A stage costs its MMAs (2 cycles a column, at least 46 an instruction) or its
 // decoding, whichever is more; all CTAs together no less than the weights from HBM.  A share of K costs a copy of the output, written
 // and read.
-MxPlan plan_mxfp4(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
-    const long sms = fb_sm_count(), tiles_n = (N + XBM - 1) / XBM;
-    MxPlan best = {32, 1, false};
+Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
+    const long sms = fb_sm_count(), tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
+    Plan best = {WIDE_TOKENS, 1};
     double best_cost = 1e300;
-    const bool wide = M > Form<false>::MOST_TOKENS;
-    const int most = wide ? Form<true>::MOST_TOKENS : Form<false>::MOST_TOKENS;
-    const long least = (M + most - 1) / most, slots = wide ? sms : 2 * sms;
-    for (long tiles_m = least; tiles_m <= least + 2; ++tiles_m) {
+    const long least = (M + WIDE_TOKENS - 1) / WIDE_TOKENS;
+    for (long tiles_m = least; tiles_m <= least + MORE_TILES; ++tiles_m) {
         const int bn = (int)(((M + tiles_m - 1) / tiles_m + 15) / 16 * 16);
-        const double stage = fmax(wide ? 4.0 * bn + 60.0 : 0.0, wide ? 260.0 : 520.0);
+        const double stage = fmax(4.0 * bn + 60.0, 260.0);
         const long tiles = tiles_n * ((M + bn - 1) / bn);
         for (int splits = 1; splits <= max_splits && splits <= kb; ++splits) {
-            if (!slabs && splits > 1 && (tiles > n_counters || tiles * splits * bn * XBM > partial_floats)) break;
-            const long rounds = (tiles * splits + slots - 1) / slots;
+            if (!slabs && splits > 1 && (tiles > n_counters || tiles * splits * bn * MX_ROWS > partial_floats)) break;
+            const long rounds = (tiles * splits + sms - 1) / sms;
             double cost = fmax((double)rounds * ((kb + splits - 1) / splits * stage + 500.0),
                                (double)tiles_n * kb * MX_TILE_BYTES / (23.0 * sms));
             cost += (splits - 1) * (double)M * N * 8.0 / (24.0 * sms) + (splits > 1 && !slabs ? 1500.0 : 0.0);
-            if (cost < best_cost * (1.0 - 1e-9)) { best_cost = cost; best = MxPlan{bn, splits, wide}; }
+            if (cost < best_cost * (1.0 - 1e-9)) { best_cost = cost; best = Plan{bn, splits}; }
         }
     }
     return best;
@@ -420,42 +636,44 @@ MxPlan plan_mxfp4(long M, long N, int kb, int max_splits, long partial_floats, i
 constexpr long SHARE_FLOATS = 16L << 20;          // most that the shares of one product may take
 constexpr int MOST_SPLITS = 16;
 
-int launch_mxfp4(const MxPlan& plan, MxArgs a, const void* X, long lda, int box_rows, long n_units, cudaStream_t stream) {
-    a.bn = plan.bn;
-    // tensor memory: two accumulators and `ring` stages of decoded weights
-    const int tmem = plan.wide ? Form<true>::TMEM : Form<false>::TMEM;
-    a.acc_cols = (a.bn + 31) / 32 * 32;
-    a.ring = (tmem - 2 * a.acc_cols) / A_COLS < MAX_R ? (tmem - 2 * a.acc_cols) / A_COLS : MAX_R;
-    const int room = (plan.wide ? Form<true>::RING : Form<false>::RING) - a.ring * a.bn * 256;
-    a.ws = (room / MX_TILE_BYTES < MAX_W ? room / MX_TILE_BYTES : MAX_W) & ~1;
-    if (a.ring < 2 || a.ws < a.ring + 2) return fb_fail(-1, "gemm_mxfp4: no room for the stages of %d tokens", a.bn);
-    if (n_units > 2000000000L) return fb_fail(-1, "gemm_mxfp4: too many tiles (M=%d N=%d)", a.M, a.N);
-    a.n_units = (int)n_units;
-    CUtensorMap mx, mo = {};
-    int rc = fb_tensor_map_bf16(&mx, X, a.M, a.K, lda, 64, box_rows);
-    if (rc) return rc;
-    a.boxed = 0;
-    if (plan.wide) {
-        rc = fb_tensor_map_out(&mo, a.out, a.o_bf16 ? 2 : 4, a.M, a.gate.act ? a.N / 2 : a.N, a.ldo, a.slab_stride > 0 ? a.splits : 1,
-                               a.slab_stride, a.gate.act ? XBM / 2 : XBM, OUT_TOKENS);
-        if (rc < 0) return rc;
-        a.boxed = rc == 0;
-    }
+// Atoms of scales that a stage's rows have: of both parts side by side, or of either part.
+int atoms_of(int bn) { return bn <= SIDE_BY_SIDE ? 1 : 2 * ((bn + 127) / 128); }
+
+template <int TOK, bool GROUPED> int launch(const MxArgs& a, const CUtensorMap& mx, const CUtensorMap& mo, long grid, cudaStream_t stream) {
+    auto kernel = gemm_mxfp4_kernel<TOK, GROUPED>;
     static bool configured[FB_MAX_DEVICES] = {};
     if (fb_needs_setup(configured)) {
-        cudaError_t e = cudaFuncSetAttribute(gemm_mxfp4_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<false>::SMEM);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(gemm_mxfp4_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<true>::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return fb_fail(-2, "gemm_mxfp4: cannot reserve shared memory: %s", cudaGetErrorString(e));
         fb_setup_done(configured);
     }
-    const long slots = plan.wide ? fb_sm_count() : 2L * fb_sm_count();
-    const int grid = (int)(n_units < slots ? n_units : slots);
-    if (plan.wide)
-        fb_launch_class(FB_LAUNCH_GEMM_WIDE, gemm_mxfp4_kernel<true>, dim3(grid), dim3(Form<true>::THREADS), Form<true>::SMEM, stream, mx, mo, a);
-    else
-        fb_launch_class(FB_LAUNCH_OTHER, gemm_mxfp4_kernel<false>, dim3(grid), dim3(Form<false>::THREADS), Form<false>::SMEM, stream, mx, mo, a);
+    fb_launch_class(Form<TOK>::WIDE ? FB_LAUNCH_GEMM_WIDE : FB_LAUNCH_OTHER, kernel, dim3((unsigned)grid), dim3(Form<TOK>::THREADS), SMEM, stream, mx, mo, a);
     return fb_check_launch("gemm_mxfp4");
+}
+
+long long scale_bytes_of(int M, int kb, bool grouped) {
+    // grouped: a word a row; else atoms a token tile, of which there are at most MORE_TILES more than the rows need
+    return grouped ? 4LL * kb * ((M + 3) / 4 * 4) : (long long)kb * ((M + WIDE_TOKENS - 1) / WIDE_TOKENS + MORE_TILES) * 4 * ATOM;
+}
+
+// The rows' parts and scales in `scratch`, their map, the output's map.
+int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, long long scratch_bytes, int box_rows, cudaStream_t stream) {
+    const bool grouped = a.tile_group != nullptr;
+    const long Kp = (long)a.kb * MX_COLS, parts = 2L * a.M * Kp;
+    a.scale_rows = (a.M + 3) / 4 * 4;
+    FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= parts + scale_bytes_of(a.M, a.kb, grouped),
+               "gemm_mxfp4: scratch for the rows' parts missing");
+    a.x_scales = (const uint8_t*)scratch + parts;
+    a.atoms = atoms_of(a.bn);
+    const MxScaleLayout layout = {grouped ? 0 : a.bn, grouped ? 0 : a.atoms * ATOM, a.scale_rows};
+    int rc = fb_mxfp4_split_rows(a.rows, a.M, a.K, scratch, (uint8_t*)scratch + parts, layout, a.tile_group, a.tile, stream);
+    if (rc) return rc;
+    rc = fb_tensor_map_bf16(&mx, scratch, 2L * a.M, Kp / 2, Kp / 2, 64, box_rows);       // (bytes, two at a time)
+    if (rc) return rc;
+    rc = fb_tensor_map_out(&mo, a.out, a.o_bf16 ? 2 : 4, a.M, a.gate.act ? a.N / 2 : a.N, a.ldo, a.slabs ? a.slabs : 1, a.slab_stride,
+                           a.gate.act ? MX_ROWS / 2 : MX_ROWS, OUT_TOKENS);
+    a.boxed = rc == 0;
+    return rc < 0 ? rc : 0;
 }
 
 int check_operands(const void* X, long long lda, const void* W, const int* shifts, const void* out, int o_dtype, long long ldo, int M, int N,
@@ -466,21 +684,32 @@ int check_operands(const void* X, long long lda, const void* W, const int* shift
                "gemm_mxfp4: a gate needs a known activation, an even number of stacked rows and no plain activation beside it");
     FB_REQUIRE(fb_plain_act_known(plain_act), "gemm_mxfp4: unknown activation code %d", plain_act);
     FB_REQUIRE(lda >= K && ldo >= (gate.act ? N / 2 : N), "gemm_mxfp4: a row stride is shorter than its row");
-    FB_REQUIRE(lda % 8 == 0 && ((uintptr_t)X & 15) == 0, "gemm_mxfp4: rows must start on 16-byte borders");
-    FB_REQUIRE(W && ((uintptr_t)W & 15) == 0 && shifts && status, "gemm_mxfp4: unaligned weights, or no shifts, or no status word");
+    FB_REQUIRE(((uintptr_t)X & 1) == 0 && W && ((uintptr_t)W & 15) == 0 && shifts && status,
+               "gemm_mxfp4: unaligned rows or weights, or no shifts, or no status word");
     FB_REQUIRE(((uintptr_t)out & (o_dtype == FB_F32 ? 3 : 1)) == 0, "gemm_mxfp4: unaligned output");
     return 0;
 }
 
 }  // namespace
 
+// Bytes of `scratch` that the products below want for M rows of K (tile: the grouped form's row tile, 0: not grouped).
+FB_API long long fb_gemm_mxfp4_rows_bytes(int M, int K, int tile) {
+    if (M <= 0 || K <= 0) return 0;
+    const long long kb = (K + MX_COLS - 1) / MX_COLS;
+    return 2LL * M * kb * MX_COLS + scale_bytes_of(M, (int)kb, tile > 0);
+}
+
 // Floats of `partials` that fb_gemm_mxfp4 wants for the same sizes with `n_counters` counters and without slabs: 0 where K is not
 // split.
-FB_API long long fb_gemm_mxfp4_scratch_floats(int M, int N, int K, int n_counters) {
+FB_API long long fb_gemm_mxfp4_share_floats(int M, int N, int K, int n_counters) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const MxPlan p = plan_mxfp4(M, N, (K + XBK - 1) / XBK, MOST_SPLITS, SHARE_FLOATS, n_counters, false);
-    if (p.splits == 1) return 0;
-    return (long long)((M + p.bn - 1) / p.bn) * ((N + XBM - 1) / XBM) * p.splits * p.bn * XBM;
+    const int tiles_n = (N + MX_ROWS - 1) / MX_ROWS, kb = (K + MX_COLS - 1) / MX_COLS;
+    if (M <= NARROW_TOKENS) {
+        const int segments = tiles_n <= n_counters ? cut_of(tiles_n, kb, ANY).segments : 1;
+        return segments > 1 ? (long long)tiles_n * segments * narrow_tokens(M) * MX_ROWS : 0;
+    }
+    const Plan p = plan_wide(M, N, kb, MOST_SPLITS, SHARE_FLOATS, n_counters, false);
+    return p.splits == 1 ? 0 : (long long)((M + p.bn - 1) / p.bn) * tiles_n * p.splits * p.bn * MX_ROWS;
 }
 
 // X [M,K] bfloat16, W one matrix in tiles with its shift (fb_mxfp4_tiles).  `act` (an FbAct code with its constants): W stacks gate
@@ -488,11 +717,12 @@ FB_API long long fb_gemm_mxfp4_scratch_floats(int M, int N, int K, int n_counter
 // `accumulate` (float32): the product is added to what `out` holds.  Shares of K: with slab_stride > 0 (float32, neither activation
 // nor accumulate) share s goes to out + s * slab_stride and *splits_used says how many there are (at most max_slabs); else they
 // meet in `partials` and `counters` (zero before the call and after it), the scratch of calls that run one after the other;
-// without it, or with fewer floats than fb_gemm_mxfp4_scratch_floats asks for, K is split less or not at all.
+// without it, or with fewer floats than fb_gemm_mxfp4_share_floats asks for, K is not split.  `scratch`: fb_gemm_mxfp4_rows_bytes
+// (M, K, 0) bytes on a 128-byte border.
 FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int* shifts, void* out, int o_dtype, long long ldo,
                          long long slab_stride, int max_slabs, int* splits_used, int M, int N, int K, int act, float limit,
                          float slope, int plain_act, int accumulate, float* partials, long long partial_floats, int* counters,
-                         int n_counters, int* status, cudaStream_t stream) {
+                         int n_counters, void* scratch, long long scratch_bytes, int* status, cudaStream_t stream) {
     const FbGate gate = {act, limit, slope};
     if (const int rc = check_operands(X, lda, W, shifts, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
     FB_REQUIRE(slab_stride == 0 || (o_dtype == FB_F32 && max_slabs >= 1 && slab_stride >= (long long)M * ldo && !act && !plain_act && !accumulate),
@@ -500,38 +730,72 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
     FB_REQUIRE(!accumulate || (o_dtype == FB_F32 && !act && !plain_act), "gemm_mxfp4: only a float32 product can be added to its output");
     if (splits_used) *splits_used = 1;
     if (M == 0) return 0;
-    const bool slabs = slab_stride > 0;
-    const MxPlan plan = plan_mxfp4(M, N, (K + XBK - 1) / XBK, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : MOST_SPLITS,
-                                   partials && counters ? partial_floats : 0, counters ? n_counters : 0, slabs);
     MxArgs a = {};
     a.W = (const uint8_t*)W; a.shifts = shifts; a.out = out; a.ldo = (long)ldo; a.slab_stride = (long)slab_stride;
+    a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, nullptr, nullptr, nullptr};
     a.o_bf16 = o_dtype == FB_BF16; a.accumulate = accumulate; a.partials = partials; a.counters = counters;
-    a.M = M; a.N = N; a.K = K; a.kb = (K + XBK - 1) / XBK;
-    a.tiles_m = (M + plan.bn - 1) / plan.bn; a.tiles_n = (N + XBM - 1) / XBM; a.splits = plan.splits;
+    a.M = M; a.N = N; a.K = K; a.kb = (K + MX_COLS - 1) / MX_COLS; a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
-    if (splits_used) *splits_used = slabs ? plan.splits : 1;
-    return launch_mxfp4(plan, a, X, (long)lda, plan.bn, (long)a.tiles_m * a.tiles_n * a.splits, stream);
+    const bool slabs = slab_stride > 0;
+    const bool join = !slabs && partials && counters && partial_floats >= fb_gemm_mxfp4_share_floats(M, N, K, n_counters);
+    CUtensorMap mx = {}, mo = {};
+    if (M <= NARROW_TOKENS) {
+        const Cut cut = cut_of(a.tiles_n, a.kb, slabs ? max_slabs : join && a.tiles_n <= n_counters ? ANY : 1);
+        a.bn = narrow_tokens(M);
+        a.tiles_m = 1; a.splits = 1; a.items = (long)a.tiles_n * a.kb;
+        a.max_segments = cut.segments;
+        if (slabs) {
+            a.slabs = cut.segments;
+            if (splits_used) *splits_used = cut.segments;
+        }
+        if (const int rc = prepare(a, mx, mo, scratch, scratch_bytes, a.bn, stream)) return rc;
+        return launch<32, false>(a, mx, mo, cut.grid, stream);
+    }
+    const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, SHARE_FLOATS,
+                                n_counters, slabs);
+    a.bn = plan.bn;
+    a.tiles_m = (M + plan.bn - 1) / plan.bn;
+    a.splits = a.max_segments = plan.splits;
+    if (slabs) {
+        a.slabs = plan.splits;
+        if (splits_used) *splits_used = plan.splits;
+    }
+    a.items = (long)a.tiles_m * a.tiles_n * a.splits;
+    if (a.items > 2000000000L) return fb_fail(-1, "gemm_mxfp4: too many tiles (M=%d N=%d)", M, N);
+    if (const int rc = prepare(a, mx, mo, scratch, scratch_bytes, a.bn, stream)) return rc;
+    const long grid = a.items < fb_sm_count() ? a.items : fb_sm_count();
+    return a.bn <= 64 ? launch<64, false>(a, mx, mo, grid, stream) : launch<128, false>(a, mx, mo, grid, stream);
 }
 
-// The grouped form: W holds `groups` matrices [N, K] in tiles with a shift each; the M rows of X and `out` come in tiles of `tile`
-// (a multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are).
-FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const void* W, const int* shifts, int groups, const int* tile_group,
-                                 int tile, void* out, int o_dtype, long long ldo, int M, int N, int K, int act, float limit,
-                                 float slope, int plain_act, int* status, cudaStream_t stream) {
+// The grouped form: W holds `groups` matrices [N, K] in tiles with a shift each; the M rows of `out` come in tiles of `tile` (a
+// multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are).  Row m is
+// X[m], or with row_index X[row_index[m]] (negative: zeros), with row_share times row_share[row_pair[m]].  `scratch`:
+// fb_gemm_mxfp4_rows_bytes(M, K, tile) bytes.
+FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_index, const float* row_share, const int* row_pair,
+                                 const void* W, const int* shifts, int groups, const int* tile_group, int tile, void* out, int o_dtype,
+                                 long long ldo, int M, int N, int K, int act, float limit, float slope, int plain_act, void* scratch,
+                                 long long scratch_bytes, int* status, cudaStream_t stream) {
     const FbGate gate = {act, limit, slope};
     if (const int rc = check_operands(X, lda, W, shifts, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
     FB_REQUIRE(groups > 0 && tile_group, "gemm_mxfp4_grouped: no groups");
     FB_REQUIRE(tile >= 16 && tile <= 128 && tile % 16 == 0 && M % tile == 0 && M / tile < (1 << 24),
                "gemm_mxfp4_grouped: the rows must be whole tiles of 16 to 128, not tiles of %d", tile);
+    FB_REQUIRE(!row_share || (row_index && row_pair), "gemm_mxfp4_grouped: shares need the rows' index and pairs");
     if (M == 0) return 0;
     MxArgs a = {};
-    a.kb = (K + XBK - 1) / XBK;
-    a.tiles_n = (N + XBM - 1) / XBM;
+    a.kb = (K + MX_COLS - 1) / MX_COLS;
+    a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     a.W = (const uint8_t*)W; a.w_group = (long)a.tiles_n * a.kb * MX_TILE_BYTES; a.shifts = shifts; a.out = out; a.ldo = (long)ldo;
-    a.o_bf16 = o_dtype == FB_BF16; a.M = M; a.N = N; a.K = K; a.tiles_m = 1; a.splits = 1;
+    a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, row_index, row_share, row_pair};
+    a.o_bf16 = o_dtype == FB_BF16; a.M = M; a.N = N; a.K = K; a.tiles_m = 1; a.splits = a.max_segments = 1;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
     a.tile_group = tile_group; a.tile = tile; a.n_tiles = M / tile;
-    const bool wide = tile > 16;
-    const int most = wide ? Form<true>::MOST_TOKENS : Form<false>::MOST_TOKENS;
-    return launch_mxfp4(MxPlan{most / tile * tile, 1, wide}, a, X, (long)lda, tile, (long)a.n_tiles * a.tiles_n, stream);
+    const long units = (long)a.n_tiles * a.tiles_n;
+    if (units > 2000000000L) return fb_fail(-1, "gemm_mxfp4_grouped: too many tiles (M=%d N=%d)", M, N);
+    CUtensorMap mx = {}, mo = {};
+    const bool narrow = tile == 16;
+    a.bn = (narrow ? NARROW_TOKENS : WIDE_TOKENS) / tile * tile;
+    if (const int rc = prepare(a, mx, mo, scratch, scratch_bytes, tile, stream)) return rc;
+    const long grid = units < fb_sm_count() ? units : fb_sm_count();
+    return narrow ? launch<32, true>(a, mx, mo, grid, stream) : launch<128, true>(a, mx, mo, grid, stream);
 }

@@ -82,10 +82,6 @@ __device__ __forceinline__ float code_value(uint32_t code, float scale) {
     const float v = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
     return copysignf(v, code & 8u ? -1.0f : 1.0f) * scale;
 }
-__device__ __forceinline__ float scale_value(uint32_t s) {
-    return __uint_as_float(s == 255u ? 0x7fc00000u : s == 0 ? 0x00400000u : s << 23);
-}
-
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long rows, int K, int blocks,
@@ -97,7 +93,7 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
         const long row = q / (blocks * 4);
         const int c = 8 * (int)(q - row * (blocks * 4));
         const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[q];
-        const float scale = scale_value(scales[q >> 2]);
+        const float scale = mx_scale_f32(scales[q >> 2]);
         T v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = fb_from_float<T>(code_value(w >> (4 * i) & 15u, scale));
@@ -147,29 +143,52 @@ tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scal
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[i] |= mx_place(in[i] >> (8 * j) & 15u, j) | mx_place(in[i] >> (8 * j + 4) & 15u, j) << 16;
+            for (int j = 0; j < 8; ++j) w[i] |= mx_place(in[i] >> (4 * j) & 15u, j);
         s = scales[at];
         if (s != 255) {
-            s -= shifts[group];
-            if (s < 0) {                 // below 2^-127 of the largest scale that the product takes: nothing is left of it
+            s += MX_RAISE - shifts[group];
+            if (s < 0) {                 // 2^248 below the largest scale: nothing is left of it
                 s = 0;
                 w[0] = w[1] = w[2] = w[3] = 0;
             }
         }
     }
     reinterpret_cast<uint4*>(dst)[(b & 3) * MX_ROWS + row] = make_uint4(w[0], w[1], w[2], w[3]);
-    dst[MX_CODE_BYTES + row * 4 + (b & 3)] = (uint8_t)s;
+    dst[MX_CODE_BYTES + ((row & 31) * 4 + (row >> 5)) * 4 + (b & 3)] = (uint8_t)s;
 }
 
-// Rows of bfloat16 numbers into rows that start on 16-byte borders.
+// A thread eight numbers: parts[p][m][k] (bytes, rows of Kp, a multiple of 128, zeros behind K), their scales as `layout` says.
 __global__ void __launch_bounds__(256)
-align_rows_kernel(const __nv_bfloat16* __restrict__ x, long ldx, int M, int K, __nv_bfloat16* __restrict__ out, long ldo) {
+split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales,
+             const __grid_constant__ MxScaleLayout layout, const int* __restrict__ tile_group, int tile) {
     fb_pdl_launch_dependents();
     fb_pdl_wait();
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)M * K; i += (long)gridDim.x * 256) {
-        const long m = i / K, k = i - m * K;
-        out[m * ldo + k] = x[m * ldx + k];
+    const int pieces = Kp / 8;
+    for (long base = (long)blockIdx.x * 256; base < (long)M * pieces; base += (long)gridDim.x * 256) {
+        const long p = base + threadIdx.x;
+        const bool mine = p < (long)M * pieces;
+        const int m = mine ? (int)(p / pieces) : 0, k = mine ? 8 * (int)(p - (long)m * pieces) : 0;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        // (rows of tiles without a group are not multiplied, whatever they hold)
+        if (mine && (!tile_group || tile_group[m / tile] >= 0)) v = mx_row8(rows, m, k, K);
+        const uint32_t scale = mx_row_scale(mx_top8(v));
+        uint2 first, second;
+        mx_split8({v.x, v.y, v.z, v.w}, scale, first, second);
+        if (!mine) continue;
+        *reinterpret_cast<uint2*>(parts + (size_t)m * Kp + k) = first;
+        *reinterpret_cast<uint2*>(parts + ((size_t)M + m) * Kp + k) = second;
+        if ((k & 31) != 0) continue;
+        const int kb = k >> 7, byte = k >> 5 & 3;
+        if (layout.tokens == 0) {
+            scales[((size_t)kb * layout.rows + m) * 4 + byte] = (uint8_t)scale;
+        } else {
+            const int tiles = (M + layout.tokens - 1) / layout.tokens, t = m / layout.tokens, q = m - t * layout.tokens;
+            uint8_t* at = scales + ((size_t)kb * tiles + t) * layout.tile_bytes + byte;
+            const int second = layout.tokens <= 64 ? layout.tokens + q : (layout.tokens + 127) / 128 * 128 + q;
+            auto place = [](int row) { return (row >> 7) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4; };
+            at[place(q)] = (uint8_t)scale;
+            at[place(second)] = (uint8_t)mx_second_scales(scale);
+        }
     }
 }
 
@@ -233,11 +252,12 @@ FB_API int fb_mxfp4_tiles(const void* codes, const void* scales, int groups, int
     return fb_check_launch("mxfp4_tiles");
 }
 
-// out[m, k] = x[m, k], rows of `out` ldo elements apart (what lies between them is left as it is).
-FB_API int fb_align_rows(const void* x, long long ldx, int M, int K, void* out, long long ldo, cudaStream_t stream) {
-    FB_REQUIRE(M >= 0 && K > 0 && (ldx >= K || M <= 1) && ldo >= K, "align_rows: bad sizes");
-    if (M == 0) return 0;
-    fb_launch(align_rows_kernel, dim3(grid_of((long)M * K, 256)), dim3(256), 0, stream, (const __nv_bfloat16*)x, (long)ldx, M, K,
-              (__nv_bfloat16*)out, (long)ldo);
-    return fb_check_launch("align_rows");
+// The rows of a product with four-bit weights as two e4m3 numbers each (mxfp4.cuh): `parts` takes 2 M Kp bytes (Kp: K rounded up to
+// a multiple of 128), `scales` what `layout` says, both 16-byte aligned.
+int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, MxScaleLayout layout, const int* tile_group, int tile,
+                        cudaStream_t stream) {
+    const int Kp = (K + MX_COLS - 1) / MX_COLS * MX_COLS;
+    fb_launch(split_kernel, dim3(grid_of((long)M * (Kp / 8), 256)), dim3(256), 0, stream, rows, M, K, Kp, (uint8_t*)parts, (uint8_t*)scales,
+              layout, tile_group, tile);
+    return fb_check_launch("mxfp4_split_rows");
 }

@@ -3,8 +3,8 @@
 //
 // Two layouts.  Rows: codes [rows][16 bytes a block], element 2 i of a block in the low half of byte i, and scales
 // [rows][blocks].  Tiles, what the product reads: 128 rows x 128 columns in MX_TILE_BYTES contiguous bytes, zeros beyond the
-// matrix, row tile by row tile, within one along the columns: [block of 32 columns][row][16 bytes], then [row][4 scales].  One bulk
-// copy fetches a tile, and the 32 threads of a warp, a row each, read 512 contiguous bytes of shared memory.
+// matrix, row tile by row tile, within one along the columns: [block of 32 columns][row][16 bytes of codes], then the scales as
+// tcgen05.mma wants them in tensor memory, [lane i][j] words of the four scales of row 32 j + i.
 #pragma once
 
 #include "common.cuh"
@@ -14,35 +14,108 @@ constexpr int MX_LAST_SCALE = 252;                                       // the 
 constexpr int MX_ROWS = 128, MX_COLS = 128;                              // a tile
 constexpr int MX_CODE_BYTES = MX_ROWS * MX_COLS / 2;
 constexpr int MX_TILE_BYTES = MX_CODE_BYTES + MX_ROWS * MX_COLS / MX_BLOCK;
-// Scales up to 2^1 are multiplied in as they are (see mx_decode); a matrix with larger ones carries a shift that its scales are
-// lowered by in the tiles, and that the product's results are raised by.
-constexpr int MX_TOP_SCALE = 128;
+// A code becomes an e4m3 number (sign, four bits of exponent, three of mantissa) by putting its magnitude bits where they are the
+// end of the exponent and the first bit of the mantissa: the number times 2^-6, subnormal ones included.  The tiles' scales make
+// up for it; where that passes their largest, a matrix carries a shift that they are lowered by, and results are raised by.
+constexpr int MX_RAISE = 6, MX_TOP_SCALE = 254 - MX_RAISE;
 
-// Eight codes in a 32-bit word of a tile: columns 2 j and 2 j + 1 (j = 0..3) in the lower and upper half, their bits where one
-// shift and one mask (for j = 3 three of each) bring the sign to bit 15 and the three magnitude bits to bits 8..6 of a
-// bfloat16: as the end of its exponent and the first bit of its mantissa they are the number times 2^-126, subnormal ones
-// included, which one multiplication by 2^(S - 1) puts right.
-//   j = 0: bits 15, 8, 7, 6    j = 1: 12, 5, 4, 3    j = 2: 9, 2, 1, 0    j = 3: 14, 13, 11, 10
-__host__ __device__ __forceinline__ uint32_t mx_place(uint32_t code, int j) {       // one code's bits within its half
-    const uint32_t s = code >> 3, m = code & 7u;
-    if (j == 3) return s << 14 | (m >> 2) << 13 | (m & 3u) << 10;
-    return (s << 15 | m << 6) >> (3 * j);
+// Eight codes in a 32-bit word of a tile.  Columns 0..3: bits 7 (sign), 4, 3, 2 of its bytes, where they are wanted.  Columns 4..7: bits 5
+// (sign), 1 (the exponent's lower bit) of its bytes, two places away, and 0 (the upper one), 6 of the byte before (the mantissa's), four
+// places away in a word that turns: two rotations and two operations for the four.
+__host__ __device__ __forceinline__ uint32_t mx_place(uint32_t code, int column) {
+    const uint32_t s = code >> 3, e1 = code >> 2 & 1u, e0 = code >> 1 & 1u, m = code & 1u;
+    const int byte = 8 * (column & 3);
+    if (column < 4) return (s << 7 | e1 << 4 | e0 << 3 | m << 2) << byte;
+    return (s << 5 | e0 << 1 | e1) << byte | m << ((byte + 30) & 31);
 }
-__device__ __forceinline__ uint32_t mx_mul(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
+// The e4m3 numbers of columns 0..3 and 4..7, packed.
+__device__ __forceinline__ void mx_decode(uint32_t w, uint32_t& first, uint32_t& second) {
+    first = w & 0x9C9C9C9Cu;
+    second = (__funnelshift_l(w, w, 2) & 0x88888888u) | (__funnelshift_l(w, w, 4) & 0x14141414u);
 }
-// The four pairs of a word, times `scale` (a bfloat16 pair of 2^(S - 1)).
-__device__ __forceinline__ void mx_decode(uint32_t w, uint32_t scale, uint32_t* out) {
-    constexpr uint32_t MASK = 0x81C081C0u;
-    out[0] = mx_mul(w & MASK, scale);
-    out[1] = mx_mul((w << 3) & MASK, scale);
-    out[2] = mx_mul((w << 6) & MASK, scale);
-    out[3] = mx_mul(((w << 1) & 0x80008000u) | ((w >> 5) & 0x01000100u) | ((w >> 4) & 0x00C000C0u), scale);
+// 2^(S - 127) in float32.
+__device__ __forceinline__ float mx_scale_f32(uint32_t s) {
+    return __uint_as_float(s == 255u ? 0x7fc00000u : s == 0 ? 0x00400000u : s << 23);
 }
-// 2^(S - 1) twice, for scales of a tile (0 .. MX_TOP_SCALE, 255: not a number).
-__device__ __forceinline__ uint32_t mx_scale(uint32_t s) {
-    const uint32_t one = s == 255u ? 0x7FC0u : (s + 126u) << 7;
-    return one | one << 16;
+
+// ---- rows of bfloat16 numbers as two e4m3 numbers each ----
+// With 2^e <= amax < 2^(e + 1) the largest magnitude of a block of 32, y = x 2^(7 - e) lies below 2^8; its first part is y rounded
+// to e4m3, its second what that left, times 2^5.  Eight bits of mantissa go into four and four: what is lost is below 2^-22 of amax.
+// Scales: MX_FIRST less than the exponent's field for the first part, 5 less again for the second; blocks below 2^-115 use that
+// exponent's.  A block with an infinity or a NaN gets scales of 255, and so do the sums that it is part of.
+constexpr int MX_LEAST_FIELD = 12, MX_FIRST = 7, MX_SECOND_LESS = 5;
+// `top`: the largest magnitude's 15 bits of the block.
+__device__ __forceinline__ uint32_t mx_row_scale(uint32_t top) {
+    const uint32_t field = top >> 7;
+    return field == 255u ? 255u : max(field, (uint32_t)MX_LEAST_FIELD) - MX_FIRST;
 }
+// Eight numbers (pairs in four words) under the block's scale: bytes of the first and the second parts.
+__device__ __forceinline__ void mx_split8(const uint32_t (&w)[4], uint32_t scale, uint2& first, uint2& second) {
+    const float inv = __uint_as_float((scale == 255u ? 127u : 254u - scale) << 23);
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __uint_as_float(w[i] << 16) * inv, b = __uint_as_float(w[i] & 0xffff0000u) * inv;
+        uint16_t p, q;
+        uint32_t back;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p) : "f"(b), "f"(a));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(p));
+        float ra, rb;
+        asm("{\n\t.reg .f16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}" : "=f"(ra), "=f"(rb) : "r"(back));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(q) : "f"((b - rb) * 32.0f), "f"((a - ra) * 32.0f));
+        h[i] = p;
+        l[i] = q;
+    }
+    first = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    second = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
+}
+__device__ __forceinline__ uint32_t mx_second_scales(uint32_t four) {       // of four first ones (255 stays; a sum is NaN by the first)
+    return __vsubus4(four, 0x01010101u * MX_SECOND_LESS);
+}
+// Eight numbers of a row from column k on: zeros from K on.  `aligned`: the row starts on a 16-byte border.
+__device__ __forceinline__ uint4 mx_load8(const __nv_bfloat16* row, int k, int K, bool aligned) {
+    if (aligned && k + 8 <= K) return *reinterpret_cast<const uint4*>(row + k);
+    uint32_t e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = k + i < K ? (uint32_t)__bfloat16_as_ushort(row[k + i]) : 0u;
+    return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+}
+// The largest magnitude's bits among eight numbers, and among the four lanes that share a block.
+__device__ __forceinline__ uint32_t mx_top8(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    return max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+}
+
+// Rows that a product reads: row m is x[m], or x[index[m]] (negative: zeros), times share[pair[m]] (rounded to bfloat16) where
+// there are shares.
+struct MxRows {
+    const __nv_bfloat16* x; long ld; int aligned;
+    const int* index; const float* share; const int* pair;
+};
+// Eight numbers times f, rounded to bfloat16.
+__device__ __forceinline__ uint4 mx_times(uint4 v, float f) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    return v;
+}
+__device__ __forceinline__ uint4 mx_row8(const MxRows& r, int m, int k, int K) {
+    const int from = r.index ? r.index[m] : m;
+    if (from < 0) return make_uint4(0, 0, 0, 0);
+    uint4 v = mx_load8(r.x + (size_t)from * r.ld, k, K, r.aligned != 0);
+    if (r.share) v = mx_times(v, r.share[r.pair[m]]);
+    return v;
+}
+// Where the rows' scales go.  tokens > 0: [K / 128][token tile][tile_bytes], a tile's first parts and then (up to 64 tokens: among
+// them as rows tokens .., else behind them, from a multiple of 128 rows on) its second ones as [128 rows][lane i][j] words of row
+// 32 j + i; tokens == 0: a word of the first part's a row, [K / 128][rows].
+struct MxScaleLayout { int tokens, tile_bytes; long rows; };
+int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, MxScaleLayout layout, const int* tile_group, int tile,
+                        cudaStream_t stream);

@@ -1702,11 +1702,12 @@ class Mxfp4Weight(PackedWeight):
             raise KernelError(f"{what}: one matrix wanted, not {tuple(self.shape)}")
         return self._operands(a, out, columns, what)
 
-    def _operands(self, a: torch.Tensor, out: torch.Tensor, columns: int, what: str) -> tuple:
+    def _operands(self, a: torch.Tensor, out: torch.Tensor, columns: int, what: str, indexed: bool = False) -> tuple:
         """Checks what a product takes: a [M, K] bfloat16, out [M, columns] float32 or bfloat16, rows dense.  (M, N, K)."""
         _cuda(a, out)
         N, K = self.shape[-2:]
-        if a.dim() != 2 or out.dim() != 2 or a.shape[1] != K or out.shape[1] != columns or out.shape[0] != a.shape[0]:
+        if a.dim() != 2 or out.dim() != 2 or a.shape[1] != K or out.shape[1] != columns \
+                or (out.shape[0] != a.shape[0] and not indexed):
             raise KernelError(f"{what}: shapes a{tuple(a.shape)} w{tuple(self.shape)} out{tuple(out.shape)} do not agree")
         if a.dtype != torch.bfloat16:
             raise KernelError(f"{what}: four-bit weights multiply bfloat16 rows, not {a.dtype}")
@@ -1716,32 +1717,21 @@ class Mxfp4Weight(PackedWeight):
         _rows(out)
         return a.shape[0], N, K
 
-    @staticmethod
-    def _aligned(a: torch.Tensor, ws) -> torch.Tensor:
-        """a, or a copy of it in the arena where its rows do not start on 16-byte borders."""
-        if _rows(a) % 8 == 0 and a.data_ptr() % 16 == 0:
-            return a
-        M, K = a.shape
-        side = ws.alloc((M, -(-K // 8) * 8), a.dtype)
-        check(lib().fb_align_rows(a.data_ptr(), _rows(a), M, K, side.data_ptr(), side.stride(0), _stream()), "align_rows")
-        return side[:, :K]
-
     def _product(self, a, out, ctx, columns: int, what: str, gate=(0, 0.0, 0.0), plain_act: int = 0, accumulate: bool = False,
                  slabs=None) -> int:
         M, N, K = self._matrix(a, out, columns, what)
         ws, used = ctx.ws, ctypes.c_int(1)
         counters = ws.counters
         with ws.scope():
-            a = self._aligned(a, ws)
-            floats, partials = 0, None
-            if slabs is None:
-                floats = lib().fb_gemm_mxfp4_scratch_floats(M, N, K, counters.numel())
-                partials = ws.alloc((floats,), torch.float32) if floats > 0 else None
+            floats = 0 if slabs is not None else lib().fb_gemm_mxfp4_share_floats(M, N, K, counters.numel())
+            partials = ws.alloc((floats,), torch.float32) if floats > 0 else None
+            nbytes = lib().fb_gemm_mxfp4_rows_bytes(M, K, 0)
+            parts = ws.alloc((nbytes,), torch.uint8) if nbytes > 0 else None
             check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self.tiles.data_ptr(), self.shifts.data_ptr(), out.data_ptr(),
                                       dtype_code(out), _rows(out), slabs.stride(0) if slabs is not None else 0,
                                       slabs.shape[0] if slabs is not None else 0, ctypes.byref(used), M, N, K, *gate, plain_act,
                                       1 if accumulate else 0, _ptr(partials), floats, counters.data_ptr(), counters.numel(),
-                                      ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
+                                      _ptr(parts), nbytes, ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
         return used.value
 
     def linear(self, a, out, ctx) -> None:
@@ -1786,20 +1776,24 @@ class Mxfp4Weight(PackedWeight):
             raise KernelError(f"{what}: weights [groups, outputs, inputs] wanted, with a gate an even number of outputs")
         if tile < 16 or tile > 128 or tile % 16 or M % tile or tile_group.numel() * tile < M or not tile_group.is_contiguous():
             raise KernelError(f"{what}: {M} rows are not whole tiles of {tile} (a multiple of 16 up to 128) with a group each")
+        if row_index is None and row_share is not None:
+            raise KernelError(f"{what}: shares of rows go with an index of rows")
+        if row_index is not None and (row_index.numel() < M or not row_index.is_contiguous()):
+            raise KernelError(f"{what}: a contiguous index of {M} rows wanted")
+        if row_share is not None and (row_share.dtype != torch.float32 or row_pair is None or row_pair.numel() < M
+                                      or not row_share.is_contiguous() or not row_pair.is_contiguous()):
+            raise KernelError(f"{what}: float32 shares come with the pair of every row")
+        _i32(row_index, "row_index")
+        _i32(row_pair, "row_pair")
+        _cuda(row_share, row_pair)
+        self._operands(a, out, N // 2 if gate is not None else N, what, indexed=row_index is not None)
+        gate_args = gate_arguments(gate) if gate is not None else (0, 0.0, 0.0)
         ws = ctx.ws
         with ws.scope():
-            if row_index is not None:
-                if row_index.numel() < M or a.shape[1] != K:
-                    raise KernelError(f"{what}: shapes do not agree")
-                side = ws.alloc((M, K), a.dtype)
-                gather_rows(a, row_index, side, row_share, row_pair, tile_group, tile)
-                a = side
-            elif row_share is not None:
-                raise KernelError(f"{what}: shares of rows go with an index of rows")
-            self._operands(a, out, N // 2 if gate is not None else N, what)
-            a = self._aligned(a, ws)
-            gate_args = gate_arguments(gate) if gate is not None else (0, 0.0, 0.0)
-            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), self.tiles.data_ptr(), self.shifts.data_ptr(),
-                                              self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(), dtype_code(out),
-                                              _rows(out), M, N, K, *gate_args, plain_activation_code(activation_name),
+            nbytes = lib().fb_gemm_mxfp4_rows_bytes(M, K, int(tile))
+            parts = ws.alloc((nbytes,), torch.uint8) if nbytes > 0 else None
+            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), _ptr(row_index), _ptr(row_share), _ptr(row_pair),
+                                              self.tiles.data_ptr(), self.shifts.data_ptr(), self.shape[0], tile_group.data_ptr(),
+                                              int(tile), out.data_ptr(), dtype_code(out), _rows(out), M, N, K, *gate_args,
+                                              plain_activation_code(activation_name), _ptr(parts), nbytes,
                                               ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4_grouped", (M, N, K))
