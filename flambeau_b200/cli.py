@@ -2,9 +2,9 @@
 (crates/cli/src/main.rs:36-278): subcommands, long options with dashes.
 
   flambeau infer --model DIR --prompt "1,2,3" --max-tokens 64 [--temperature T --top-p P --top-k K --min-p M
-                 --seed S --dtype bfloat16|float32 --devices cuda:0 --inflight-slots N --prefill-ubatch N
+                 --seed S --dtype bfloat16|float32 --weights stored|mxfp4 --devices cuda:0 --inflight-slots N --prefill-ubatch N
                  --prefill-chunk-tokens N --paged-kv PAGES --ctx-cap N]
-  flambeau replay --model DIR --dtype ... --out DIR --max-tokens N      (steps as JSON lines on stdin)
+  flambeau replay --model DIR --dtype ... [--weights ...] --out DIR --max-tokens N      (steps as JSON lines on stdin)
   flambeau random-model --config CONFIG.json --out DIR --seed S --dtype bfloat16|float32
   flambeau inspect --model DIR
   flambeau bench [--shape 7b|nemo12b|small24b] [--only headline|mixed|shapes] [--steps K] ...   (one JSON line)
@@ -38,7 +38,8 @@ def cmd_infer(a) -> int:
                     presence_penalty=a.presence_penalty, frequency_penalty=a.frequency_penalty, seed=a.seed,
                     stop_token_ids=tuple(a.stop_token_id or ()), dtype=a.dtype, devices=a.devices,
                     inflight_slots=a.inflight_slots, prefill_ubatch=a.prefill_ubatch,
-                    prefill_chunk_tokens=a.prefill_chunk_tokens, paged_kv=a.paged_kv, ctx_cap=a.ctx_cap)
+                    prefill_chunk_tokens=a.prefill_chunk_tokens, paged_kv=a.paged_kv, ctx_cap=a.ctx_cap,
+                    weights=a.weights)
     for o in outs:
         print(",".join(str(t) for t in o))
     return 0
@@ -46,7 +47,8 @@ def cmd_infer(a) -> int:
 
 def cmd_replay(a) -> int:
     from .engine.trace import main as trace_main
-    return trace_main(["--model", a.model, "--dtype", a.dtype, "--out", a.out, "--max-tokens", str(a.max_tokens)])
+    return trace_main(["--model", a.model, "--dtype", a.dtype, "--out", a.out, "--max-tokens", str(a.max_tokens),
+                       "--weights", a.weights])
 
 
 def cmd_random_model(a) -> int:
@@ -97,6 +99,8 @@ def main(argv=None) -> int:
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--stop-token-id", type=int, action="append")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--weights", choices=["stored", "mxfp4"], default="stored",
+                   help="mxfp4: quantise the large maps' weights to four bits when the model is loaded")
     p.add_argument("--inflight-slots", type=int, default=4)
     p.add_argument("--prefill-ubatch", type=int, default=2048, help="most rows of one step")
     p.add_argument("--prefill-chunk-tokens", type=int, default=2048, help="longest portion of a prompt in one step")
@@ -109,6 +113,7 @@ def main(argv=None) -> int:
     p.add_argument("--dtype", choices=["bfloat16", "float32"], required=True)
     p.add_argument("--out", required=True)
     p.add_argument("--max-tokens", type=int, required=True)
+    p.add_argument("--weights", choices=["stored", "mxfp4"], default="stored")
     p.set_defaults(fn=cmd_replay)
 
     p = sub.add_parser("random-model", help="write a model folder with seeded random weights")

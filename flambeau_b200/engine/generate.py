@@ -90,7 +90,7 @@ def generate(model, prompts, *, max_tokens: int = 64, temperature: float = 0.0, 
              repetition_penalty: float = 1.0, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
              logit_bias=None, seed: int = 0, stop_token_ids=(), dtype: str = "bfloat16", devices: str = "cuda:0",
              inflight_slots: int = 4, prefill_ubatch: int = 2048, prefill_chunk_tokens: int = 2048,
-             paged_kv: int | None = None, ctx_cap: int | None = None, page_size: int = 16) -> list:
+             paged_kv: int | None = None, ctx_cap: int | None = None, page_size: int = 16, weights: str = "stored") -> list:
     """Generate `max_tokens` tokens for each prompt (lists of token ids).
 
     model: a folder with config.json and model.safetensors, or an Engine to reuse.
@@ -101,7 +101,9 @@ def generate(model, prompts, *, max_tokens: int = 64, temperature: float = 0.0, 
     long (27 ms for the 7B shape) as a 512-row step does there.
     paged_kv: number of cache pages (default: enough for `inflight_slots` requests of the longest prompt
     plus max_tokens); ctx_cap: the most tokens one request may hold, prompt and generated together: a request
-    that reaches it ends there, one whose prompt is longer gets no tokens."""
+    that reaches it ends there, one whose prompt is longer gets no tokens.
+    weights: 'stored', or 'mxfp4': the large maps' weights are quantised to four bits when the model is loaded (an Engine
+    given as `model` keeps its own)."""
     if max_tokens < 0:
         raise ValueError("max_tokens must not be negative")
     longest = max((len(p) for p in prompts), default=1) + max_tokens
@@ -116,7 +118,7 @@ def generate(model, prompts, *, max_tokens: int = 64, temperature: float = 0.0, 
         cache_tokens = paged_kv * page_size if paged_kv else inflight_slots * per_request
         engine = Engine.from_folder(model, EngineOptions(
             dtype=dtype, page_size=page_size, cache_tokens=cache_tokens, max_requests=inflight_slots,
-            max_step_tokens=max(prefill_ubatch, inflight_slots), max_seq_len=longest, device=devices))
+            max_step_tokens=max(prefill_ubatch, inflight_slots), max_seq_len=longest, device=devices, weights=weights))
     gen = Generator(engine, prefill_chunk_tokens=prefill_chunk_tokens, prefill_ubatch=prefill_ubatch,
                     inflight_slots=inflight_slots)
     params = [SamplingParams(temperature=temperature, top_p=top_p, top_k=top_k, min_p=min_p,

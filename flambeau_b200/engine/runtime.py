@@ -12,6 +12,15 @@ import torch
 
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
 
+WEIGHT_FORMATS = ("stored", "mxfp4")
+
+
+def parse_weight_format(name: str) -> str:
+    if name not in WEIGHT_FORMATS:
+        raise ValueError(f"weights must be one of {', '.join(WEIGHT_FORMATS)}, not {name!r}")
+    return name
+
+
 STATUS_BITS = {1: "a token id outside the vocabulary", 2: "a block table entry missing for a live key",
                4: "a bounded wait inside a kernel ran out"}
 
@@ -96,9 +105,15 @@ class Workspace:
 
 
 class Runtime:
-    def __init__(self, device="cuda:0", dtype="bfloat16", page_size: int = 16, workspace_bytes: int = 1 << 24):
+    """`weights`: how the large maps of attention and feed-forwards hold their weights, 'stored' (as the model folder and the
+    dtype rule say) or 'mxfp4' (quantised to four bits when they are bound; embedding, head, norms, routers and the maps
+    whose outputs are rates of a recurrence stay as stored)."""
+
+    def __init__(self, device="cuda:0", dtype="bfloat16", page_size: int = 16, workspace_bytes: int = 1 << 24,
+                 weights: str = "stored"):
         self.device = torch.device(device)
         self.dtype = parse_dtype(dtype)
+        self.weight_format = parse_weight_format(weights)
         self.page_size = int(page_size)
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")

@@ -31,6 +31,7 @@ class EngineOptions:
     max_step_tokens: int = 2048        # rows of one step
     max_seq_len: Optional[int] = None  # longest request; default: the pool size or the model's position limit
     device: str = "cuda:0"
+    weights: str = "stored"            # 'stored', or 'mxfp4': the large maps' weights in four bits (Runtime)
     cuda_graphs: bool = True           # replay steps of single decoded tokens from a captured CUDA graph
 
 
@@ -132,7 +133,7 @@ class Engine:
         from .. import models  # noqa: F401  (registers the built-in architectures)
         from ..weights.loader import load_model
         options = options or EngineOptions(**kw)
-        rt = Runtime(options.device, options.dtype, options.page_size)
+        rt = Runtime(options.device, options.dtype, options.page_size, weights=options.weights)
         return cls(load_model(folder, rt), options)
 
     @classmethod
@@ -143,7 +144,7 @@ class Engine:
         from ..models.decoder import DecoderModel
         from ..weights.random_init import fill_random_on_device
         options = options or EngineOptions(**kw)
-        rt = Runtime(options.device, options.dtype, options.page_size)
+        rt = Runtime(options.device, options.dtype, options.page_size, weights=options.weights)
         model = DecoderModel(resolve(config.architecture).build_spec(config), rt)
         model.config = config
         fill_random_on_device(model, seed)

@@ -63,6 +63,7 @@ def main(argv=None) -> int:
                     help="most tokens live requests hold at any time (each rounded up to a multiple of 64)")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--max-requests", type=int, default=4, help="live requests at most (state slots)")
+    ap.add_argument("--weights", choices=["stored", "mxfp4"], default="stored", help="how the large maps hold their weights")
     args = ap.parse_args(argv)
     tokens = max(64, -(-args.max_tokens // 64) * 64)
 
@@ -74,7 +75,7 @@ def main(argv=None) -> int:
     try:
         engine = Engine.from_folder(args.model, EngineOptions(
             dtype=args.dtype, page_size=args.page_size, cache_tokens=tokens, max_requests=args.max_requests,
-            max_step_tokens=tokens))           # a request may grow to the pool's size or the model's position limit
+            max_step_tokens=tokens, weights=args.weights))           # a request may grow to the pool's size or the model's position limit
         replay(engine, sys.stdin, args.out, report)
     except USER_ERRORS as e:                       # what the input or the model folder can cause: one line, no trace
         sys.stderr.write(f"trace_run: error: {type(e).__name__}: {e}\n")

@@ -730,7 +730,10 @@ def linear_slabs(a: torch.Tensor, w: torch.Tensor, slabs: torch.Tensor, ctx) -> 
 
 
 def grouped_tc_supported(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> bool:
-    """Whether the tcgen05 kernel takes a grouped product: bfloat16 operands whose rows TMA can fetch."""
+    """Whether a tcgen05 kernel takes a grouped product: bfloat16 operands whose rows TMA can fetch, or bfloat16 rows with
+    four-bit weights."""
+    if isinstance(w, PackedWeight):
+        return a.dtype == torch.bfloat16
     return (a.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and out.dtype in (torch.float32, torch.bfloat16)
             and a.dim() == 2 and a.stride(1) == 1 and a.stride(0) % 8 == 0 and w.shape[-1] % 8 == 0
             and a.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0 and w.is_contiguous()

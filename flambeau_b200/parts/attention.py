@@ -7,7 +7,7 @@ import torch
 
 from ..kernels import ops
 from .base import KVRequirement, Mixer, TensorSpec
-from .linear import Linear, concat_rows
+from .linear import Linear, concat_rows, held
 from .spec import PartSpec, build_part, register_part
 
 
@@ -148,8 +148,10 @@ class PagedAttention(Mixer):
         if rows % 8 and (self._wants_norm_kernel() or self.gate == "head") and self._fused_norm_kernel():
             # rows of zeros up to a multiple of 8, so that the product's float32 rows stay 16-byte aligned
             stack.append(torch.zeros((8 - rows % 8, self.width), dtype=stack[0].dtype, device=stack[0].device))
-        self.qkv = Linear(concat_rows(stack))
-        self.o = Linear(tensors[p + nm["o"]])
+        qkv = concat_rows(stack)
+        # (query/key norms without the fused kernel multiply with row slices of the weight, which stays a tensor then)
+        self.qkv = Linear(qkv if self.q_norm is not None and not self._fused_norm_kernel() else held(self.runtime, qkv))
+        self.o = Linear(held(self.runtime, tensors[p + nm["o"]]))
         if self.sink:
             self.sinks = tensors[p + nm["sink"]].float().contiguous()      # scores are float32 in both modes
 
@@ -203,7 +205,7 @@ class PagedAttention(Mixer):
                     self.nkv, self.hd, self.vd, rt.status, n_partials=parts, partial_stride=slabs.stride(0),
                     v_off=self.qw if self.values_from_keys else None)
                 a = ctx.ws.alloc((n, self.nh * self.vd), rt.dtype)
-                hint = self.o.weight if ctx.l2_hints and n <= 64 else None
+                hint = self.o.weight if ctx.l2_hints and n <= 64 and not self.o.packed else None
                 ops.paged_attention(ctx, q, a, cache, self.nh, self.nkv, self.hd, self.window, self.scale,
                                     next_weight=hint, score_slopes=self.distance_slopes, sinks=self.sinks, vd=self.vd,
                                     weights_float32=self.weights_float32, keep_first=self.keep_first,
@@ -257,7 +259,7 @@ class PagedAttention(Mixer):
                                   table_head=cache.table_head)
             a = ctx.ws.alloc((n, self.qw), rt.dtype)
             # few rows: the attention kernel fetches the start of the output projection's weights into L2 at its end
-            hint = self.o.weight if ctx.l2_hints and n <= 64 else None
+            hint = self.o.weight if ctx.l2_hints and n <= 64 and not self.o.packed else None
             ops.paged_attention(ctx, q, a, cache, self.nh, self.nkv, self.hd, self.window, self.scale,
                                 next_weight=hint, score_slopes=self.distance_slopes, sinks=self.sinks,
                                 weights_float32=self.weights_float32, keep_first=self.keep_first, softcap=self.softcap,

@@ -110,7 +110,7 @@ class Part:
 
     def weight_bytes(self) -> int:
         """Bytes of weights this part reads in one step (children included)."""
-        return sum(t.numel() * t.element_size() for t in self.own_weights()) + \
+        return sum(t.nbytes for t in self.own_weights()) + \
             sum(c.weight_bytes() for c in self.children())
 
     def own_weights(self) -> list:

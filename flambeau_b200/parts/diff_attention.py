@@ -7,7 +7,7 @@ import torch
 
 from ..kernels import ops
 from .base import KVRequirement, Mixer, TensorSpec
-from .linear import Linear, concat_rows
+from .linear import Linear, concat_rows, held
 from .spec import PartSpec, build_part, register_part
 
 
@@ -99,8 +99,8 @@ class DifferentialAttention(Mixer):
         rows = sum(t.shape[0] for t in stack)
         if rows % 8:          # rows of zeros up to a multiple of 8, so that the product's float32 rows stay 16-byte aligned
             stack.append(torch.zeros((8 - rows % 8, self.width), dtype=stack[0].dtype, device=stack[0].device))
-        self.proj = Linear(concat_rows(stack))
-        self.o = Linear(tensors[p + "o"])
+        self.proj = Linear(held(self.runtime, concat_rows(stack)))
+        self.o = Linear(held(self.runtime, tensors[p + "o"]))
         self.proj_bias = torch.cat([tensors[p + "q.b"], tensors[p + "k.b"], tensors[p + "v.b"]]).contiguous() \
             if self.bias else None
         self.o_bias = tensors[p + "o.b"].contiguous() if self.out_bias else None

@@ -7,7 +7,7 @@ import torch
 
 from ..kernels import ops
 from .base import FeedForward, TensorSpec
-from .linear import Linear, interleave_rows
+from .linear import Linear, held, interleave_rows
 from .spec import register_part
 
 
@@ -49,8 +49,8 @@ class GatedMLP(FeedForward):
     def own_bind(self, tensors):
         p = self.prefix
         gate, up, down = self.names
-        self.gate_up = Linear(interleave_rows(tensors[p + gate], tensors[p + up]))
-        self.down = Linear(tensors[p + down])
+        self.gate_up = Linear(held(self.runtime, interleave_rows(tensors[p + gate], tensors[p + up])))
+        self.down = Linear(held(self.runtime, tensors[p + down]))
         # Few rows (decoding): when the stacked matrix has at least as many 128-row tiles as the device has SMs,
         # one CTA per tile streams its rows over the whole of K and applies the activation in its epilogue; that
         # many CTAs draw the full memory bandwidth, and the separate activation kernel and the float32 shares it
@@ -58,7 +58,7 @@ class GatedMLP(FeedForward):
         # faster that way and keeps the split).  Narrower matrices keep the split of K, which is what fills the
         # device for them.
         sms = torch.cuda.get_device_properties(self.gate_up.weight.device).multi_processor_count \
-            if self.gate_up.weight.is_cuda else 0
+            if self.gate_up.weight.device.type == "cuda" else 0
         want = os.environ.get("FLAMBEAU_FFN_DECODE_EPILOGUE")
         self.decode_epilogue = (2 * self.inner // 128 >= sms > 0) if want is None else want != "0"
 
@@ -69,8 +69,10 @@ class GatedMLP(FeedForward):
         n = ctx.n_tokens
         with ctx.ws.scope():
             a = ctx.ws.alloc((n, self.inner), self.runtime.dtype)
-            fused = ops.tc_supported(h, self.gate_up.weight, a)
-            if n <= 64 and not (fused and self.decode_epilogue and n >= 2):
+            fused = not self.gate_up.packed and ops.tc_supported(h, self.gate_up.weight, a)
+            if self.gate_up.packed:
+                ops.gated_linear(h, self.gate_up.weight, a, self.activation, ctx)
+            elif n <= 64 and not (fused and self.decode_epilogue and n >= 2):
                 # few rows: float32 split-K shares, added by the activation kernel
                 gu = ctx.ws.alloc((ctx.max_slabs, n, 2 * self.inner), torch.float32)
                 parts = self.gate_up.slabs(ctx, h, gu)
@@ -111,8 +113,8 @@ class PlainMLP(FeedForward):
 
     def own_bind(self, tensors):
         up, down = self.names
-        self.up = Linear(tensors[self.prefix + up])
-        self.down = Linear(tensors[self.prefix + down])
+        self.up = Linear(held(self.runtime, tensors[self.prefix + up]))
+        self.down = Linear(held(self.runtime, tensors[self.prefix + down]))
 
     def own_weights(self):
         return [self.up.weight, self.down.weight]
@@ -121,7 +123,9 @@ class PlainMLP(FeedForward):
         n = ctx.n_tokens
         with ctx.ws.scope():
             a = ctx.ws.alloc((n, self.inner), self.runtime.dtype)
-            if n > 64 and ops.tc_supported(h, self.up.weight, a):
+            if self.up.packed:
+                ops.activated_linear(h, self.up.weight, a, self.activation, ctx)
+            elif n > 64 and ops.tc_supported(h, self.up.weight, a):
                 ops.gemm_tc_act(h, self.up.weight, a, self.runtime.status, self.activation)       # in the epilogue
             else:
                 z = ctx.ws.alloc((ctx.max_slabs, n, self.inner), torch.float32)

@@ -5,7 +5,7 @@ import torch
 
 from ..kernels import ops
 from .base import Mixer, StateRequirement, TensorSpec
-from .linear import Linear, concat_rows
+from .linear import Linear, concat_rows, held
 from .spec import register_part
 
 
@@ -106,8 +106,8 @@ class GatedDeltaRule(Mixer):
                                  f"{tensors[p + second].shape[1]} inputs")
         if rows % 8:          # rows of zeros up to a multiple of 8, so that the product's float32 rows stay 16-byte aligned
             stack.append(torch.zeros((8 - rows % 8, self.width), dtype=stack[0].dtype, device=stack[0].device))
-        self.proj = Linear(concat_rows(stack))
-        self.o = Linear(tensors[p + "o"])
+        self.proj = Linear(concat_rows(stack))          # (rates of the recurrence are among its rows: held as stored)
+        self.o = Linear(held(self.runtime, tensors[p + "o"]))
         self.conv_w = torch.cat([tensors[p + "q.conv"], tensors[p + "k.conv"], tensors[p + "v.conv"]]).contiguous()
         if self.by_channel:
             self.a2 = tensors[p + "a2"].contiguous()

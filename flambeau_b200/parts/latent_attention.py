@@ -5,7 +5,7 @@ import torch
 
 from ..kernels import ops
 from .base import KVRequirement, Mixer, TensorSpec
-from .linear import Linear, concat_rows
+from .linear import Linear, concat_rows, held
 from .spec import PartSpec, build_part, register_part
 
 
@@ -92,9 +92,9 @@ class LatentAttention(Mixer):
         self.gate_off = self.kv_off + (0 if self.shares_latent else self.hd)
         if rows % 8:          # rows of zeros up to a multiple of 8, so that the product's float32 rows stay 16-byte aligned
             stack.append(torch.zeros((8 - rows % 8, self.width), dtype=stack[0].dtype, device=stack[0].device))
-        self.proj = Linear(concat_rows(stack))
-        self.uq = Linear(tensors[p + "uq"]) if self.Rq else None
-        self.o = Linear(tensors[p + "o"])
+        self.proj = Linear(held(self.runtime, concat_rows(stack)))
+        self.uq = Linear(held(self.runtime, tensors[p + "uq"])) if self.Rq else None
+        self.o = Linear(held(self.runtime, tensors[p + "o"]))
         # per head: the map that carries a query into the latent is Wuk_h^T, stored with the latent as its outputs
         self.uk_t = tensors[p + "uk"].view(self.H, self.d, self.Rc).transpose(1, 2).contiguous()     # [H, Rc, d]
         self.uv = tensors[p + "uv"].view(self.H, self.e, self.Rc).contiguous()                      # [H, e, Rc]

@@ -8,10 +8,13 @@ from ..kernels import ops
 
 
 class Linear:
-    def __init__(self, weight: torch.Tensor):
+    """`weight`: a tensor, or a weight in a layout of its own (kernels.ops.PackedWeight)."""
+
+    def __init__(self, weight):
         if weight.dim() != 2:
             raise ValueError("a linear weight is 2-d [outputs, inputs]")
         self.weight = weight
+        self.packed = isinstance(weight, ops.PackedWeight)
         self.out_features, self.in_features = weight.shape
 
     def __call__(self, ctx, a: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
@@ -25,7 +28,26 @@ class Linear:
     def add_into(self, ctx, a: torch.Tensor, acc: torch.Tensor) -> bool:
         """acc += a W^T where the product's own epilogue can do the add (see ops.gemm_tc_add); False, with nothing
         done, where it cannot."""
-        return ops.gemm_tc_add(a, self.weight, acc, ctx.runtime.status, ctx.max_slabs)
+        return ops.linear_add(a, self.weight, acc, ctx, ctx.max_slabs)
+
+
+def held(runtime, weight: torch.Tensor):
+    """A map's weight ([outputs, inputs] or [groups, outputs, inputs]) as the runtime holds the large maps' weights
+    (Runtime.weight_format): as it is, or in four bits; in the 32-bit mode four-bit weights are held as the float32 numbers
+    that they stand for."""
+    if getattr(runtime, "weight_format", "stored") != "mxfp4":
+        return weight
+    if runtime.full_precision:
+        return ops.dequantize_mxfp4(*ops.quantize_mxfp4(weight.contiguous()), weight.shape[-1], torch.float32)
+    return ops.Mxfp4Weight.from_dense(weight)
+
+
+def held_groups(runtime, weights):
+    """`held` of the stacked weights of equal sizes, made one after the other."""
+    if getattr(runtime, "weight_format", "stored") == "mxfp4" and not runtime.full_precision:
+        rows = [ops.quantize_mxfp4(w.contiguous()) for w in weights]
+        return ops.Mxfp4Weight(torch.stack([r[0] for r in rows]), torch.stack([r[1] for r in rows]), weights[0].shape[-1])
+    return torch.stack([held(runtime, w) for w in weights]).contiguous()
 
 
 def interleave_rows(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:

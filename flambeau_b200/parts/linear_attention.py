@@ -5,7 +5,7 @@ import torch
 
 from ..kernels import ops
 from .base import Mixer, StateRequirement, TensorSpec
-from .linear import Linear, concat_rows
+from .linear import Linear, concat_rows, held
 from .spec import register_part
 
 
@@ -65,8 +65,8 @@ class GatedLinearAttention(Mixer):
         rows = sum(t.shape[0] for t in stack)
         if rows % 8:          # rows of zeros up to a multiple of 8, so that the product's float32 rows stay 16-byte aligned
             stack.append(torch.zeros((8 - rows % 8, self.width), dtype=stack[0].dtype, device=stack[0].device))
-        self.proj = Linear(concat_rows(stack))
-        self.o = Linear(tensors[p + "o"])
+        self.proj = Linear(concat_rows(stack))          # (rates of the recurrence are among its rows: held as stored)
+        self.o = Linear(held(self.runtime, tensors[p + "o"]))
         self.a2 = a2.contiguous()
         self.a2_b = tensors[p + "a2.b"].to(a2.dtype).contiguous()
         self.norm = tensors[p + "norm"]

@@ -5,7 +5,7 @@ import torch
 
 from ..kernels import ops
 from .base import FeedForward, TensorSpec
-from .linear import Linear, concat_rows, interleave_rows
+from .linear import Linear, concat_rows, held, held_groups, interleave_rows
 from .spec import PartSpec, build_part, register_part
 
 
@@ -118,11 +118,11 @@ class RoutedExperts(FeedForward):
     def own_bind(self, tensors):
         p = self.prefix
         if self.gated:      # gate and up rows alternate, so that the product's epilogue finds a gate beside its up
-            self.up = torch.stack([interleave_rows(tensors[f"{p}e{e}.gate"], tensors[f"{p}e{e}.up"])
-                                   for e in range(self.E)]).contiguous()                           # [E, 2 inner, width]
+            self.up = held_groups(self.runtime, [interleave_rows(tensors[f"{p}e{e}.gate"], tensors[f"{p}e{e}.up"])
+                                                 for e in range(self.E)])                          # [E, 2 inner, width]
         else:
-            self.up = torch.stack([tensors[f"{p}e{e}.up"] for e in range(self.E)]).contiguous()    # [E, inner, width]
-        self.down = torch.stack([tensors[f"{p}e{e}.down"] for e in range(self.E)]).contiguous()    # [E, width, inner]
+            self.up = held_groups(self.runtime, [tensors[f"{p}e{e}.up"] for e in range(self.E)])   # [E, inner, width]
+        self.down = held_groups(self.runtime, [tensors[f"{p}e{e}.down"] for e in range(self.E)])   # [E, width, inner]
         # the router and the shared expert's gate are one product: the gate's row lies behind the experts' rows
         # (then rows of zeros up to a multiple of 8, so that the product's float32 rows stay 16-byte aligned)
         rows = [tensors[p + "router"]]
@@ -134,8 +134,8 @@ class RoutedExperts(FeedForward):
         self.router = Linear(concat_rows(rows))
         self.router_b = tensors[p + self.bias_name].to(rows[0].dtype).contiguous() if self.router_bias else None
         if self.shared_inner:
-            self.shared_up = Linear(tensors[p + "shared.up"])
-            self.shared_down = Linear(tensors[p + "shared.down"])
+            self.shared_up = Linear(held(self.runtime, tensors[p + "shared.up"]))
+            self.shared_down = Linear(held(self.runtime, tensors[p + "shared.down"]))
 
     def own_weights(self):
         # a step reads the router, the shared expert, and of the routed experts at most what its tokens choose
@@ -145,7 +145,7 @@ class RoutedExperts(FeedForward):
         return w
 
     def weight_bytes(self) -> int:
-        per_expert = (self.up[0].numel() + self.down[0].numel()) * self.up.element_size()
+        per_expert = (self.up.nbytes + self.down.nbytes) // self.E
         return super().weight_bytes() + self.K * per_expert         # one token's worth; a batch reads more experts
 
     def _shared_part(self, ctx, h, n):

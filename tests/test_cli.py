@@ -5,6 +5,8 @@ import subprocess
 import sys
 from pathlib import Path
 
+import pytest
+
 import tiny
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -61,3 +63,14 @@ def test_bench_subcommand_keeps_the_contract_for_more_than_one_gpu(capsys):
     assert main(["bench", "--impl", "reference"]) == 0
     line = json.loads(capsys.readouterr().out)
     assert line["impl"] == "reference" and "unavailable" in line
+
+
+def test_weight_formats_are_named_and_others_refused(capsys):
+    from flambeau_b200.cli import main
+    from flambeau_b200.engine.runtime import Runtime, parse_weight_format
+    assert [parse_weight_format(n) for n in ("stored", "mxfp4")] == ["stored", "mxfp4"]
+    with pytest.raises(ValueError, match="weights must be one of"):
+        Runtime("cuda:0", weights="int4")
+    with pytest.raises(SystemExit):
+        main(["infer", "--model", "nowhere", "--prompt", "1", "--weights", "int4"])
+    assert "mxfp4" in capsys.readouterr().err
