@@ -147,6 +147,62 @@ __device__ __forceinline__ float silu_times(float g, float u) {
     return g * r * u;
 }
 
+// The shares of a row tile, n_tok x 128 float32 each, added in order; a thread has four neighbouring features of a token.  (As the epilogue's own lanes lie, one share after the other, this took 4 us of a call.)
+__device__ __noinline__ void join_shares(const MxArgs& a, const Unit& w, int tid, int rows, const float* __restrict__ base) {
+    const size_t step = (size_t)a.bn * (MX_ROWS / 4);
+    const int shift = a.shifts[w.group];
+    const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
+    constexpr int U = 4;                         // sums of a thread at a time, two shares of each on their way
+    const int all = rows * (MX_ROWS / 4);
+    for (int e0 = tid; e0 < all; e0 += U * EPI) {
+        float4 sum[U];
+#pragma unroll
+        for (int q = 0; q < U; ++q) sum[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4* p = reinterpret_cast<const float4*>(base) + e0;
+        for (int s = 0; s < w.shares; s += 2, p += 2 * step) {
+            float4 t[2][U];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < U; ++q)
+                    t[h][q] = s + h < w.shares && e0 + q * EPI < all ? __ldcg(p + h * step + q * EPI) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    sum[q].x += t[h][q].x; sum[q].y += t[h][q].y; sum[q].z += t[h][q].z; sum[q].w += t[h][q].w;
+                }
+        }
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            const int e = e0 + q * EPI;
+            if (e >= all) break;
+            const int m = w.m0 + e / (MX_ROWS / 4), n = w.nt * MX_ROWS + 4 * (e % (MX_ROWS / 4));
+            float v[4] = {sum[q].x * raise, sum[q].y * raise, sum[q].z * raise, sum[q].w * raise};
+            int count = 4, columns = a.N, col = n;
+            if (a.gate.act) {                    // features alternate gate, up
+                v[0] = a.gate.act == FB_ACT_SILU ? silu_times(v[0], v[1]) : fb_gate_times(a.gate, v[0], v[1]);
+                v[1] = a.gate.act == FB_ACT_SILU ? silu_times(v[2], v[3]) : fb_gate_times(a.gate, v[2], v[3]);
+                count = 2; columns = a.N / 2; col = n / 2;
+            } else if (a.plain_act) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = fb_plain_act(a.plain_act, v[i]);
+            }
+            const size_t at = (size_t)m * a.ldo + col;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i >= count || col + i >= columns) break;
+                if (a.o_bf16) {
+                    reinterpret_cast<__nv_bfloat16*>(a.out)[at + i] = __float2bfloat16_rn(v[i]);
+                } else {
+                    float* o = reinterpret_cast<float*>(a.out) + at + i;
+                    *o = a.accumulate ? *o + v[i] : v[i];
+                }
+            }
+        }
+    }
+}
+
 template <int TOK, bool GROUPED>
 __global__ void __launch_bounds__(Form<TOK>::THREADS, 1)
 gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_o,
@@ -439,7 +495,6 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             const bool both = w.n_tok <= SIDE_BY_SIDE, join = !GROUPED && w.shares > 1 && a.slabs == 0;
             const int b = j & 1, n0 = w.nt * MX_ROWS, n = n0 + row;
             const int rows = min(w.n_tok, a.M - w.m0);                   // (grouped: whole tiles)
-            const float* from = nullptr;                                 // where shares are joined: the first one of this tile
             if (bailed() || !wait(&acc_full[b], (uint32_t)(j >> 1) & 1u)) *bail = 1;
             asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
             if (tid == 0) *flag = bailed() ? 2 : 0;                      // one thread decides for all: they meet at barriers below
@@ -475,28 +530,16 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
                 if (*flag == 1) {
                     __threadfence();
-                    from = a.partials + (size_t)w.id * a.max_segments * (size_t)(a.bn * MX_ROWS) + row;
+                    join_shares(a, w, tid, rows, a.partials + (size_t)w.id * a.max_segments * (size_t)(a.bn * MX_ROWS));
                 }
-            }
-            if (!join || from) {
+            } else {
                 const int shift = a.shifts[w.group];
                 const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
                 const int slab = a.slabs ? w.share : 0;
 #pragma unroll 1
                 for (int c = half * OUT_TOKENS; c < rows; c += STEP) {
                     float v[16];
-                    if (from) {
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) v[q] = 0.0f;
-                        for (int s = 0; s < w.shares; ++s) {
-                            const float* p = from + ((size_t)s * a.bn + c) * MX_ROWS;
-#pragma unroll
-                            for (int q = 0; q < 16; ++q)
-                                if (c + q < rows) v[q] += __ldcg(p + q * MX_ROWS);
-                        }
-                    } else {
-                        sums(c, v);
-                    }
+                    sums(c, v);
                     if (shift > 0) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) v[q] *= raise;
@@ -588,12 +631,14 @@ int segments_of(long tiles_n, long kb, long grid) {           // the most stretc
 }
 // CTAs, one an SM, each with a few tiles at least, and the most stretches that they cut a row tile into: as many CTAs as leave no
 // more than `limit`.
-constexpr int ANY = 1 << 30, LEAST_ITEMS = 4;
+// Where shares have to meet (`join`), row tiles stay whole if the longest stretch and the meeting take longer.  In cycles: STAGE for
+// a tile of an SM, JOIN for the partial sums' way through L2 and back.
+constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 4000;
 struct Cut { int grid, segments; };
-Cut cut_of(int tiles_n, int kb, int limit) {
+Cut cut_of(int tiles_n, int kb, int limit, bool join) {
     static std::map<std::tuple<int, int, int, int>, Cut> known;              // (counting through the tiles takes microseconds)
     static std::mutex mu;
-    const std::tuple<int, int, int, int> key{tiles_n, kb, limit, fb_sm_count()};
+    const std::tuple<int, int, int, int> key{tiles_n, kb, join ? -limit : limit, fb_sm_count()};
     std::lock_guard<std::mutex> lock(mu);
     const auto it = known.find(key);
     if (it != known.end()) return it->second;
@@ -601,6 +646,10 @@ Cut cut_of(int tiles_n, int kb, int limit) {
     long grid = most < slots ? most : slots;
     int segments = segments_of(tiles_n, kb, grid);
     while (segments > limit && grid > 1) segments = segments_of(tiles_n, kb, --grid);
+    if (join && segments > 1 && tiles_n <= slots && ((long)tiles_n * kb + grid - 1) / grid * STAGE + JOIN >= (long)kb * STAGE) {
+        grid = tiles_n;
+        segments = 1;
+    }
     if (known.size() > 4096) known.clear();
     return known[key] = Cut{(int)grid, segments};
 }
@@ -647,7 +696,7 @@ template <int TOK, bool GROUPED> int launch(const MxArgs& a, const CUtensorMap& 
         if (e != cudaSuccess) return fb_fail(-2, "gemm_mxfp4: cannot reserve shared memory: %s", cudaGetErrorString(e));
         fb_setup_done(configured);
     }
-    fb_launch_class(Form<TOK>::WIDE ? FB_LAUNCH_GEMM_WIDE : FB_LAUNCH_OTHER, kernel, dim3((unsigned)grid), dim3(Form<TOK>::THREADS), SMEM, stream, mx, mo, a);
+    fb_launch_class(a.M > 128 && Form<TOK>::WIDE ? FB_LAUNCH_GEMM_WIDE : FB_LAUNCH_OTHER, kernel, dim3((unsigned)grid), dim3(Form<TOK>::THREADS), SMEM, stream, mx, mo, a);
     return fb_check_launch("gemm_mxfp4");
 }
 
@@ -657,12 +706,10 @@ long long scale_bytes_of(int M, int kb, bool grouped) {
 }
 
 // The rows' parts and scales in `scratch`, their map, the output's map.
-int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, long long scratch_bytes, int box_rows, cudaStream_t stream) {
+int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, int box_rows, cudaStream_t stream) {
     const bool grouped = a.tile_group != nullptr;
     const long Kp = (long)a.kb * MX_COLS, parts = 2L * a.M * Kp;
     a.scale_rows = (a.M + 3) / 4 * 4;
-    FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= parts + scale_bytes_of(a.M, a.kb, grouped),
-               "gemm_mxfp4: scratch for the rows' parts missing");
     a.x_scales = (const uint8_t*)scratch + parts;
     a.atoms = atoms_of(a.bn);
     const MxScaleLayout layout = {grouped ? 0 : a.bn, grouped ? 0 : a.atoms * ATOM, a.scale_rows};
@@ -670,6 +717,8 @@ int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, long lon
     if (rc) return rc;
     rc = fb_tensor_map_bf16(&mx, scratch, 2L * a.M, Kp / 2, Kp / 2, 64, box_rows);       // (bytes, two at a time)
     if (rc) return rc;
+    a.boxed = 0;
+    if (box_rows <= NARROW_TOKENS && (!grouped || a.tile == 16)) return 0;               // (the narrow form stores directly)
     rc = fb_tensor_map_out(&mo, a.out, a.o_bf16 ? 2 : 4, a.M, a.gate.act ? a.N / 2 : a.N, a.ldo, a.slabs ? a.slabs : 1, a.slab_stride,
                            a.gate.act ? MX_ROWS / 2 : MX_ROWS, OUT_TOKENS);
     a.boxed = rc == 0;
@@ -692,37 +741,41 @@ int check_operands(const void* X, long long lda, const void* W, const int* shift
 
 }  // namespace
 
-// Bytes of `scratch` that the products below want for M rows of K (tile: the grouped form's row tile, 0: not grouped).
-FB_API long long fb_gemm_mxfp4_rows_bytes(int M, int K, int tile) {
+// What the rows' parts and their scales take, a multiple of 256 bytes (tile: the grouped form's row tile, 0: not grouped).
+static long long rows_bytes(int M, int K, int tile) {
     if (M <= 0 || K <= 0) return 0;
     const long long kb = (K + MX_COLS - 1) / MX_COLS;
-    return 2LL * M * kb * MX_COLS + scale_bytes_of(M, (int)kb, tile > 0);
+    return (2LL * M * kb * MX_COLS + scale_bytes_of(M, (int)kb, tile > 0) + 255) / 256 * 256;
 }
 
-// Floats of `partials` that fb_gemm_mxfp4 wants for the same sizes with `n_counters` counters and without slabs: 0 where K is not
-// split.
-FB_API long long fb_gemm_mxfp4_share_floats(int M, int N, int K, int n_counters) {
+// Floats that shares of K take which meet in scratch: 0 where K is not split.
+static long long share_floats(int M, int N, int K, int n_counters) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
     const int tiles_n = (N + MX_ROWS - 1) / MX_ROWS, kb = (K + MX_COLS - 1) / MX_COLS;
     if (M <= NARROW_TOKENS) {
-        const int segments = tiles_n <= n_counters ? cut_of(tiles_n, kb, ANY).segments : 1;
+        const int segments = tiles_n <= n_counters ? cut_of(tiles_n, kb, ANY, true).segments : 1;
         return segments > 1 ? (long long)tiles_n * segments * narrow_tokens(M) * MX_ROWS : 0;
     }
     const Plan p = plan_wide(M, N, kb, MOST_SPLITS, SHARE_FLOATS, n_counters, false);
     return p.splits == 1 ? 0 : (long long)((M + p.bn - 1) / p.bn) * tiles_n * p.splits * p.bn * MX_ROWS;
 }
 
+// Bytes of `scratch` that the products below want for M rows, with `n_counters` counters.  slabs: shares of K go to slabs; tile: the
+// grouped form's row tile (0: not grouped).
+FB_API long long fb_gemm_mxfp4_scratch_bytes(int M, int N, int K, int n_counters, int slabs, int tile) {
+    return rows_bytes(M, K, tile) + (slabs || tile ? 0 : 4 * share_floats(M, N, K, n_counters));
+}
+
 // X [M,K] bfloat16, W one matrix in tiles with its shift (fb_mxfp4_tiles).  `act` (an FbAct code with its constants): W stacks gate
 // and up rows alternately and out[m, c] = act(g_c) u_c has N / 2 columns; `plain_act` (an FbPlainAct code): out = act(product);
 // `accumulate` (float32): the product is added to what `out` holds.  Shares of K: with slab_stride > 0 (float32, neither activation
 // nor accumulate) share s goes to out + s * slab_stride and *splits_used says how many there are (at most max_slabs); else they
-// meet in `partials` and `counters` (zero before the call and after it), the scratch of calls that run one after the other;
-// without it, or with fewer floats than fb_gemm_mxfp4_share_floats asks for, K is not split.  `scratch`: fb_gemm_mxfp4_rows_bytes
-// (M, K, 0) bytes on a 128-byte border.
+// meet in `scratch` and at `counters` (zero before the call and after it).  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a
+// 128-byte border, of calls that run one after the other.
 FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int* shifts, void* out, int o_dtype, long long ldo,
                          long long slab_stride, int max_slabs, int* splits_used, int M, int N, int K, int act, float limit,
-                         float slope, int plain_act, int accumulate, float* partials, long long partial_floats, int* counters,
-                         int n_counters, void* scratch, long long scratch_bytes, int* status, cudaStream_t stream) {
+                         float slope, int plain_act, int accumulate, int* counters, int n_counters, void* scratch,
+                         long long scratch_bytes, int* status, cudaStream_t stream) {
     const FbGate gate = {act, limit, slope};
     if (const int rc = check_operands(X, lda, W, shifts, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
     FB_REQUIRE(slab_stride == 0 || (o_dtype == FB_F32 && max_slabs >= 1 && slab_stride >= (long long)M * ldo && !act && !plain_act && !accumulate),
@@ -733,14 +786,18 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
     MxArgs a = {};
     a.W = (const uint8_t*)W; a.shifts = shifts; a.out = out; a.ldo = (long)ldo; a.slab_stride = (long)slab_stride;
     a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, nullptr, nullptr, nullptr};
-    a.o_bf16 = o_dtype == FB_BF16; a.accumulate = accumulate; a.partials = partials; a.counters = counters;
+    a.o_bf16 = o_dtype == FB_BF16; a.accumulate = accumulate; a.counters = counters;
     a.M = M; a.N = N; a.K = K; a.kb = (K + MX_COLS - 1) / MX_COLS; a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
     const bool slabs = slab_stride > 0;
-    const bool join = !slabs && partials && counters && partial_floats >= fb_gemm_mxfp4_share_floats(M, N, K, n_counters);
+    const long long need = fb_gemm_mxfp4_scratch_bytes(M, N, K, n_counters, slabs, 0), rows = rows_bytes(M, K, 0);
+    FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= need && (slabs || (counters && n_counters > 0)),
+               "gemm_mxfp4: %lld bytes of scratch wanted, and counters", need);
+    a.partials = need > rows ? (float*)((uint8_t*)scratch + rows) : nullptr;
+    const bool join = a.partials != nullptr;
     CUtensorMap mx = {}, mo = {};
     if (M <= NARROW_TOKENS) {
-        const Cut cut = cut_of(a.tiles_n, a.kb, slabs ? max_slabs : join && a.tiles_n <= n_counters ? ANY : 1);
+        const Cut cut = cut_of(a.tiles_n, a.kb, slabs ? max_slabs : join ? ANY : 1, !slabs);
         a.bn = narrow_tokens(M);
         a.tiles_m = 1; a.splits = 1; a.items = (long)a.tiles_n * a.kb;
         a.max_segments = cut.segments;
@@ -748,7 +805,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
             a.slabs = cut.segments;
             if (splits_used) *splits_used = cut.segments;
         }
-        if (const int rc = prepare(a, mx, mo, scratch, scratch_bytes, a.bn, stream)) return rc;
+        if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
         return launch<32, false>(a, mx, mo, cut.grid, stream);
     }
     const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, SHARE_FLOATS,
@@ -762,7 +819,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
     }
     a.items = (long)a.tiles_m * a.tiles_n * a.splits;
     if (a.items > 2000000000L) return fb_fail(-1, "gemm_mxfp4: too many tiles (M=%d N=%d)", M, N);
-    if (const int rc = prepare(a, mx, mo, scratch, scratch_bytes, a.bn, stream)) return rc;
+    if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
     const long grid = a.items < fb_sm_count() ? a.items : fb_sm_count();
     return a.bn <= 64 ? launch<64, false>(a, mx, mo, grid, stream) : launch<128, false>(a, mx, mo, grid, stream);
 }
@@ -770,7 +827,8 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
 // The grouped form: W holds `groups` matrices [N, K] in tiles with a shift each; the M rows of `out` come in tiles of `tile` (a
 // multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are).  Row m is
 // X[m], or with row_index X[row_index[m]] (negative: zeros), with row_share times row_share[row_pair[m]].  `scratch`:
-// fb_gemm_mxfp4_rows_bytes(M, K, tile) bytes.
+// at least
+// fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
 FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_index, const float* row_share, const int* row_pair,
                                  const void* W, const int* shifts, int groups, const int* tile_group, int tile, void* out, int o_dtype,
                                  long long ldo, int M, int N, int K, int act, float limit, float slope, int plain_act, void* scratch,
@@ -781,6 +839,7 @@ FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_in
     FB_REQUIRE(tile >= 16 && tile <= 128 && tile % 16 == 0 && M % tile == 0 && M / tile < (1 << 24),
                "gemm_mxfp4_grouped: the rows must be whole tiles of 16 to 128, not tiles of %d", tile);
     FB_REQUIRE(!row_share || (row_index && row_pair), "gemm_mxfp4_grouped: shares need the rows' index and pairs");
+    FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= rows_bytes(M, K, tile), "gemm_mxfp4_grouped: scratch missing");
     if (M == 0) return 0;
     MxArgs a = {};
     a.kb = (K + MX_COLS - 1) / MX_COLS;
@@ -795,7 +854,7 @@ FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_in
     CUtensorMap mx = {}, mo = {};
     const bool narrow = tile == 16;
     a.bn = (narrow ? NARROW_TOKENS : WIDE_TOKENS) / tile * tile;
-    if (const int rc = prepare(a, mx, mo, scratch, scratch_bytes, tile, stream)) return rc;
+    if (const int rc = prepare(a, mx, mo, scratch, tile, stream)) return rc;
     const long grid = units < fb_sm_count() ? units : fb_sm_count();
     return narrow ? launch<32, true>(a, mx, mo, grid, stream) : launch<128, true>(a, mx, mo, grid, stream);
 }

@@ -10,6 +10,8 @@
 // a row.
 #include "mxfp4.cuh"
 
+#include <cuda_fp16.h>
+
 namespace {
 
 // Eight numbers of a row from column c on; zeros beyond K.
@@ -28,7 +30,61 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-// VEC: rows start on 16-byte borders (and their strides keep them there).
+// One quarter of a block: eight numbers into codes; the lanes of a block are neighbours.  Every lane of the warp.
+__device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& scale) {
+    uint32_t top = 0;                                                    // the largest magnitude's bits (NaN above infinity)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int s = min(MX_LAST_SCALE, max(0, (int)(top >> 23) - 2 + ((top & 0x7fffffu) >= 0x600000u ? 1 : 0)));
+    const float inv = __uint_as_float((uint32_t)(254 - s) << 23);        // 2^(127 - s)
+    uint32_t out;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(out)
+        : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv),
+          "f"(v[7] * inv));
+    const bool finite = top < 0x7f800000u;
+    scale = finite ? (uint32_t)s : 255u;
+    return finite ? out : 0u;
+}
+
+// Rows of whole blocks, one behind the other on 16-byte borders: UNROLL quarters a thread, all fetched before the first is used.
+// (28,672 x 4,096 bfloat16 with the form below: 94 us, of which 45 are memory's; like this QUANTUS.)
+constexpr int UNROLL = 4;
+template <typename T>
+__global__ void __launch_bounds__(256)
+quantize_flat_kernel(const T* __restrict__ x, long quarters, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    fb_pdl_launch_dependents();
+    fb_pdl_wait();
+    const long first = (long)blockIdx.x * (256 * UNROLL) + threadIdx.x;
+    float v[UNROLL][8];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const long q = first + 256 * u;
+        if (q < quarters) load8(x + 8 * q, v[u]);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const long q = first + 256 * u;
+        uint32_t scale;
+        const uint32_t out = quantize8(v[u], scale);
+        if (q < quarters) {
+            reinterpret_cast<uint32_t*>(codes)[q] = out;
+            if ((q & 3) == 0) scales[q >> 2] = (uint8_t)scale;
+        }
+    }
+}
+
+// Any rows.  VEC: they start on 16-byte borders.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 quantize_kernel(const T* __restrict__ x, long ldx, long rows, int K, int blocks, uint8_t* __restrict__ codes,
@@ -50,38 +106,53 @@ quantize_kernel(const T* __restrict__ x, long ldx, long rows, int K, int blocks,
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = mine && c + i < K ? fb_to_float(p[i]) : 0.0f;
         }
-        uint32_t top = 0;                                                // the largest magnitude's bits (NaN above infinity)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int s = min(MX_LAST_SCALE, max(0, (int)(top >> 23) - 2 + ((top & 0x7fffffu) >= 0x600000u ? 1 : 0)));
-        const bool finite = top < 0x7f800000u;
-        const float inv = __uint_as_float((uint32_t)(254 - s) << 23);    // 2^(127 - s)
-        uint32_t out = 0;
-        if (finite) {
-            asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
-                "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
-                : "=r"(out)
-                : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
-                  "f"(v[6] * inv), "f"(v[7] * inv));
-        }
+        uint32_t scale;
+        const uint32_t out = quantize8(v, scale);
         if (mine) {
             reinterpret_cast<uint32_t*>(codes)[q] = out;                 // (quarters of a row follow one another)
-            if ((q & 3) == 0) scales[q >> 2] = finite ? (uint8_t)s : 255;
+            if ((q & 3) == 0) scales[q >> 2] = (uint8_t)scale;
         }
     }
 }
 
-__device__ __forceinline__ float code_value(uint32_t code, float scale) {
-    const uint32_t m = code & 7u;
-    const float v = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-    return copysignf(v, code & 8u ? -1.0f : 1.0f) * scale;
+// Eight codes into the numbers that they stand for.
+template <typename T>
+__device__ __forceinline__ void dequantize8(uint32_t w, float scale, T (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t pair;                                                   // (two codes of a byte in float16)
+        asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\t}" : "=r"(pair) : "r"(w >> (8 * i)));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+        v[2 * i] = fb_from_float<T>(f.x * scale);
+        v[2 * i + 1] = fb_from_float<T>(f.y * scale);
+    }
 }
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+dequantize_flat_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long quarters, T* __restrict__ out) {
+    fb_pdl_launch_dependents();
+    fb_pdl_wait();
+    const long first = (long)blockIdx.x * (256 * UNROLL) + threadIdx.x;
+    uint32_t w[UNROLL], s[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const long q = first + 256 * u;
+        w[u] = q < quarters ? reinterpret_cast<const uint32_t*>(codes)[q] : 0u;
+        s[u] = q < quarters ? scales[q >> 2] : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const long q = first + 256 * u;
+        alignas(16) T v[8];
+        dequantize8(w[u], mx_scale_f32(s[u]), v);
+        if (q < quarters) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(v) / 16; ++i) reinterpret_cast<uint4*>(out + 8 * q)[i] = reinterpret_cast<const uint4*>(v)[i];
+        }
+    }
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long rows, int K, int blocks,
@@ -92,11 +163,8 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     for (long q = (long)blockIdx.x * 256 + threadIdx.x; q < quarters; q += step) {
         const long row = q / (blocks * 4);
         const int c = 8 * (int)(q - row * (blocks * 4));
-        const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[q];
-        const float scale = mx_scale_f32(scales[q >> 2]);
-        T v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fb_from_float<T>(code_value(w >> (4 * i) & 15u, scale));
+        alignas(16) T v[8];
+        dequantize8(reinterpret_cast<const uint32_t*>(codes)[q], mx_scale_f32(scales[q >> 2]), v);
         T* p = out + row * ldo + c;
         if (VEC && c + 8 <= K) {
 #pragma unroll
@@ -210,6 +278,12 @@ FB_API int fb_quantize_mxfp4(const void* x, int dtype, long long ldx, long long 
     const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     FB_DISPATCH_DTYPE(dtype, T, {
         const bool vec = ((uintptr_t)x & 15) == 0 && (rows == 1 || ldx * sizeof(T) % 16 == 0);
+        if (vec && K % MX_BLOCK == 0 && (rows == 1 || ldx == K) && rows * blocks < (1LL << 36)) {
+            const long quarters = (long)rows * blocks * 4, per = 256 * UNROLL;
+            fb_launch((quantize_flat_kernel<T>), dim3((unsigned)((quarters + per - 1) / per)), dim3(256), 0, stream, (const T*)x, quarters,
+                      (uint8_t*)codes, (uint8_t*)scales);
+            return fb_check_launch("quantize_mxfp4");
+        }
         auto kernel = vec ? quantize_kernel<T, true> : quantize_kernel<T, false>;
         fb_launch(kernel, dim3(grid_of((long)rows * blocks * 4, 256)), dim3(256), 0, stream, (const T*)x, (long)ldx, (long)rows, K,
                   blocks, (uint8_t*)codes, (uint8_t*)scales);
@@ -228,6 +302,12 @@ FB_API int fb_dequantize_mxfp4(const void* codes, const void* scales, long long 
     const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK;
     FB_DISPATCH_DTYPE(dtype, T, {
         const bool vec = ((uintptr_t)out & 15) == 0 && (rows == 1 || ldo * sizeof(T) % 16 == 0);
+        if (vec && K % MX_BLOCK == 0 && (rows == 1 || ldo == K) && rows * blocks < (1LL << 36)) {
+            const long quarters = (long)rows * blocks * 4, per = 256 * UNROLL;
+            fb_launch((dequantize_flat_kernel<T>), dim3((unsigned)((quarters + per - 1) / per)), dim3(256), 0, stream, (const uint8_t*)codes,
+                      (const uint8_t*)scales, quarters, (T*)out);
+            return fb_check_launch("dequantize_mxfp4");
+        }
         auto kernel = vec ? dequantize_kernel<T, true> : dequantize_kernel<T, false>;
         fb_launch(kernel, dim3(grid_of((long)rows * blocks * 4, 256)), dim3(256), 0, stream, (const uint8_t*)codes,
                   (const uint8_t*)scales, (long)rows, K, blocks, (T*)out, (long)ldo);

@@ -74,6 +74,15 @@ class Workspace:
         for s in shape:
             n *= s
         nbytes = n * _ELEMENT_SIZE[dtype]
+        start = self._take(nbytes)
+        return self.buffer[start:start + nbytes].view(dtype).view(shape)
+
+    def reserve(self, nbytes: int) -> int:
+        """The address of `nbytes` of the arena: scratch of a launcher, which needs no tensor."""
+        start = self._take(nbytes)               # (which may replace the buffer)
+        return self.buffer.data_ptr() + start
+
+    def _take(self, nbytes: int) -> int:
         start = (self.top + self.ALIGN - 1) // self.ALIGN * self.ALIGN
         end = start + nbytes
         if end > self.buffer.numel():
@@ -84,7 +93,7 @@ class Workspace:
             # older tensors keep the previous storage; this step continues in the new one
         self.top = end
         self.high_water = max(self.high_water, end)
-        return self.buffer[start:end].view(dtype).view(shape)
+        return start
 
     def mark(self) -> int:
         return self.top

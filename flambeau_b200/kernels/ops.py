@@ -611,6 +611,7 @@ def tc_supported(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> bool:
 
 
 _SPLITS_USED = ctypes.c_int(1)
+_SPLITS_USED_REF = ctypes.byref(_SPLITS_USED)
 
 
 def gemm_tc(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, status: torch.Tensor, splits: int = 0,
@@ -1685,6 +1686,7 @@ class Mxfp4Weight(PackedWeight):
         self.device = codes.device
         self.tiles = torch.empty(groups * lib().fb_mxfp4_tile_bytes(outputs, int(inputs)), dtype=torch.uint8, device=codes.device)
         self.shifts = torch.empty(groups, dtype=torch.int32, device=codes.device)
+        self._tiles, self._shifts, self._scratch = self.tiles.data_ptr(), self.shifts.data_ptr(), {}
         check(lib().fb_mxfp4_tiles(codes.data_ptr(), scales.data_ptr(), groups, outputs, int(inputs), self.tiles.data_ptr(),
                                    self.shifts.data_ptr(), _stream()), "mxfp4_tiles")
 
@@ -1707,7 +1709,6 @@ class Mxfp4Weight(PackedWeight):
 
     def _operands(self, a: torch.Tensor, out: torch.Tensor, columns: int, what: str, indexed: bool = False) -> tuple:
         """Checks what a product takes: a [M, K] bfloat16, out [M, columns] float32 or bfloat16, rows dense.  (M, N, K)."""
-        _cuda(a, out)
         N, K = self.shape[-2:]
         if a.dim() != 2 or out.dim() != 2 or a.shape[1] != K or out.shape[1] != columns \
                 or (out.shape[0] != a.shape[0] and not indexed):
@@ -1723,19 +1724,28 @@ class Mxfp4Weight(PackedWeight):
     def _product(self, a, out, ctx, columns: int, what: str, gate=(0, 0.0, 0.0), plain_act: int = 0, accumulate: bool = False,
                  slabs=None) -> int:
         M, N, K = self._matrix(a, out, columns, what)
-        ws, used = ctx.ws, ctypes.c_int(1)
+        ws = ctx.ws
         counters = ws.counters
-        with ws.scope():
-            floats = 0 if slabs is not None else lib().fb_gemm_mxfp4_share_floats(M, N, K, counters.numel())
-            partials = ws.alloc((floats,), torch.float32) if floats > 0 else None
-            nbytes = lib().fb_gemm_mxfp4_rows_bytes(M, K, 0)
-            parts = ws.alloc((nbytes,), torch.uint8) if nbytes > 0 else None
-            check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self.tiles.data_ptr(), self.shifts.data_ptr(), out.data_ptr(),
-                                      dtype_code(out), _rows(out), slabs.stride(0) if slabs is not None else 0,
-                                      slabs.shape[0] if slabs is not None else 0, ctypes.byref(used), M, N, K, *gate, plain_act,
-                                      1 if accumulate else 0, _ptr(partials), floats, counters.data_ptr(), counters.numel(),
-                                      _ptr(parts), nbytes, ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
-        return used.value
+        nbytes = self._scratch_bytes(M, counters.numel(), slabs is not None, 0)
+        mark = ws.mark()
+        try:
+            check(lib().fb_gemm_mxfp4(a.data_ptr(), a.stride(0), self._tiles, self._shifts, out.data_ptr(), _CODES[out.dtype], out.stride(0),
+                                      slabs.stride(0) if slabs is not None else 0, slabs.shape[0] if slabs is not None else 0,
+                                      _SPLITS_USED_REF, M, N, K, *gate, plain_act, accumulate, counters.data_ptr(), counters.numel(),
+                                      ws.reserve(nbytes), nbytes, ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
+        finally:
+            ws.release(mark)
+        return _SPLITS_USED.value
+
+    def _scratch_bytes(self, M: int, counters: int, slabs: bool, tile: int) -> int:
+        """What the products want of the arena for M rows (asked of the library once per number of rows)."""
+        key = (M, counters, slabs, tile)
+        nbytes = self._scratch.get(key)
+        if nbytes is None:
+            if len(self._scratch) > 4096:
+                self._scratch.clear()
+            nbytes = self._scratch[key] = lib().fb_gemm_mxfp4_scratch_bytes(M, *self.shape[-2:], counters, slabs, tile)
+        return nbytes
 
     def linear(self, a, out, ctx) -> None:
         self._product(a, out, ctx, self.shape[-2], "linear")
@@ -1792,11 +1802,13 @@ class Mxfp4Weight(PackedWeight):
         self._operands(a, out, N // 2 if gate is not None else N, what, indexed=row_index is not None)
         gate_args = gate_arguments(gate) if gate is not None else (0, 0.0, 0.0)
         ws = ctx.ws
-        with ws.scope():
-            nbytes = lib().fb_gemm_mxfp4_rows_bytes(M, K, int(tile))
-            parts = ws.alloc((nbytes,), torch.uint8) if nbytes > 0 else None
-            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), _ptr(row_index), _ptr(row_share), _ptr(row_pair),
-                                              self.tiles.data_ptr(), self.shifts.data_ptr(), self.shape[0], tile_group.data_ptr(),
-                                              int(tile), out.data_ptr(), dtype_code(out), _rows(out), M, N, K, *gate_args,
-                                              plain_activation_code(activation_name), _ptr(parts), nbytes,
+        nbytes = self._scratch_bytes(M, 0, False, int(tile))
+        mark = ws.mark()
+        try:
+            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), _ptr(row_index), _ptr(row_share), _ptr(row_pair), self._tiles,
+                                              self._shifts, self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(),
+                                              dtype_code(out), _rows(out), M, N, K, *gate_args,
+                                              plain_activation_code(activation_name), ws.reserve(nbytes), nbytes,
                                               ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4_grouped", (M, N, K))
+        finally:
+            ws.release(mark)
