@@ -39,9 +39,10 @@ constexpr int A_COLS = MX_COLS / 4;               // tensor-memory columns of a 
 constexpr int SFA_COLS = 4;
 constexpr int MAX_W = 16, MAX_R = 8;              // most stages of packed weights / of rows and decoded weights
 constexpr int LIST = 512;                         // units of the grouped form that are kept in shared memory
-constexpr int OUT_TOKENS = 16;
-constexpr int OUT_BYTES = OUT_TOKENS * MX_ROWS * 4;       // a staged box of the output
-constexpr int CONTROL = 512 + 4 * LIST;           // barriers and flags, the list
+constexpr int CHUNK = 16;                         // tokens that a group of four epilogue warps takes at a time
+constexpr int OUT_BYTES = 4096, OUT_BUFFERS = 3;  // a staged box of the output: 16 tokens, 8 of ungated float32
+constexpr int FLAGS = 640;                        // bytes of barriers and flags
+constexpr int CONTROL = FLAGS + 4 * LIST;         // and the list
 constexpr int NARROW_TOKENS = 32, WIDE_TOKENS = 128;      // most tokens of a tile of either form
 constexpr int SIDE_BY_SIDE = 64;                  // most tokens whose two parts are one operand
 constexpr int ATOM = 512;                         // scales of 128 rows for a stage, as tcgen05.cp brings them to tensor memory
@@ -51,38 +52,47 @@ constexpr int TMEM = 512, SMEM = 227 * 1024;
 // TOK: most tokens of a tile.  R stages of rows and decoded weights, GROUPS of four decoding warps: a stage is 1,500 cycles on its way
 // from the first look at its weights to the end of its MMAs, of which a group works on it for half, so that it takes
 // four groups and eight stages to keep up with memory where the MMAs are short.
-template <int TOK> struct Form {
+// PAIR: a unit is two neighbouring feature tiles, which share the stages of rows; their accumulators are the two that are otherwise
+// those of successive units.  Many tokens want it: a CTA's rows come from L2, whose bandwidth was the bound (82 bytes a cycle and SM
+// for 128 x 128, like this 49).
+template <int TOK, bool PAIR> struct Form {
     static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow form cuts the line of tiles, and stores directly)
-    static constexpr int R = TOK <= NARROW_TOKENS ? 8 : 4;
-    static constexpr int GROUPS = TOK <= NARROW_TOKENS ? 4 : 3;
+    static constexpr int TILES = PAIR ? 2 : 1;
+    static constexpr int R = TOK <= NARROW_TOKENS ? 8 : PAIR ? 3 : 4;
+    static constexpr int GROUPS = TOK <= NARROW_TOKENS || PAIR ? 4 : 3;
+    static constexpr int TURNS = GROUPS / TILES;                         // groups that take a feature tile's stages in turn
     static constexpr int EPI_WARP = 4 + 4 * GROUPS, THREADS = 32 * EPI_WARP + EPI;
     static constexpr int ATOMS = TOK <= SIDE_BY_SIDE ? 1 : 2 * ((TOK + 127) / 128);
     static constexpr int ACC_COLS = TOK <= SIDE_BY_SIDE ? 2 * TOK : TOK;
-    static constexpr int RING_COLS = (A_COLS + SFA_COLS + 4 * ATOMS + 7) / 8 * 8;      // [weights | their scales | the rows' scales]
+    static constexpr int W_COLS = A_COLS + SFA_COLS;
+    static constexpr int RING_COLS = (TILES * W_COLS + 4 * ATOMS + 7) / 8 * 8;         // [weights | their scales] a tile, the rows' scales
     static constexpr int STAGE_BYTES = (TOK * 256 + ATOMS * ATOM + 1023) / 1024 * 1024;
-    static constexpr int OUT = WIDE ? 4 * OUT_BYTES : 0;
+    static constexpr int OUT = WIDE ? 2 * OUT_BUFFERS * OUT_BYTES : 0;
     static constexpr int RING = SMEM - 1024 - CONTROL - OUT;             // for the rings of stages
     static constexpr int FIT = (RING - R * STAGE_BYTES) / MX_TILE_BYTES;
     static constexpr int WS = FIT < MAX_W ? FIT : MAX_W;
     static_assert(2 * ACC_COLS + R * RING_COLS <= TMEM, "tensor memory");
-    static_assert(GROUPS <= R && WS >= GROUPS + R, "a wait names a phase by its parity: see the decoding warps");
+    static_assert(TURNS <= R && WS >= GROUPS + TILES * R, "a wait names a phase by its parity: see the decoding warps");
 };
+
+// Atoms of scales that the rows of a tile have: of both parts side by side, or of either part.
+__host__ __device__ constexpr int atoms_of(int tokens) { return tokens <= SIDE_BY_SIDE ? 1 : 2 * ((tokens + 127) / 128); }
 
 struct MxArgs {
     const uint8_t* W; long w_group; const int* shifts;    // tiles, bytes of one group's, what each group's results are raised by
     MxRows rows;                                          // what X's parts, which come by map_x, are made from
-    const uint8_t* x_scales; long scale_rows;             // their scales
+    const uint8_t* x_scales; int scale_bytes;             // their scales, bytes of a tile's
     void* out; long ldo, slab_stride;
-    int o_bf16, accumulate, boxed, slabs;
+    int o_bf16, accumulate, boxed, slabs;                 // boxed: tokens of a box, 0: stored directly
     float* partials; int* counters; int max_segments;
-    int M, N, K, kb, bn, atoms, tiles_m, tiles_n, splits;
+    int M, N, K, kb, bn, tiles_m, tiles_n, units_n, splits;      // units_n: feature tiles, or pairs of them
     long items;                                           // narrow, not grouped: tiles_n * kb; wide, not grouped: units
     const int* tile_group; int tile, n_tiles;
     FbGate gate; int plain_act;
     int* status;
 };
 
-// What a CTA works on at a time: a row tile of a group's matrix, tiles kb0 .. kb0 + n_kb along K, over n_tok rows from m0 on.
+// What a CTA works on at a time: row tile nt (and the one behind it) of a group's matrix, tiles kb0 .. kb0 + n_kb along K, over n_tok rows from m0 on.
 struct Unit { int m0, n_tok, nt, group, kb0, n_kb, share, shares, id; };
 
 __device__ __forceinline__ void mma_mx(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
@@ -147,6 +157,24 @@ __device__ __forceinline__ float silu_times(float g, float u) {
     return g * r * u;
 }
 
+// The epilogue's code is walked a few times a tile only, so that its instructions come from far: every 128 bytes of them cost
+// about as much as ten of the instructions.  What is seldom wanted is kept out of its straight way.
+__device__ __noinline__ float gate_slowly(const FbGate& gate, float g, float u) { return fb_gate_times(gate, g, u); }
+__device__ __noinline__ float act_slowly(int act, float z) { return fb_plain_act(act, z); }
+template <int N> __device__ __forceinline__ void gate_all(const FbGate& gate, float (&g)[N], const float (&u)[N]) {
+    if (__builtin_expect(gate.act == FB_ACT_SILU, 1)) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) g[q] = silu_times(g[q], u[q]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q) g[q] = gate_slowly(gate, g[q], u[q]);
+    }
+}
+__device__ __forceinline__ void st_shared(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void st_shared(uint32_t addr, __nv_bfloat16 v) {
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(__bfloat16_as_ushort(v)) : "memory");
+}
+
 // The shares of a row tile, n_tok x 128 float32 each, added in order; a thread has four neighbouring features of a token.  (As the epilogue's own lanes lie, one share after the other, this took 4 us of a call.)
 __device__ __noinline__ void join_shares(const MxArgs& a, const Unit& w, int tid, int rows, const float* __restrict__ base) {
     const size_t step = (size_t)a.bn * (MX_ROWS / 4);
@@ -181,12 +209,15 @@ __device__ __noinline__ void join_shares(const MxArgs& a, const Unit& w, int tid
             float v[4] = {sum[q].x * raise, sum[q].y * raise, sum[q].z * raise, sum[q].w * raise};
             int count = 4, columns = a.N, col = n;
             if (a.gate.act) {                    // features alternate gate, up
-                v[0] = a.gate.act == FB_ACT_SILU ? silu_times(v[0], v[1]) : fb_gate_times(a.gate, v[0], v[1]);
-                v[1] = a.gate.act == FB_ACT_SILU ? silu_times(v[2], v[3]) : fb_gate_times(a.gate, v[2], v[3]);
+                float g[2] = {v[0], v[2]};
+                const float u[2] = {v[1], v[3]};
+                gate_all(a.gate, g, u);
+                v[0] = g[0];
+                v[1] = g[1];
                 count = 2; columns = a.N / 2; col = n / 2;
             } else if (a.plain_act) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = fb_plain_act(a.plain_act, v[i]);
+                for (int i = 0; i < 4; ++i) v[i] = act_slowly(a.plain_act, v[i]);
             }
             const size_t at = (size_t)m * a.ldo + col;
 #pragma unroll
@@ -203,13 +234,13 @@ __device__ __noinline__ void join_shares(const MxArgs& a, const Unit& w, int tid
     }
 }
 
-template <int TOK, bool GROUPED>
-__global__ void __launch_bounds__(Form<TOK>::THREADS, 1)
+template <int TOK, bool GROUPED, bool PAIR>
+__global__ void __launch_bounds__(Form<TOK, PAIR>::THREADS, 1)
 gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_o,
                   const __grid_constant__ MxArgs a) {
-    using F = Form<TOK>;
+    using F = Form<TOK, PAIR>;
     constexpr bool WIDE = F::WIDE;
-    constexpr int WS = F::WS, R = F::R, G = F::GROUPS, EPI_WARP = F::EPI_WARP;
+    constexpr int WS = F::WS, R = F::R, G = F::GROUPS, EPI_WARP = F::EPI_WARP, TILES = F::TILES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* w_base = smem + R * F::STAGE_BYTES;                         // [stages of rows | weight stages | output boxes | control]
@@ -221,7 +252,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     int* flag = (int*)(tmem_slot + 1);           // what the epilogue decided together
     int* bail = flag + 1;                        // a bounded wait ran out somewhere in this CTA
     int* unit_count = bail + 1;
-    uint32_t* list = (uint32_t*)((uint8_t*)bars + 512);
+    int* group_failed = unit_count + 1;          // [group][round]
+    uint32_t* list = (uint32_t*)((uint8_t*)bars + FLAGS);
+    static_assert(8 * (2 * MAX_W + 3 * MAX_R + 4) + 4 * (4 + 2 * G) <= FLAGS, "barriers and flags");
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_long(smem_u32(bar), parity, a.status); };
     auto bailed = [&]() { return *(volatile int*)bail != 0; };
@@ -231,11 +264,12 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         for (int s = 0; s < MAX_W; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4); }
         for (int s = 0; s < R; ++s) {
             mbar_init(smem_u32(&x_full[s]), 1);
-            mbar_init(smem_u32(&full[s]), 4);
+            mbar_init(smem_u32(&full[s]), 4 * TILES);
             mbar_init(smem_u32(&done[s]), 1);
         }
         for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&acc_full[s]), 1); mbar_init(smem_u32(&acc_empty[s]), EPI); }
         *bail = 0;
+        for (int g = 0; g < 2 * G; ++g) group_failed[g] = 0;
         mbar_fence_init();
     }
     if (warp == 3) tmem_alloc(tmem_slot, TMEM);
@@ -257,7 +291,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             if (lane == 0) *unit_count = found;
         }
         __syncthreads();
-        last = (long)*unit_count * a.tiles_n;
+        last = (long)*unit_count * a.units_n;
     } else if constexpr (LINE) {
         first = blockIdx.x * a.items / gridDim.x;
         last = (blockIdx.x + 1) * a.items / gridDim.x;
@@ -266,21 +300,22 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     auto unit_at = [&](long item) {              // (asked for ascending items only)
         Unit w;
         if constexpr (GROUPED) {                 // feature tiles vary fastest: the CTAs that run together share few units' rows
-            const int i = (int)(item / a.tiles_n);
+            const int i = (int)(item / a.units_n);
             const uint32_t entry = group_unit<LIST>(a.tile_group, a.n_tiles, most, list, i, walk);
             const int t = (int)(entry & 0xffffffu);
             w.m0 = t * a.tile;
             w.n_tok = (int)(entry >> 24) * a.tile;
             w.group = a.tile_group[t];
-            w.nt = (int)(item - (long)i * a.tiles_n);
+            w.nt = TILES * (int)(item - (long)i * a.units_n);
             w.kb0 = 0; w.n_kb = a.kb; w.share = 0; w.shares = 1; w.id = 0;
         } else if constexpr (WIDE) {             // token tiles vary fastest: the CTAs that run together share weight tiles
-            const long tiles = (long)a.tiles_m * a.tiles_n;
-            w.share = (int)(item / tiles);
+            const long units = (long)a.tiles_m * a.units_n;
+            w.share = (int)(item / units);
             w.shares = a.splits;
-            w.id = (int)(item - w.share * tiles);
-            w.m0 = w.id % a.tiles_m * a.bn;
-            w.nt = w.id / a.tiles_m;
+            const int u = (int)(item - w.share * units), mt = u % a.tiles_m;
+            w.m0 = mt * a.bn;
+            w.nt = TILES * (u / a.tiles_m);
+            w.id = mt * a.tiles_n + w.nt;
             w.n_tok = a.bn;
             w.group = 0;
             w.kb0 = (int)((long)w.share * a.kb / a.splits);
@@ -306,12 +341,18 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             for (long u = first; u < last && !bailed();) {
                 const Unit w = unit_at(u);
                 const uint8_t* src = a.W + (size_t)w.group * a.w_group + ((size_t)w.nt * a.kb + w.kb0) * MX_TILE_BYTES;
-                for (int i = 0; i < w.n_kb; ++i, src += MX_TILE_BYTES) {
-                    if (!wait(&w_empty[s], phase)) { *bail = 1; break; }
+                // (a pair's second tile that is none of the matrix is its first one again: nobody stores what comes of it)
+                const size_t next = w.nt + 1 < a.tiles_n ? (size_t)a.kb * MX_TILE_BYTES : 0;
+                bool ok = true;
+                for (int i = 0; i < TILES * w.n_kb && ok; ++i) {
+                    ok = wait(&w_empty[s], phase);
+                    if (!ok) break;
                     mbar_expect_tx(smem_u32(&w_full[s]), MX_TILE_BYTES);
-                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES), src, MX_TILE_BYTES, smem_u32(&w_full[s]));
+                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES), src + (size_t)(i / TILES) * MX_TILE_BYTES + (i % TILES) * next,
+                                  MX_TILE_BYTES, smem_u32(&w_full[s]));
                     if (++s == WS) { s = 0; phase ^= 1u; }
                 }
+                if (!ok) *bail = 1;
                 u = after(u, w);
             }
         }
@@ -328,15 +369,15 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 for (int i = 0; i < w.n_kb; ++i) {
                     if (!wait(&done[s], phase)) { *bail = 1; break; }
                     const uint32_t bar = smem_u32(&x_full[s]), dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES);
-                    const uint32_t scale_bytes = GROUPED ? (uint32_t)w.n_tok * 4 : (uint32_t)a.atoms * ATOM;
+                    const uint32_t scale_bytes = (uint32_t)(atoms_of(w.n_tok) * ATOM);
                     mbar_expect_tx(bar, (uint32_t)w.n_tok * 2 * 128 + scale_bytes);
                     for (int b = 0; b < boxes; ++b) {
 #pragma unroll
                         for (int p = 0; p < 2; ++p)          // (rows beyond M are the other part's, or zeros: nobody stores them)
                             tma_load_2d(dst + (uint32_t)(p * w.n_tok + b * box) * 128, &map_x, bar, (w.kb0 + i) * 64, p * a.M + w.m0 + b * box);
                     }
-                    const size_t at = GROUPED ? ((size_t)(w.kb0 + i) * a.scale_rows + w.m0) * 4
-                                              : ((size_t)(w.kb0 + i) * a.tiles_m + w.m0 / a.bn) * (a.atoms * ATOM);
+                    const size_t tiles = GROUPED ? a.n_tiles : a.tiles_m, tile = w.m0 / (GROUPED ? a.tile : a.bn);
+                    const size_t at = ((size_t)(w.kb0 + i) * tiles + tile) * a.scale_bytes;
                     bulk_copy_g2s(dst + TOK * 256, a.x_scales + at, scale_bytes, bar);
                     if (++s == R) { s = 0; phase ^= 1u; }
                 }
@@ -358,35 +399,45 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             for (long u = first; u < last && ok && !bailed(); ++j) {
                 const Unit w = unit_at(u);
                 const bool both = w.n_tok <= SIDE_BY_SIDE;               // both parts in one operand
-                const int b = j & 1;
+                const int b = PAIR ? 0 : j & 1;
                 const uint32_t idesc = mx_idesc(both ? 2 * w.n_tok : w.n_tok), second = (uint32_t)w.n_tok * 8;      // (128 bytes, in sixteens)
                 const uint32_t sfb_second = (uint32_t)(w.n_tok + 127) / 128 * 4;
-                ok = wait(&acc_empty[b], ((uint32_t)(j >> 1) & 1u) ^ 1u);        // (the epilogue has drained it, two units ago)
+                // (the epilogue has drained the accumulator, two units ago, or both of the pair before)
+                ok = wait(&acc_empty[b], ((uint32_t)(PAIR ? j : j >> 1) & 1u) ^ 1u) && (!PAIR || wait(&acc_empty[1], ((uint32_t)j & 1u) ^ 1u));
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = tmem + (uint32_t)(b * F::ACC_COLS);
                 auto stage = [&](int at, bool fresh) {                   // the stage in place `at` of the ring
                     if (!wait_long(full_base + 8 * at, phase, a.status)) return false;
                     tmem_fence_after();
-                    const uint32_t A = ring + (uint32_t)(at * F::RING_COLS), sfb = A + A_COLS + SFA_COLS;
+                    const uint32_t A0 = ring + (uint32_t)(at * F::RING_COLS), sfb = A0 + TILES * F::W_COLS;
                     const uint64_t x = desc + (uint64_t)(at * (F::STAGE_BYTES / 16));
-                    if constexpr (!GROUPED) {
+                    {
 #pragma unroll
                         for (int t = 0; t < F::ATOMS; ++t)
-                            if (t == 0 || t < a.atoms) copy_scales(sfb + 4 * t, desc_scales + (uint64_t)((at * F::STAGE_BYTES + t * ATOM) / 16));
+                            if (t == 0 || !both) copy_scales(sfb + 4 * t, desc_scales + (uint64_t)((at * F::STAGE_BYTES + t * ATOM) / 16));
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_mx(d, A + 8 * k, x + 2 * k, idesc + mx_block(k), A + A_COLS, sfb, fresh && k == 0 ? 0u : 1u);
-                    if (TOK > SIDE_BY_SIDE && !both) {
+                    for (int h = 0; h < TILES; ++h) {
+                        const uint32_t A = A0 + h * F::W_COLS, to = d + h * F::ACC_COLS;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) mma_mx(d, A + 8 * k, x + second + 2 * k, idesc + mx_block(k), A + A_COLS, sfb + sfb_second, 1u);
+                        for (int k = 0; k < 4; ++k)
+                            mma_mx(to, A + 8 * k, x + 2 * k, idesc + mx_block(k), A + A_COLS, sfb, fresh && k == 0 ? 0u : 1u);
+                        if (TOK > SIDE_BY_SIDE && !both) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                mma_mx(to, A + 8 * k, x + second + 2 * k, idesc + mx_block(k), A + A_COLS, sfb + sfb_second, 1u);
+                        }
                     }
                     umma_commit(done_base + 8 * at);
                     return true;
                 };
                 for (int i = 0; i < w.n_kb && ok;) {
-                    static_assert(R == 4 || R == 8, "blocks of four places");
-                    if (s == 0 && i + 4 <= w.n_kb) {
+                    static_assert(R == 3 || R == 4 || R == 8, "blocks of three or four places");
+                    if (R == 3 && s == 0 && i + 3 <= w.n_kb) {
+                        ok = stage(0, i == 0) && stage(1, false) && stage(2, false);
+                        s = 3; i += 3;
+                    } else if (R != 3 && s == 0 && i + 4 <= w.n_kb) {
                         ok = stage(0, i == 0) && stage(1, false) && stage(2, false) && stage(3, false);
                         s = 4; i += 4;
                     } else if (R == 8 && s == 4 && i + 4 <= w.n_kb) {
@@ -399,38 +450,49 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     if (s == R) { s = 0; phase ^= 1u; }
                 }
                 if (ok) umma_commit(smem_u32(&acc_full[b]));
+                if (PAIR && ok) umma_commit(smem_u32(&acc_full[1]));
                 u = after(u, w);
             }
             if (!ok) *bail = 1;
         }
         __syncwarp();
     } else if (warp >= 4 && warp < EPI_WARP) {
-        // ---------------- decode: a thread a feature; the group's stages are it = group, group + G, ... ----------------
-        // (A wait names a phase by its parity alone, and a group does not come to every slot in every round of a ring.  It has seen the
-        // MMAs of stage it - G - R done, so with G <= R no slot of that ring is two rounds behind, and with WS >= G + R none
-        // of the weights'; x_full is looked at behind done, by which the round before it has arrived.)
+        // ---------------- decode: a thread a feature; weight tiles it = group, group + G, ... (of a pair, always the same one) ----------------
+        // (A wait names a phase by its parity alone, and a group does not come to every slot in every round of a ring.  It comes every
+        // TURNS stages and has seen the MMAs of the stage TURNS + R ago done, so with TURNS <= R no slot of that ring is two rounds
+        // behind, and with WS >= GROUPS + TILES R none of the weights'; x_full is looked at behind done, by which the round before
+        // it has arrived.)
         const int quarter = warp & 3, row = quarter * 32 + lane, group = (warp - 4) >> 2;
         const uint32_t lanes = ring + ((uint32_t)(quarter * 32) << 16);
-        int ws = group, r = group;
-        uint32_t w_phase = 0, r_phase = 0, it = 0;       // it: stages ahead of the unit, modulo G
+        constexpr int TURNS = F::TURNS;
+        const int turn = group / TILES, tile = group % TILES;
+        int ws = group, r = turn;
+        uint32_t w_phase = 0, r_phase = 0, it = 0;       // it: stages ahead of the unit, modulo TURNS
+        int round = 0;
         bool ok = true;
-        for (long u = first; u < last && ok && !bailed();) {
+        for (long u = first; u < last && ok;) {                 // (not `bailed`, which the four warps might see at different times)
             const Unit w = unit_at(u);
-            int i = group - (int)it;                                     // the group's first stage of the unit
-            if (i < 0) i += G;
-            for (; i < w.n_kb; i += G) {
-                ok = wait(&w_full[ws], w_phase);
+            int i = turn - (int)it;                                      // the group's first stage of the unit
+            if (i < 0) i += TURNS;
+            for (; i < w.n_kb; i += TURNS) {
+                // one of the four warps asks: twenty that ask at every barrier again and again take half of the issue slots
+                if (quarter == 0) {
+                    ok = wait(&w_full[ws], w_phase);
+                    if (ok) ok = wait(&done[r], r_phase ^ 1u);           // the MMAs that read this buffer are done
+                    if (ok) ok = wait(&x_full[r], r_phase);
+                    if (!ok) group_failed[2 * group + round] = 1;
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(4 + group) : "memory");
+                ok = *(volatile int*)&group_failed[2 * group + round] == 0;      // (two flags in turn: the next round's is not seen yet)
+                round ^= 1;
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 const uint8_t* src = w_base + (size_t)ws * MX_TILE_BYTES;
                 const uint4 scales = *reinterpret_cast<const uint4*>(src + MX_CODE_BYTES + lane * 16);
                 uint4 c[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) c[q] = *reinterpret_cast<const uint4*>(src + (q * MX_ROWS + row) * 16);
-                ok = wait(&done[r], r_phase ^ 1u);                   // the MMAs that read this buffer are done
-                if (ok) ok = wait(&x_full[r], r_phase);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tmem_fence_after();
-                const uint32_t dst = lanes + (uint32_t)(r * F::RING_COLS);
+                const uint32_t dst = lanes + (uint32_t)(r * F::RING_COLS + tile * F::W_COLS);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t v[16];
@@ -443,31 +505,6 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     tmem_st16(dst + 16 * h, v);
                 }
                 tmem_st4(dst + A_COLS, scales);
-                if (GROUPED) {                                       // the rows' scales: lane l of word j has row 32 j + l
-                    const uint32_t* sx = reinterpret_cast<const uint32_t*>(smem + r * F::STAGE_BYTES + TOK * 256);
-                    const uint32_t sfb = dst + A_COLS + SFA_COLS;
-                    auto word = [&](int q) { return q < w.n_tok ? sx[q] : 0u; };
-                    if (w.n_tok <= SIDE_BY_SIDE) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int q = j * 32 + lane;
-                            v[j] = q < w.n_tok ? sx[q] : mx_second_scales(word(q - w.n_tok));
-                        }
-                        tmem_st4(sfb, make_uint4(v[0], v[1], v[2], v[3]));
-                    } else {
-                        const int second = (w.n_tok + 127) / 128 * 4;
-                        for (int j = 0; j < second; j += 4) {
-                            uint32_t v[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) v[q] = word((j + q) * 32 + lane);
-                            tmem_st4(sfb + j, make_uint4(v[0], v[1], v[2], v[3]));
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) v[q] = mx_second_scales(v[q]);
-                            tmem_st4(sfb + second + j, make_uint4(v[0], v[1], v[2], v[3]));
-                        }
-                    }
-                }
                 // (behind the stores, which need every number of the row: see gemm_f32_tc.cu)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&w_empty[ws]));
@@ -476,9 +513,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&full[r]));
                 if ((ws += G) >= WS) { ws -= WS; w_phase ^= 1u; }
-                if ((r += G) >= R) { r -= R; r_phase ^= 1u; }
+                if ((r += TURNS) >= R) { r -= R; r_phase ^= 1u; }
             }
-            it = (it + (uint32_t)w.n_kb) % G;
+            it = (it + (uint32_t)w.n_kb) % TURNS;
             u = after(u, w);
         }
         if (!ok) *bail = 1;
@@ -487,19 +524,26 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         fb_pdl_wait();
         const int quarter = warp & 3, half = (warp - EPI_WARP) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 32 * EPI_WARP;
         const bool leader = quarter == 0 && lane == 0;
-        constexpr int STEP = OUT_TOKENS * 2;
-        uint32_t boxes = 0;                      // boxes this group of warps has staged: the buffers take turns
+        constexpr int STEP = CHUNK * 2;
+        const uint32_t box_first = smem_u32(out_stage) + half * (OUT_BUFFERS * OUT_BYTES);       // the group's boxes
+        const uint32_t box_last = box_first + (OUT_BUFFERS - 1) * OUT_BYTES;
+        uint32_t box_at = box_first;
         int j = 0;
         for (long u = first; u < last; ++j) {
-            const Unit w = unit_at(u);
+            Unit w = unit_at(u);
+            const long following = after(u, w);
+            bool stop = false;
+#pragma unroll 1
+            for (int h = 0; h < TILES; ++h, ++w.nt, ++w.id) {
             const bool both = w.n_tok <= SIDE_BY_SIDE, join = !GROUPED && w.shares > 1 && a.slabs == 0;
-            const int b = j & 1, n0 = w.nt * MX_ROWS, n = n0 + row;
+            const int b = PAIR ? h : j & 1, n0 = w.nt * MX_ROWS, n = n0 + row;
             const int rows = min(w.n_tok, a.M - w.m0);                   // (grouped: whole tiles)
-            if (bailed() || !wait(&acc_full[b], (uint32_t)(j >> 1) & 1u)) *bail = 1;
+            if (warp == EPI_WARP && (bailed() || !wait(&acc_full[b], (uint32_t)(PAIR ? j : j >> 1) & 1u))) *bail = 1;
             asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
             if (tid == 0) *flag = bailed() ? 2 : 0;                      // one thread decides for all: they meet at barriers below
             asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
-            if (*flag == 2) break;
+            stop = *flag == 2;
+            if (stop) break;
             tmem_fence_after();
             const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * F::ACC_COLS);
             auto sums = [&](int c, float (&v)[16]) {
@@ -511,9 +555,10 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     for (int q = 0; q < 16; ++q) v[q] += second[q];
                 }
             };
-            if (join) {
+            if (PAIR && w.nt >= a.tiles_n) {             // (a pair's second tile that is none of the matrix)
+            } else if (join) {
                 float* mine = a.partials + ((size_t)w.id * a.max_segments + w.share) * (size_t)(a.bn * MX_ROWS) + row;
-                for (int c = half * OUT_TOKENS; c < rows; c += STEP) {
+                for (int c = half * CHUNK; c < rows; c += STEP) {
                     float v[16];
                     sums(c, v);
 #pragma unroll
@@ -537,54 +582,74 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
                 const int slab = a.slabs ? w.share : 0;
 #pragma unroll 1
-                for (int c = half * OUT_TOKENS; c < rows; c += STEP) {
+                for (int c = half * CHUNK; c < rows; c += STEP) {
                     float v[16];
                     sums(c, v);
-                    if (shift > 0) {
+                    if (__builtin_expect(shift > 0, 0)) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) v[q] *= raise;
                     }
-                    if (a.plain_act) {
+                    if (__builtin_expect(a.plain_act != 0, 0)) {
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) v[q] = fb_plain_act(a.plain_act, v[q]);
+                        for (int q = 0; q < 16; ++q) v[q] = act_slowly(a.plain_act, v[q]);
+                    }
+                    if (WIDE && a.boxed) {
+                        // The values go to shared memory as [token][feature], and one thread sends the box on its way (what lies beyond
+                        // the output's edge is not written).  Of three buffers the one that is written was read by the time of the
+                        // barrier before: its store is the third last, and the thread that sends waits for all but the last.
+                        const int x = a.gate.act ? n0 / 2 : n0;
+                        auto send = [&](int token) {
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            if (leader) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                            asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
+                            if (leader) store_box(&map_o, box_at, x, w.m0 + token, slab, a.accumulate != 0);
+                            box_at = box_at == box_last ? box_first : box_at + OUT_BYTES;
+                        };
+                        if (a.gate.act) {
+                            // features alternate gate, up: the even lane takes the first eight tokens of the pair, the odd one the others
+                            float r[8], up[8];
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) {
+                                const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[q] : v[8 + q], 1);
+                                r[q] = lane & 1 ? other : v[q];
+                                up[q] = lane & 1 ? v[8 + q] : other;
+                            }
+                            gate_all(a.gate, r, up);
+                            const int at = (lane & 1) * 8 * (MX_ROWS / 2) + (row >> 1);
+                            if (a.o_bf16) {
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) st_shared(box_at + 2 * (at + q * (MX_ROWS / 2)), __float2bfloat16_rn(r[q]));
+                            } else {
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) st_shared(box_at + 4 * (at + q * (MX_ROWS / 2)), r[q]);
+                            }
+                            send(c);
+                        } else if (a.o_bf16) {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) st_shared(box_at + 2 * (q * MX_ROWS + row), __float2bfloat16_rn(v[q]));
+                            send(c);
+                        } else {
+#pragma unroll
+                            for (int p = 0; p < 2; ++p) {
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) st_shared(box_at + 4 * (q * MX_ROWS + row), v[8 * p + q]);
+                                send(c + 8 * p);
+                            }
+                        }
+                        continue;
                     }
                     // gated: features alternate gate, up; the even lane has act(gate) * up of column n / 2
                     bool writes = n < a.N;
-                    int col = n, width = MX_ROWS, at = row;
+                    int col = n;
                     if (a.gate.act) {
                         float up[16];
 #pragma unroll
                         for (int q = 0; q < 16; ++q) up[q] = __shfl_xor_sync(0xffffffffu, v[q], 1);
-                        if (a.gate.act == FB_ACT_SILU) {
-#pragma unroll
-                            for (int q = 0; q < 16; ++q) v[q] = silu_times(v[q], up[q]);
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 16; ++q) v[q] = fb_gate_times(a.gate, v[q], up[q]);
-                        }
+                        gate_all(a.gate, v, up);
                         writes = !(lane & 1) && n + 1 < a.N;
-                        col = n >> 1; width = MX_ROWS / 2; at = row >> 1;
+                        col = n >> 1;
                     }
-                    if (WIDE && a.boxed) {
-                        // the values go to shared memory as [token][feature], and one thread sends the box on its way (what lies
-                        // beyond the output's edge is not written)
-                        uint8_t* box = out_stage + (half * 2 + (boxes & 1u)) * OUT_BYTES;
-                        ++boxes;
-                        if (leader) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // it has left this buffer
-                        asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
-                        if (!a.gate.act || !(lane & 1)) {
-                            if (a.o_bf16) {
-#pragma unroll
-                                for (int q = 0; q < 16; ++q) reinterpret_cast<__nv_bfloat16*>(box)[q * width + at] = __float2bfloat16_rn(v[q]);
-                            } else {
-#pragma unroll
-                                for (int q = 0; q < 16; ++q) reinterpret_cast<float*>(box)[q * width + at] = v[q];
-                            }
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        asm volatile("bar.sync %0, 128;" ::"r"(2 + half) : "memory");
-                        if (leader) store_box(&map_o, smem_u32(box), a.gate.act ? n0 / 2 : n0, w.m0 + c, slab, a.accumulate != 0);
-                    } else if (writes) {
+                    if (writes) {
                         const size_t begin = (size_t)slab * a.slab_stride + (size_t)(w.m0 + c) * a.ldo + col;
                         if (a.o_bf16) {
                             __nv_bfloat16* p = reinterpret_cast<__nv_bfloat16*>(a.out) + begin;
@@ -607,7 +672,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             }
             tmem_fence_before();
             mbar_arrive(smem_u32(&acc_empty[b]));
-            u = after(u, w);
+            }
+            if (stop) break;
+            u = following;
         }
         if (WIDE && leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");        // the boxes it sent are in memory
     }
@@ -656,27 +723,34 @@ Cut cut_of(int tiles_n, int kb, int limit, bool join) {
 int narrow_tokens(int M) { return (M + 7) / 8 * 8; }
 
 // ---- wide: token tiles and shares of K ----
-struct Plan { int bn, splits; };
+struct Plan { int bn, splits; bool pair; };
 constexpr int MORE_TILES = 2;
+constexpr double L2_BYTES = 62.0;                 // what an SM gets from L2 a cycle when all of them ask
 // The cheapest of the choices in cycles of an SM.  A stage costs its MMAs (2 cycles a column, at least 46 an instruction) or its
-// decoding, whichever is more; all CTAs together no less than the weights from HBM.  A share of K costs a copy of the output, written
+// decoding or its way from L2, whichever is most; all CTAs together no less than the weights from HBM.  A share of K costs a copy of the output, written
 // and read.
 Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
     const long sms = fb_sm_count(), tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
-    Plan best = {WIDE_TOKENS, 1};
+    Plan best = {WIDE_TOKENS, 1, false};
     double best_cost = 1e300;
     const long least = (M + WIDE_TOKENS - 1) / WIDE_TOKENS;
     for (long tiles_m = least; tiles_m <= least + MORE_TILES; ++tiles_m) {
         const int bn = (int)(((M + tiles_m - 1) / tiles_m + 15) / 16 * 16);
-        const double stage = fmax(4.0 * bn + 60.0, 260.0);
-        const long tiles = tiles_n * ((M + bn - 1) / bn);
-        for (int splits = 1; splits <= max_splits && splits <= kb; ++splits) {
-            if (!slabs && splits > 1 && (tiles > n_counters || tiles * splits * bn * MX_ROWS > partial_floats)) break;
-            const long rounds = (tiles * splits + sms - 1) / sms;
-            double cost = fmax((double)rounds * ((kb + splits - 1) / splits * stage + 500.0),
-                               (double)tiles_n * kb * MX_TILE_BYTES / (23.0 * sms));
-            cost += (splits - 1) * (double)M * N * 8.0 / (24.0 * sms) + (splits > 1 && !slabs ? 1500.0 : 0.0);
-            if (cost < best_cost * (1.0 - 1e-9)) { best_cost = cost; best = Plan{bn, splits}; }
+        const long tiles = (M + bn - 1) / bn;
+        for (int pair = 0; pair <= 1; ++pair) {
+            if (pair && bn <= SIDE_BY_SIDE) continue;
+            const long units_n = pair ? (tiles_n + 1) / 2 : tiles_n;
+            const double l2 = (bn * 256.0 + (pair ? 2 : 1) * (double)MX_TILE_BYTES) / L2_BYTES;
+            const double stage = fmax(fmax((pair ? 8.0 : 4.0) * bn, l2) + 30.0, pair ? 520.0 : 300.0);
+            for (int splits = 1; splits <= max_splits && splits <= kb; ++splits) {
+                if (!slabs && splits > 1 && (tiles * tiles_n > n_counters || tiles * tiles_n * splits * bn * MX_ROWS > partial_floats)) break;
+                const long rounds = (tiles * units_n * splits + sms - 1) / sms;
+                // (a pair's epilogue does not overlap the products of the next one)
+                double cost = fmax((double)rounds * ((kb + splits - 1) / splits * stage + (pair ? 35.0 * bn : 500.0)),
+                                   (double)tiles_n * kb * MX_TILE_BYTES / (23.0 * sms));
+                cost += (splits - 1) * (double)M * N * 8.0 / (24.0 * sms) + (splits > 1 && !slabs ? 3000.0 : 0.0);
+                if (cost < best_cost * (1.0 - 1e-9)) { best_cost = cost; best = Plan{bn, splits, pair != 0}; }
+            }
         }
     }
     return best;
@@ -685,43 +759,42 @@ Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int 
 constexpr long SHARE_FLOATS = 16L << 20;          // most that the shares of one product may take
 constexpr int MOST_SPLITS = 16;
 
-// Atoms of scales that a stage's rows have: of both parts side by side, or of either part.
-int atoms_of(int bn) { return bn <= SIDE_BY_SIDE ? 1 : 2 * ((bn + 127) / 128); }
-
-template <int TOK, bool GROUPED> int launch(const MxArgs& a, const CUtensorMap& mx, const CUtensorMap& mo, long grid, cudaStream_t stream) {
-    auto kernel = gemm_mxfp4_kernel<TOK, GROUPED>;
+template <int TOK, bool GROUPED, bool PAIR> int launch(const MxArgs& a, const CUtensorMap& mx, const CUtensorMap& mo, long grid, cudaStream_t stream) {
+    auto kernel = gemm_mxfp4_kernel<TOK, GROUPED, PAIR>;
     static bool configured[FB_MAX_DEVICES] = {};
     if (fb_needs_setup(configured)) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return fb_fail(-2, "gemm_mxfp4: cannot reserve shared memory: %s", cudaGetErrorString(e));
         fb_setup_done(configured);
     }
-    fb_launch_class(a.M > 128 && Form<TOK>::WIDE ? FB_LAUNCH_GEMM_WIDE : FB_LAUNCH_OTHER, kernel, dim3((unsigned)grid), dim3(Form<TOK>::THREADS), SMEM, stream, mx, mo, a);
+    fb_launch_class(a.M > 128 && Form<TOK, PAIR>::WIDE ? FB_LAUNCH_GEMM_WIDE : FB_LAUNCH_OTHER, kernel, dim3((unsigned)grid), dim3(Form<TOK, PAIR>::THREADS), SMEM, stream, mx, mo, a);
     return fb_check_launch("gemm_mxfp4");
 }
 
-long long scale_bytes_of(int M, int kb, bool grouped) {
-    // grouped: a word a row; else atoms a token tile, of which there are at most MORE_TILES more than the rows need
-    return grouped ? 4LL * kb * ((M + 3) / 4 * 4) : (long long)kb * ((M + WIDE_TOKENS - 1) / WIDE_TOKENS + MORE_TILES) * 4 * ATOM;
+// (Token tiles are at most MORE_TILES more than the rows need; the grouped form has a place for every row tile.)
+long long scale_bytes_of(int M, int kb, int tile) {
+    const long long tiles = tile ? M / tile : (M + WIDE_TOKENS - 1) / WIDE_TOKENS + MORE_TILES;
+    return kb * tiles * ATOM * (tile == 16 || (!tile && M <= SIDE_BY_SIDE) ? 1 : 2);
 }
 
 // The rows' parts and scales in `scratch`, their map, the output's map.
 int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, int box_rows, cudaStream_t stream) {
     const bool grouped = a.tile_group != nullptr;
     const long Kp = (long)a.kb * MX_COLS, parts = 2L * a.M * Kp;
-    a.scale_rows = (a.M + 3) / 4 * 4;
     a.x_scales = (const uint8_t*)scratch + parts;
-    a.atoms = atoms_of(a.bn);
-    const MxScaleLayout layout = {grouped ? 0 : a.bn, grouped ? 0 : a.atoms * ATOM, a.scale_rows};
-    int rc = fb_mxfp4_split_rows(a.rows, a.M, a.K, scratch, (uint8_t*)scratch + parts, layout, a.tile_group, a.tile, stream);
+    a.scale_bytes = atoms_of(a.bn) * ATOM;
+    const int most = grouped ? a.bn / a.tile : 0;
+    int rc = fb_mxfp4_split_rows(a.rows, a.M, a.K, scratch, (uint8_t*)scratch + parts,
+                                 MxScaleLayout{a.bn, a.scale_bytes, a.tile_group, a.tile, most, a.n_tiles}, stream);
     if (rc) return rc;
     rc = fb_tensor_map_bf16(&mx, scratch, 2L * a.M, Kp / 2, Kp / 2, 64, box_rows);       // (bytes, two at a time)
     if (rc) return rc;
     a.boxed = 0;
     if (box_rows <= NARROW_TOKENS && (!grouped || a.tile == 16)) return 0;               // (the narrow form stores directly)
+    const int tokens = a.o_bf16 || a.gate.act ? 16 : 8;
     rc = fb_tensor_map_out(&mo, a.out, a.o_bf16 ? 2 : 4, a.M, a.gate.act ? a.N / 2 : a.N, a.ldo, a.slabs ? a.slabs : 1, a.slab_stride,
-                           a.gate.act ? MX_ROWS / 2 : MX_ROWS, OUT_TOKENS);
-    a.boxed = rc == 0;
+                           a.gate.act ? MX_ROWS / 2 : MX_ROWS, tokens);
+    a.boxed = rc == 0 ? tokens : 0;
     return rc < 0 ? rc : 0;
 }
 
@@ -745,7 +818,7 @@ int check_operands(const void* X, long long lda, const void* W, const int* shift
 static long long rows_bytes(int M, int K, int tile) {
     if (M <= 0 || K <= 0) return 0;
     const long long kb = (K + MX_COLS - 1) / MX_COLS;
-    return (2LL * M * kb * MX_COLS + scale_bytes_of(M, (int)kb, tile > 0) + 255) / 256 * 256;
+    return (2LL * M * kb * MX_COLS + scale_bytes_of(M, (int)kb, tile) + 255) / 256 * 256;
 }
 
 // Floats that shares of K take which meet in scratch: 0 where K is not split.
@@ -806,22 +879,24 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
             if (splits_used) *splits_used = cut.segments;
         }
         if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
-        return launch<32, false>(a, mx, mo, cut.grid, stream);
+        return launch<32, false, false>(a, mx, mo, cut.grid, stream);
     }
     const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, SHARE_FLOATS,
                                 n_counters, slabs);
     a.bn = plan.bn;
     a.tiles_m = (M + plan.bn - 1) / plan.bn;
+    a.units_n = plan.pair ? (a.tiles_n + 1) / 2 : a.tiles_n;
     a.splits = a.max_segments = plan.splits;
     if (slabs) {
         a.slabs = plan.splits;
         if (splits_used) *splits_used = plan.splits;
     }
-    a.items = (long)a.tiles_m * a.tiles_n * a.splits;
+    a.items = (long)a.tiles_m * a.units_n * a.splits;
     if (a.items > 2000000000L) return fb_fail(-1, "gemm_mxfp4: too many tiles (M=%d N=%d)", M, N);
     if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
     const long grid = a.items < fb_sm_count() ? a.items : fb_sm_count();
-    return a.bn <= 64 ? launch<64, false>(a, mx, mo, grid, stream) : launch<128, false>(a, mx, mo, grid, stream);
+    if (plan.pair) return launch<128, false, true>(a, mx, mo, grid, stream);
+    return a.bn <= 64 ? launch<64, false, false>(a, mx, mo, grid, stream) : launch<128, false, false>(a, mx, mo, grid, stream);
 }
 
 // The grouped form: W holds `groups` matrices [N, K] in tiles with a shift each; the M rows of `out` come in tiles of `tile` (a
@@ -849,12 +924,13 @@ FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_in
     a.o_bf16 = o_dtype == FB_BF16; a.M = M; a.N = N; a.K = K; a.tiles_m = 1; a.splits = a.max_segments = 1;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
     a.tile_group = tile_group; a.tile = tile; a.n_tiles = M / tile;
-    const long units = (long)a.n_tiles * a.tiles_n;
+    const bool narrow = tile == 16;
+    a.units_n = narrow ? a.tiles_n : (a.tiles_n + 1) / 2;
+    const long units = (long)a.n_tiles * a.units_n;
     if (units > 2000000000L) return fb_fail(-1, "gemm_mxfp4_grouped: too many tiles (M=%d N=%d)", M, N);
     CUtensorMap mx = {}, mo = {};
-    const bool narrow = tile == 16;
-    a.bn = (narrow ? NARROW_TOKENS : WIDE_TOKENS) / tile * tile;
+    a.bn = narrow ? tile : WIDE_TOKENS / tile * tile;    // (narrow: a group has few rows, seldom two tiles)
     if (const int rc = prepare(a, mx, mo, scratch, tile, stream)) return rc;
     const long grid = units < fb_sm_count() ? units : fb_sm_count();
-    return narrow ? launch<32, true>(a, mx, mo, grid, stream) : launch<128, true>(a, mx, mo, grid, stream);
+    return narrow ? launch<32, true, false>(a, mx, mo, grid, stream) : launch<128, true, true>(a, mx, mo, grid, stream);
 }

@@ -225,37 +225,67 @@ tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scal
     dst[MX_CODE_BYTES + ((row & 31) * 4 + (row >> 5)) * 4 + (b & 3)] = (uint8_t)s;
 }
 
-// A thread eight numbers: parts[p][m][k] (bytes, rows of Kp, a multiple of 128, zeros behind K), their scales as `layout` says.
+// A thread eight numbers of each of four rows, which lie in one tile: parts[p][m][k] (bytes, rows of Kp, a multiple of 128, zeros behind
+// K), their scales as `layout` says.
+constexpr int SPLIT_COLS = 2048, SPLIT_ROWS = 4;
+template <bool GROUPED>
 __global__ void __launch_bounds__(256)
 split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales,
-             const __grid_constant__ MxScaleLayout layout, const int* __restrict__ tile_group, int tile) {
+             const __grid_constant__ MxScaleLayout layout) {
     fb_pdl_launch_dependents();
     fb_pdl_wait();
-    const int pieces = Kp / 8;
-    for (long base = (long)blockIdx.x * 256; base < (long)M * pieces; base += (long)gridDim.x * 256) {
-        const long p = base + threadIdx.x;
-        const bool mine = p < (long)M * pieces;
-        const int m = mine ? (int)(p / pieces) : 0, k = mine ? 8 * (int)(p - (long)m * pieces) : 0;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        // (rows of tiles without a group are not multiplied, whatever they hold)
-        if (mine && (!tile_group || tile_group[m / tile] >= 0)) v = mx_row8(rows, m, k, K);
-        const uint32_t scale = mx_row_scale(mx_top8(v));
-        uint2 first, second;
-        mx_split8({v.x, v.y, v.z, v.w}, scale, first, second);
-        if (!mine) continue;
-        *reinterpret_cast<uint2*>(parts + (size_t)m * Kp + k) = first;
-        *reinterpret_cast<uint2*>(parts + ((size_t)M + m) * Kp + k) = second;
-        if ((k & 31) != 0) continue;
-        const int kb = k >> 7, byte = k >> 5 & 3;
-        if (layout.tokens == 0) {
-            scales[((size_t)kb * layout.rows + m) * 4 + byte] = (uint8_t)scale;
-        } else {
-            const int tiles = (M + layout.tokens - 1) / layout.tokens, t = m / layout.tokens, q = m - t * layout.tokens;
-            uint8_t* at = scales + ((size_t)kb * tiles + t) * layout.tile_bytes + byte;
-            const int second = layout.tokens <= 64 ? layout.tokens + q : (layout.tokens + 127) / 128 * 128 + q;
+    const int k = blockIdx.y * SPLIT_COLS + 8 * threadIdx.x, lane = threadIdx.x & 31, first = blockIdx.x * SPLIT_ROWS;
+    int unit, tokens, at, tiles;                         // the scales' tile, its tokens, the first row's place in it, all tiles
+    if constexpr (GROUPED) {
+        const int t = first / layout.tile, g = layout.tile_group[t];
+        if (g < 0) return;                               // (rows of tiles without a group are not multiplied, whatever they hold)
+        unit = t;
+        int n = 1;
+        if (layout.most > 1) {
+            // where the run of tiles of this group begins, 32 at a time, and so where the unit of up to `most` that holds t does
+            int begin = 0;
+            for (int t0 = t; t0 > 0; t0 -= 32) {
+                const int left = t0 - 1 - lane;
+                const uint32_t other = __ballot_sync(0xffffffffu, left < 0 || layout.tile_group[left] != g);
+                if (other) {
+                    begin = t0 - (__ffs((int)other) - 1);
+                    break;
+                }
+            }
+            unit = begin + (t - begin) / layout.most * layout.most;
+            while (n < layout.most && unit + n < layout.n_tiles && layout.tile_group[unit + n] == g) ++n;
+        }
+        tokens = n * layout.tile;
+        at = first - unit * layout.tile;
+        tiles = layout.n_tiles;
+    } else {
+        unit = first / layout.tokens;
+        tokens = layout.tokens;
+        at = first - unit * layout.tokens;
+        tiles = (M + layout.tokens - 1) / layout.tokens;
+    }
+    const int apart = tokens <= 64 ? tokens : (tokens + 127) / 128 * 128;
+    uint8_t* to = scales + ((size_t)(k >> 7) * tiles + unit) * layout.tile_bytes;
+    uint4 v[SPLIT_ROWS];
+#pragma unroll
+    for (int q = 0; q < SPLIT_ROWS; ++q) v[q] = k < K && first + q < M ? mx_row8(rows, first + q, k, K) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int q = 0; q < SPLIT_ROWS; ++q) {
+        const int m = first + q;
+        const uint32_t scale = mx_row_scale(mx_top8(v[q]));
+        uint2 one, two;
+        mx_split8({v[q].x, v[q].y, v[q].z, v[q].w}, scale, one, two);
+        // the four scales of 128 columns, which sixteen lanes share, as a word
+        const uint32_t s1 = __shfl_down_sync(0xffffffffu, scale, 4), s2 = __shfl_down_sync(0xffffffffu, scale, 8),
+                       s3 = __shfl_down_sync(0xffffffffu, scale, 12);
+        if (k >= Kp || m >= M) continue;
+        *reinterpret_cast<uint2*>(parts + (size_t)m * Kp + k) = one;
+        *reinterpret_cast<uint2*>(parts + ((size_t)M + m) * Kp + k) = two;
+        if ((lane & 15) == 0) {
+            const uint32_t word = scale | s1 << 8 | s2 << 16 | s3 << 24;
             auto place = [](int row) { return (row >> 7) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4; };
-            at[place(q)] = (uint8_t)scale;
-            at[place(second)] = (uint8_t)mx_second_scales(scale);
+            *reinterpret_cast<uint32_t*>(to + place(at + q)) = word;
+            *reinterpret_cast<uint32_t*>(to + place(apart + at + q)) = mx_second_scales(word);
         }
     }
 }
@@ -334,10 +364,10 @@ FB_API int fb_mxfp4_tiles(const void* codes, const void* scales, int groups, int
 
 // The rows of a product with four-bit weights as two e4m3 numbers each (mxfp4.cuh): `parts` takes 2 M Kp bytes (Kp: K rounded up to
 // a multiple of 128), `scales` what `layout` says, both 16-byte aligned.
-int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, MxScaleLayout layout, const int* tile_group, int tile,
-                        cudaStream_t stream) {
+int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, const MxScaleLayout& layout, cudaStream_t stream) {
     const int Kp = (K + MX_COLS - 1) / MX_COLS * MX_COLS;
-    fb_launch(split_kernel, dim3(grid_of((long)M * (Kp / 8), 256)), dim3(256), 0, stream, rows, M, K, Kp, (uint8_t*)parts, (uint8_t*)scales,
-              layout, tile_group, tile);
+    const dim3 grid((unsigned)((M + SPLIT_ROWS - 1) / SPLIT_ROWS), (unsigned)((Kp + SPLIT_COLS - 1) / SPLIT_COLS));
+    if (layout.tile_group) fb_launch(split_kernel<true>, grid, dim3(256), 0, stream, rows, M, K, Kp, (uint8_t*)parts, (uint8_t*)scales, layout);
+    else fb_launch(split_kernel<false>, grid, dim3(256), 0, stream, rows, M, K, Kp, (uint8_t*)parts, (uint8_t*)scales, layout);
     return fb_check_launch("mxfp4_split_rows");
 }

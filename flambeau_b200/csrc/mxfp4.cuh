@@ -113,9 +113,8 @@ __device__ __forceinline__ uint4 mx_row8(const MxRows& r, int m, int k, int K) {
     if (r.share) v = mx_times(v, r.share[r.pair[m]]);
     return v;
 }
-// Where the rows' scales go.  tokens > 0: [K / 128][token tile][tile_bytes], a tile's first parts and then (up to 64 tokens: among
-// them as rows tokens .., else behind them, from a multiple of 128 rows on) its second ones as [128 rows][lane i][j] words of row
-// 32 j + i; tokens == 0: a word of the first part's a row, [K / 128][rows].
-struct MxScaleLayout { int tokens, tile_bytes; long rows; };
-int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, MxScaleLayout layout, const int* tile_group, int tile,
-                        cudaStream_t stream);
+// Where the rows' scales go: [K / 128][token tile][tile_bytes], for a tile of n tokens the first parts as rows 0 .. and the second ones
+// up to 64 tokens as rows n .., else from the next multiple of 128 on, by 128 rows as [lane i][j] words of row 32 j + i.  A tile is
+// `tokens` rows; grouped: up to `most` neighbouring row tiles of `tile` rows of one group, in the place of the first of them.
+struct MxScaleLayout { int tokens, tile_bytes; const int* tile_group; int tile, most, n_tiles; };
+int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, const MxScaleLayout& layout, cudaStream_t stream);
