@@ -22,7 +22,7 @@
 // meet in scratch, where the CTA that arrives last (a counter a row tile, no waiting) adds them in order.  Grouped (routed
 // experts): row tiles of one group each; a unit is a run of neighbouring ones.
 //
-// full[s]: a stage's rows and its decoded weights are there; done[s]: its MMAs are.  Two accumulators, so that the epilogue of one
+// full[s]: a stage's rows (by bytes) and its decoded weights (by arrivals) are there; done[s]: its MMAs are.  Two accumulators, so that the epilogue of one
 // unit overlaps the products of the next.  Every mbarrier wait is bounded as in gemm_tc.cu.
 #include "group_units.cuh"
 #include "mxfp4.cuh"
@@ -46,7 +46,6 @@ constexpr int CONTROL = FLAGS + 4 * LIST;         // and the list
 constexpr int NARROW_TOKENS = 32, WIDE_TOKENS = 128;      // most tokens of a tile of either form
 constexpr int SIDE_BY_SIDE = 64;                  // most tokens whose two parts are one operand
 constexpr int ATOM = 512;                         // scales of 128 rows for a stage, as tcgen05.cp brings them to tensor memory
-constexpr int EPI = 256;                          // threads of the epilogue
 constexpr int TMEM = 512, SMEM = 227 * 1024;
 
 // TOK: most tokens of a tile.  R stages of rows and decoded weights, GROUPS of four decoding warps: a stage is 1,500 cycles on its way
@@ -59,7 +58,8 @@ template <int TOK, bool PAIR> struct Form {
     static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow form cuts the line of tiles, and stores directly)
     static constexpr int TILES = PAIR ? 2 : 1;
     static constexpr int R = TOK <= NARROW_TOKENS ? 8 : PAIR ? 3 : 4;
-    static constexpr int GROUPS = TOK <= NARROW_TOKENS || PAIR ? 4 : 3;
+    static constexpr int GROUPS = TOK <= NARROW_TOKENS ? 4 : PAIR ? 2 : 3;
+    static constexpr int EPI_GROUPS = PAIR ? 4 : 2, EPI = 128 * EPI_GROUPS;   // groups of four warps, threads of the epilogue
     static constexpr int TURNS = GROUPS / TILES;                         // groups that take a feature tile's stages in turn
     static constexpr int EPI_WARP = 4 + 4 * GROUPS, THREADS = 32 * EPI_WARP + EPI;
     static constexpr int ATOMS = TOK <= SIDE_BY_SIDE ? 1 : 2 * ((TOK + 127) / 128);
@@ -67,7 +67,7 @@ template <int TOK, bool PAIR> struct Form {
     static constexpr int W_COLS = A_COLS + SFA_COLS;
     static constexpr int RING_COLS = (TILES * W_COLS + 4 * ATOMS + 7) / 8 * 8;         // [weights | their scales] a tile, the rows' scales
     static constexpr int STAGE_BYTES = (TOK * 256 + ATOMS * ATOM + 1023) / 1024 * 1024;
-    static constexpr int OUT = WIDE ? 2 * OUT_BUFFERS * OUT_BYTES : 0;
+    static constexpr int OUT = WIDE ? EPI_GROUPS * OUT_BUFFERS * OUT_BYTES : 0;
     static constexpr int RING = SMEM - 1024 - CONTROL - OUT;             // for the rings of stages
     static constexpr int FIT = (RING - R * STAGE_BYTES) / MX_TILE_BYTES;
     static constexpr int WS = FIT < MAX_W ? FIT : MAX_W;
@@ -176,7 +176,7 @@ __device__ __forceinline__ void st_shared(uint32_t addr, __nv_bfloat16 v) {
 }
 
 // The shares of a row tile, n_tok x 128 float32 each, added in order; a thread has four neighbouring features of a token.  (As the epilogue's own lanes lie, one share after the other, this took 4 us of a call.)
-__device__ __noinline__ void join_shares(const MxArgs& a, const Unit& w, int tid, int rows, const float* __restrict__ base) {
+template <int EPI> __device__ __noinline__ void join_shares(const MxArgs& a, const Unit& w, int tid, int rows, const float* __restrict__ base) {
     const size_t step = (size_t)a.bn * (MX_ROWS / 4);
     const int shift = a.shifts[w.group];
     const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
@@ -240,13 +240,13 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                   const __grid_constant__ MxArgs a) {
     using F = Form<TOK, PAIR>;
     constexpr bool WIDE = F::WIDE;
-    constexpr int WS = F::WS, R = F::R, G = F::GROUPS, EPI_WARP = F::EPI_WARP, TILES = F::TILES;
+    constexpr int WS = F::WS, R = F::R, G = F::GROUPS, EPI = F::EPI, EPI_WARP = F::EPI_WARP, TILES = F::TILES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* w_base = smem + R * F::STAGE_BYTES;                         // [stages of rows | weight stages | output boxes | control]
     uint8_t* out_stage = smem + F::RING;
     uint64_t* bars = (uint64_t*)(out_stage + F::OUT);
-    uint64_t *w_full = bars, *w_empty = w_full + MAX_W, *x_full = w_empty + MAX_W, *full = x_full + MAX_R, *done = full + MAX_R,
+    uint64_t *w_full = bars, *w_empty = w_full + MAX_W, *full = w_empty + MAX_W, *done = full + MAX_R,
              *acc_full = done + MAX_R, *acc_empty = acc_full + 2;
     uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
     int* flag = (int*)(tmem_slot + 1);           // what the epilogue decided together
@@ -254,7 +254,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     int* unit_count = bail + 1;
     int* group_failed = unit_count + 1;          // [group][round]
     uint32_t* list = (uint32_t*)((uint8_t*)bars + FLAGS);
-    static_assert(8 * (2 * MAX_W + 3 * MAX_R + 4) + 4 * (4 + 2 * G) <= FLAGS, "barriers and flags");
+    static_assert(8 * (2 * MAX_W + 2 * MAX_R + 4) + 4 * (4 + 2 * G) <= FLAGS, "barriers and flags");
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_long(smem_u32(bar), parity, a.status); };
     auto bailed = [&]() { return *(volatile int*)bail != 0; };
@@ -263,8 +263,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     if (threadIdx.x == 0) {
         for (int s = 0; s < MAX_W; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4); }
         for (int s = 0; s < R; ++s) {
-            mbar_init(smem_u32(&x_full[s]), 1);
-            mbar_init(smem_u32(&full[s]), 4 * TILES);
+            mbar_init(smem_u32(&full[s]), 4 * TILES + 1);
             mbar_init(smem_u32(&done[s]), 1);
         }
         for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&acc_full[s]), 1); mbar_init(smem_u32(&acc_empty[s]), EPI); }
@@ -368,7 +367,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 const int boxes = GROUPED ? w.n_tok / a.tile : 1, box = GROUPED ? a.tile : a.bn;
                 for (int i = 0; i < w.n_kb; ++i) {
                     if (!wait(&done[s], phase)) { *bail = 1; break; }
-                    const uint32_t bar = smem_u32(&x_full[s]), dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES);
+                    const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES);
                     const uint32_t scale_bytes = (uint32_t)(atoms_of(w.n_tok) * ATOM);
                     mbar_expect_tx(bar, (uint32_t)w.n_tok * 2 * 128 + scale_bytes);
                     for (int b = 0; b < boxes; ++b) {
@@ -402,37 +401,61 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 const int b = PAIR ? 0 : j & 1;
                 const uint32_t idesc = mx_idesc(both ? 2 * w.n_tok : w.n_tok), second = (uint32_t)w.n_tok * 8;      // (128 bytes, in sixteens)
                 const uint32_t sfb_second = (uint32_t)(w.n_tok + 127) / 128 * 4;
-                // (the epilogue has drained the accumulator, two units ago, or both of the pair before)
-                ok = wait(&acc_empty[b], ((uint32_t)(PAIR ? j : j >> 1) & 1u) ^ 1u) && (!PAIR || wait(&acc_empty[1], ((uint32_t)j & 1u) ^ 1u));
+                // (the epilogue has drained the accumulator, of two units ago or of the pair before)
+                ok = wait(&acc_empty[b], ((uint32_t)(PAIR ? j : j >> 1) & 1u) ^ 1u);
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = tmem + (uint32_t)(b * F::ACC_COLS);
-                auto stage = [&](int at, bool fresh) {                   // the stage in place `at` of the ring
-                    if (!wait_long(full_base + 8 * at, phase, a.status)) return false;
-                    tmem_fence_after();
+                auto products = [&](int at, int h, bool fresh) {         // of the stage in place `at` of the ring with the h-th feature tile
                     const uint32_t A0 = ring + (uint32_t)(at * F::RING_COLS), sfb = A0 + TILES * F::W_COLS;
                     const uint64_t x = desc + (uint64_t)(at * (F::STAGE_BYTES / 16));
-                    {
+                    const uint32_t A = A0 + h * F::W_COLS, to = d + h * F::ACC_COLS;
 #pragma unroll
-                        for (int t = 0; t < F::ATOMS; ++t)
-                            if (t == 0 || !both) copy_scales(sfb + 4 * t, desc_scales + (uint64_t)((at * F::STAGE_BYTES + t * ATOM) / 16));
-                    }
-#pragma unroll
-                    for (int h = 0; h < TILES; ++h) {
-                        const uint32_t A = A0 + h * F::W_COLS, to = d + h * F::ACC_COLS;
+                    for (int k = 0; k < 4; ++k)
+                        mma_mx(to, A + 8 * k, x + 2 * k, idesc + mx_block(k), A + A_COLS, sfb, fresh && k == 0 ? 0u : 1u);
+                    if (TOK > SIDE_BY_SIDE && !both) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            mma_mx(to, A + 8 * k, x + 2 * k, idesc + mx_block(k), A + A_COLS, sfb, fresh && k == 0 ? 0u : 1u);
-                        if (TOK > SIDE_BY_SIDE && !both) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                mma_mx(to, A + 8 * k, x + second + 2 * k, idesc + mx_block(k), A + A_COLS, sfb + sfb_second, 1u);
-                        }
+                            mma_mx(to, A + 8 * k, x + second + 2 * k, idesc + mx_block(k), A + A_COLS, sfb + sfb_second, 1u);
                     }
+                };
+                auto begin = [&](int at) {
+                    if (!wait_long(full_base + 8 * at, phase, a.status)) return false;
+                    tmem_fence_after();
+                    const uint32_t sfb = ring + (uint32_t)(at * F::RING_COLS) + TILES * F::W_COLS;
+#pragma unroll
+                    for (int t = 0; t < F::ATOMS; ++t)
+                        if (t == 0 || !both) copy_scales(sfb + 4 * t, desc_scales + (uint64_t)((at * F::STAGE_BYTES + t * ATOM) / 16));
+                    return true;
+                };
+                auto stage = [&](int at, bool fresh) {
+                    if (!begin(at)) return false;
+#pragma unroll
+                    for (int h = 0; h < TILES; ++h) products(at, h, fresh);
                     umma_commit(done_base + 8 * at);
                     return true;
                 };
-                for (int i = 0; i < w.n_kb && ok;) {
+                int i = 0;
+                if constexpr (PAIR) {
+                    // the first tile's products of the stages that the ring holds run ahead, while the epilogue still has the other accumulator
+                    const int s0 = s, ahead = w.n_kb < R ? w.n_kb : R;
+                    const uint32_t phase0 = phase;
+                    for (; i < ahead && ok; ++i) {
+                        ok = begin(s);
+                        if (ok) products(s, 0, i == 0);
+                        if (++s == R) { s = 0; phase ^= 1u; }
+                    }
+                    if (!ok || !(ok = wait(&acc_empty[1], ((uint32_t)j & 1u) ^ 1u))) break;
+                    tmem_fence_after();
+                    s = s0;
+                    phase = phase0;
+                    for (int t = 0; t < ahead; ++t) {
+                        products(s, 1, t == 0);
+                        umma_commit(done_base + 8 * s);
+                        if (++s == R) { s = 0; phase ^= 1u; }
+                    }
+                }
+                while (i < w.n_kb && ok) {
                     static_assert(R == 3 || R == 4 || R == 8, "blocks of three or four places");
                     if (R == 3 && s == 0 && i + 3 <= w.n_kb) {
                         ok = stage(0, i == 0) && stage(1, false) && stage(2, false);
@@ -449,8 +472,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     }
                     if (s == R) { s = 0; phase ^= 1u; }
                 }
-                if (ok) umma_commit(smem_u32(&acc_full[b]));
-                if (PAIR && ok) umma_commit(smem_u32(&acc_full[1]));
+                if (PAIR && ok) umma_commit(smem_u32(&acc_full[0]));
+                if (ok) umma_commit(smem_u32(&acc_full[PAIR ? 1 : b]));
                 u = after(u, w);
             }
             if (!ok) *bail = 1;
@@ -460,8 +483,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         // ---------------- decode: a thread a feature; weight tiles it = group, group + G, ... (of a pair, always the same one) ----------------
         // (A wait names a phase by its parity alone, and a group does not come to every slot in every round of a ring.  It comes every
         // TURNS stages and has seen the MMAs of the stage TURNS + R ago done, so with TURNS <= R no slot of that ring is two rounds
-        // behind, and with WS >= GROUPS + TILES R none of the weights'; x_full is looked at behind done, by which the round before
-        // it has arrived.)
+        // behind, and with WS >= GROUPS + TILES R none of the weights'.)
         const int quarter = warp & 3, row = quarter * 32 + lane, group = (warp - 4) >> 2;
         const uint32_t lanes = ring + ((uint32_t)(quarter * 32) << 16);
         constexpr int TURNS = F::TURNS;
@@ -478,11 +500,10 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 // one of the four warps asks: twenty that ask at every barrier again and again take half of the issue slots
                 if (quarter == 0) {
                     ok = wait(&w_full[ws], w_phase);
-                    if (ok) ok = wait(&done[r], r_phase ^ 1u);           // the MMAs that read this buffer are done
-                    if (ok) ok = wait(&x_full[r], r_phase);
+                    if (ok) ok = wait(&done[r], r_phase ^ 1u);           // the MMAs that read this place are done
                     if (!ok) group_failed[2 * group + round] = 1;
                 }
-                asm volatile("bar.sync %0, 128;" ::"r"(4 + group) : "memory");
+                asm volatile("bar.sync %0, 128;" ::"r"(6 + group) : "memory");
                 ok = *(volatile int*)&group_failed[2 * group + round] == 0;      // (two flags in turn: the next round's is not seen yet)
                 round ^= 1;
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -524,7 +545,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         fb_pdl_wait();
         const int quarter = warp & 3, half = (warp - EPI_WARP) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 32 * EPI_WARP;
         const bool leader = quarter == 0 && lane == 0;
-        constexpr int STEP = CHUNK * 2;
+        constexpr int STEP = CHUNK * F::EPI_GROUPS;
         const uint32_t box_first = smem_u32(out_stage) + half * (OUT_BUFFERS * OUT_BYTES);       // the group's boxes
         const uint32_t box_last = box_first + (OUT_BUFFERS - 1) * OUT_BYTES;
         uint32_t box_at = box_first;
@@ -533,6 +554,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             Unit w = unit_at(u);
             const long following = after(u, w);
             bool stop = false;
+            const int shift = a.shifts[w.group];
+            const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
 #pragma unroll 1
             for (int h = 0; h < TILES; ++h, ++w.nt, ++w.id) {
             const bool both = w.n_tok <= SIDE_BY_SIDE, join = !GROUPED && w.shares > 1 && a.slabs == 0;
@@ -575,11 +598,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
                 if (*flag == 1) {
                     __threadfence();
-                    join_shares(a, w, tid, rows, a.partials + (size_t)w.id * a.max_segments * (size_t)(a.bn * MX_ROWS));
+                    join_shares<EPI>(a, w, tid, rows, a.partials + (size_t)w.id * a.max_segments * (size_t)(a.bn * MX_ROWS));
                 }
             } else {
-                const int shift = a.shifts[w.group];
-                const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
                 const int slab = a.slabs ? w.share : 0;
 #pragma unroll 1
                 for (int c = half * CHUNK; c < rows; c += STEP) {

@@ -225,16 +225,17 @@ tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scal
     dst[MX_CODE_BYTES + ((row & 31) * 4 + (row >> 5)) * 4 + (b & 3)] = (uint8_t)s;
 }
 
-// A thread eight numbers of each of four rows, which lie in one tile: parts[p][m][k] (bytes, rows of Kp, a multiple of 128, zeros behind
-// K), their scales as `layout` says.
-constexpr int SPLIT_COLS = 2048, SPLIT_ROWS = 4;
+// A thread a block of 32 numbers, SPLIT_ROWS rows (of one tile) a group of blocks: parts[p][m][k] (bytes, rows of Kp, a multiple of 128,
+// zeros behind K), their scales as `layout` says.
+constexpr int SPLIT_ROWS = 4;
 template <bool GROUPED>
 __global__ void __launch_bounds__(256)
 split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales,
              const __grid_constant__ MxScaleLayout layout) {
     fb_pdl_launch_dependents();
     fb_pdl_wait();
-    const int k = blockIdx.y * SPLIT_COLS + 8 * threadIdx.x, lane = threadIdx.x & 31, first = blockIdx.x * SPLIT_ROWS;
+    const int blocks = Kp / MX_BLOCK, lane = threadIdx.x & 31, first = blockIdx.x * SPLIT_ROWS;
+    const int item = blockIdx.y * 256 + threadIdx.x, q = item / blocks, m = first + q, k = (item - q * blocks) * MX_BLOCK;
     int unit, tokens, at, tiles;                         // the scales' tile, its tokens, the first row's place in it, all tiles
     if constexpr (GROUPED) {
         const int t = first / layout.tile, g = layout.tile_group[t];
@@ -264,29 +265,41 @@ split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t*
         at = first - unit * layout.tokens;
         tiles = (M + layout.tokens - 1) / layout.tokens;
     }
-    const int apart = tokens <= 64 ? tokens : (tokens + 127) / 128 * 128;
-    uint8_t* to = scales + ((size_t)(k >> 7) * tiles + unit) * layout.tile_bytes;
-    uint4 v[SPLIT_ROWS];
+    const bool mine = q < SPLIT_ROWS && m < M;           // (of the four lanes that share 128 columns all or none)
+    const int from = mine ? rows.index ? rows.index[m] : m : -1;
+    uint4 v[4];
 #pragma unroll
-    for (int q = 0; q < SPLIT_ROWS; ++q) v[q] = k < K && first + q < M ? mx_row8(rows, first + q, k, K) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) v[i] = make_uint4(0, 0, 0, 0);
+    if (from >= 0) {
+        const __nv_bfloat16* row = rows.x + (size_t)from * rows.ld;
 #pragma unroll
-    for (int q = 0; q < SPLIT_ROWS; ++q) {
-        const int m = first + q;
-        const uint32_t scale = mx_row_scale(mx_top8(v[q]));
-        uint2 one, two;
-        mx_split8({v[q].x, v[q].y, v[q].z, v[q].w}, scale, one, two);
-        // the four scales of 128 columns, which sixteen lanes share, as a word
-        const uint32_t s1 = __shfl_down_sync(0xffffffffu, scale, 4), s2 = __shfl_down_sync(0xffffffffu, scale, 8),
-                       s3 = __shfl_down_sync(0xffffffffu, scale, 12);
-        if (k >= Kp || m >= M) continue;
-        *reinterpret_cast<uint2*>(parts + (size_t)m * Kp + k) = one;
-        *reinterpret_cast<uint2*>(parts + ((size_t)M + m) * Kp + k) = two;
-        if ((lane & 15) == 0) {
-            const uint32_t word = scale | s1 << 8 | s2 << 16 | s3 << 24;
-            auto place = [](int row) { return (row >> 7) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4; };
-            *reinterpret_cast<uint32_t*>(to + place(at + q)) = word;
-            *reinterpret_cast<uint32_t*>(to + place(apart + at + q)) = mx_second_scales(word);
+        for (int i = 0; i < 4; ++i) v[i] = mx_load8(row, k + 8 * i, K, rows.aligned != 0);
+        if (rows.share) {
+            const float share = rows.share[rows.pair[m]];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = mx_times(v[i], share);
         }
+    }
+    const uint32_t two = __vmaxu2(__vmaxu2(mx_top8(v[0]), mx_top8(v[1])), __vmaxu2(mx_top8(v[2]), mx_top8(v[3])));
+    const uint32_t scale = mx_row_scale(max(two & 0xffffu, two >> 16));
+    const uint32_t half = scale | __shfl_down_sync(0xffffffffu, scale, 1) << 8, word = half | __shfl_down_sync(0xffffffffu, half, 2) << 16;
+    if (!mine) return;
+    uint4* to_first = reinterpret_cast<uint4*>(parts + (size_t)m * Kp + k);
+    uint4* to_second = reinterpret_cast<uint4*>(parts + ((size_t)M + m) * Kp + k);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint2 one[2], two[2];
+        mx_split8(v[2 * h], scale, one[0], two[0]);
+        mx_split8(v[2 * h + 1], scale, one[1], two[1]);
+        to_first[h] = make_uint4(one[0].x, one[0].y, one[1].x, one[1].y);
+        to_second[h] = make_uint4(two[0].x, two[0].y, two[1].x, two[1].y);
+    }
+    if ((lane & 3) == 0) {
+        const int apart = tokens <= 64 ? tokens : (tokens + 127) / 128 * 128;
+        uint8_t* to = scales + ((size_t)(k >> 7) * tiles + unit) * layout.tile_bytes;
+        auto place = [](int row) { return (row >> 7) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4; };
+        *reinterpret_cast<uint32_t*>(to + place(at + q)) = word;
+        *reinterpret_cast<uint32_t*>(to + place(apart + at + q)) = mx_second_scales(word);
     }
 }
 
@@ -366,8 +379,8 @@ FB_API int fb_mxfp4_tiles(const void* codes, const void* scales, int groups, int
 // a multiple of 128), `scales` what `layout` says, both 16-byte aligned.
 int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, const MxScaleLayout& layout, cudaStream_t stream) {
     const int Kp = (K + MX_COLS - 1) / MX_COLS * MX_COLS;
-    const dim3 grid((unsigned)((M + SPLIT_ROWS - 1) / SPLIT_ROWS), (unsigned)((Kp + SPLIT_COLS - 1) / SPLIT_COLS));
-    if (layout.tile_group) fb_launch(split_kernel<true>, grid, dim3(256), 0, stream, rows, M, K, Kp, (uint8_t*)parts, (uint8_t*)scales, layout);
-    else fb_launch(split_kernel<false>, grid, dim3(256), 0, stream, rows, M, K, Kp, (uint8_t*)parts, (uint8_t*)scales, layout);
+    const dim3 grid((unsigned)((M + SPLIT_ROWS - 1) / SPLIT_ROWS), (unsigned)((SPLIT_ROWS * (Kp / MX_BLOCK) + 255) / 256));
+    fb_launch(layout.tile_group ? split_kernel<true> : split_kernel<false>, grid, dim3(256), 0, stream, rows, M, K, Kp, (uint8_t*)parts,
+              (uint8_t*)scales, layout);
     return fb_check_launch("mxfp4_split_rows");
 }

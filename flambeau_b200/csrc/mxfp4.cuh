@@ -9,6 +9,8 @@
 
 #include "common.cuh"
 
+#include <cuda_fp16.h>
+
 constexpr int MX_BLOCK = 32;                                             // numbers that share a scale
 constexpr int MX_LAST_SCALE = 252;                                       // the largest that quantising writes: 6 x 2^125 is a float32
 constexpr int MX_ROWS = 128, MX_COLS = 128;                              // a tile
@@ -40,7 +42,7 @@ __device__ __forceinline__ float mx_scale_f32(uint32_t s) {
 
 // ---- rows of bfloat16 numbers as two e4m3 numbers each ----
 // With 2^e <= amax < 2^(e + 1) the largest magnitude of a block of 32, y = x 2^(7 - e) lies below 2^8; its first part is y rounded
-// to e4m3, its second what that left, times 2^5.  Eight bits of mantissa go into four and four: what is lost is below 2^-22 of amax.
+// to e4m3, its second what that left, times 2^5.  Eight bits of mantissa go into four and four: what is lost is 2^-22 of amax at most.
 // Scales: MX_FIRST less than the exponent's field for the first part, 5 less again for the second; blocks below 2^-115 use that
 // exponent's.  A block with an infinity or a NaN gets scales of 255, and so do the sums that it is part of.
 constexpr int MX_LEAST_FIELD = 12, MX_FIRST = 7, MX_SECOND_LESS = 5;
@@ -49,20 +51,22 @@ __device__ __forceinline__ uint32_t mx_row_scale(uint32_t top) {
     const uint32_t field = top >> 7;
     return field == 255u ? 255u : max(field, (uint32_t)MX_LEAST_FIELD) - MX_FIRST;
 }
-// Eight numbers (pairs in four words) under the block's scale: bytes of the first and the second parts.
-__device__ __forceinline__ void mx_split8(const uint32_t (&w)[4], uint32_t scale, uint2& first, uint2& second) {
+// Eight numbers (pairs in four words) under the block's scale: bytes of the first and the second parts.  y goes through half precision,
+// which holds eight bits of mantissa from 2^-14 on and is off by at most 2^-25 below.
+__device__ __forceinline__ void mx_split8(const uint4& eight, uint32_t scale, uint2& first, uint2& second) {
+    const uint32_t w[4] = {eight.x, eight.y, eight.z, eight.w};
     const float inv = __uint_as_float((scale == 255u ? 127u : 254u - scale) << 23);
+    const __half2 by = __float2half2_rn(32.0f);
     uint32_t h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float a = __uint_as_float(w[i] << 16) * inv, b = __uint_as_float(w[i] & 0xffff0000u) * inv;
+        const __half2 y = __floats2half2_rn(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
         uint16_t p, q;
         uint32_t back;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(p) : "f"(b), "f"(a));
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(p) : "r"(*reinterpret_cast<const uint32_t*>(&y)));
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(p));
-        float ra, rb;
-        asm("{\n\t.reg .f16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.f32.f16 %0, x;\n\tcvt.f32.f16 %1, y;\n\t}" : "=f"(ra), "=f"(rb) : "r"(back));
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(q) : "f"((b - rb) * 32.0f), "f"((a - ra) * 32.0f));
+        const __half2 left = __hmul2(__hsub2(y, *reinterpret_cast<const __half2*>(&back)), by);
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q) : "r"(*reinterpret_cast<const uint32_t*>(&left)));
         h[i] = p;
         l[i] = q;
     }
@@ -80,14 +84,10 @@ __device__ __forceinline__ uint4 mx_load8(const __nv_bfloat16* row, int k, int K
     for (int i = 0; i < 8; ++i) e[i] = k + i < K ? (uint32_t)__bfloat16_as_ushort(row[k + i]) : 0u;
     return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
 }
-// The largest magnitude's bits among eight numbers, and among the four lanes that share a block.
+// The largest magnitudes' bits among eight numbers, of the even and of the odd ones.
 __device__ __forceinline__ uint32_t mx_top8(const uint4& v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    return max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    constexpr uint32_t MAGNITUDES = 0x7fff7fffu;
+    return __vmaxu2(__vmaxu2(v.x & MAGNITUDES, v.y & MAGNITUDES), __vmaxu2(v.z & MAGNITUDES, v.w & MAGNITUDES));
 }
 
 // Rows that a product reads: row m is x[m], or x[index[m]] (negative: zeros), times share[pair[m]] (rounded to bfloat16) where
@@ -104,13 +104,6 @@ __device__ __forceinline__ uint4 mx_times(uint4 v, float f) {
         const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
         w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    return v;
-}
-__device__ __forceinline__ uint4 mx_row8(const MxRows& r, int m, int k, int K) {
-    const int from = r.index ? r.index[m] : m;
-    if (from < 0) return make_uint4(0, 0, 0, 0);
-    uint4 v = mx_load8(r.x + (size_t)from * r.ld, k, K, r.aligned != 0);
-    if (r.share) v = mx_times(v, r.share[r.pair[m]]);
     return v;
 }
 // Where the rows' scales go: [K / 128][token tile][tile_bytes], for a tile of n tokens the first parts as rows 0 .. and the second ones
