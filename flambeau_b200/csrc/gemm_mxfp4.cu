@@ -57,7 +57,7 @@ constexpr int TMEM = 512, SMEM = 227 * 1024;
 template <int TOK, bool PAIR> struct Form {
     static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow form cuts the line of tiles, and stores directly)
     static constexpr int TILES = PAIR ? 2 : 1;
-    static constexpr int R = TOK <= NARROW_TOKENS ? 8 : PAIR ? 3 : 4;
+    static constexpr int R = TOK <= NARROW_TOKENS ? 8 : TOK <= SIDE_BY_SIDE ? 6 : PAIR ? 3 : 4;
     static constexpr int GROUPS = TOK <= NARROW_TOKENS ? 4 : PAIR ? 2 : 3;
     static constexpr int EPI_GROUPS = PAIR ? 4 : 2, EPI = 128 * EPI_GROUPS;   // groups of four warps, threads of the epilogue
     static constexpr int TURNS = GROUPS / TILES;                         // groups that take a feature tile's stages in turn
@@ -175,25 +175,26 @@ __device__ __forceinline__ void st_shared(uint32_t addr, __nv_bfloat16 v) {
     asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(__bfloat16_as_ushort(v)) : "memory");
 }
 
-// The shares of a row tile, n_tok x 128 float32 each, added in order; a thread has four neighbouring features of a token.  (As the epilogue's own lanes lie, one share after the other, this took 4 us of a call.)
-template <int EPI> __device__ __noinline__ void join_shares(const MxArgs& a, const Unit& w, int tid, int rows, const float* __restrict__ base) {
-    const size_t step = (size_t)a.bn * (MX_ROWS / 4);
-    const int shift = a.shifts[w.group];
-    const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
+// The shares of a row tile, `step` float4 apart, added in order; a thread has four neighbouring features of a token, n .. n + 3 of row
+// m0 + e / 32.  (What it needs comes by value: read through a reference again and again, behind every store, it made this ten times as long.)
+template <int EPI>
+__device__ __noinline__ void join_shares(const float4* __restrict__ base, size_t step, int shares, int all, int tid, float raise, void* out,
+                                         long ldo, int m0, int n0, int N, int act, float limit, float slope, int plain_act, int o_bf16,
+                                         int accumulate) {
     constexpr int U = 4;                         // sums of a thread at a time, two shares of each on their way
-    const int all = rows * (MX_ROWS / 4);
+    const FbGate gate = {act, limit, slope};
     for (int e0 = tid; e0 < all; e0 += U * EPI) {
         float4 sum[U];
 #pragma unroll
         for (int q = 0; q < U; ++q) sum[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4* p = reinterpret_cast<const float4*>(base) + e0;
-        for (int s = 0; s < w.shares; s += 2, p += 2 * step) {
+        const float4* p = base + e0;
+        for (int s = 0; s < shares; s += 2, p += 2 * step) {
             float4 t[2][U];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int q = 0; q < U; ++q)
-                    t[h][q] = s + h < w.shares && e0 + q * EPI < all ? __ldcg(p + h * step + q * EPI) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    t[h][q] = s + h < shares && e0 + q * EPI < all ? __ldcg(p + h * step + q * EPI) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -205,29 +206,29 @@ template <int EPI> __device__ __noinline__ void join_shares(const MxArgs& a, con
         for (int q = 0; q < U; ++q) {
             const int e = e0 + q * EPI;
             if (e >= all) break;
-            const int m = w.m0 + e / (MX_ROWS / 4), n = w.nt * MX_ROWS + 4 * (e % (MX_ROWS / 4));
+            const int m = m0 + e / (MX_ROWS / 4), n = n0 + 4 * (e % (MX_ROWS / 4));
             float v[4] = {sum[q].x * raise, sum[q].y * raise, sum[q].z * raise, sum[q].w * raise};
-            int count = 4, columns = a.N, col = n;
-            if (a.gate.act) {                    // features alternate gate, up
+            int count = 4, columns = N, col = n;
+            if (act) {                           // features alternate gate, up
                 float g[2] = {v[0], v[2]};
                 const float u[2] = {v[1], v[3]};
-                gate_all(a.gate, g, u);
+                gate_all(gate, g, u);
                 v[0] = g[0];
                 v[1] = g[1];
-                count = 2; columns = a.N / 2; col = n / 2;
-            } else if (a.plain_act) {
+                count = 2; columns = N / 2; col = n / 2;
+            } else if (plain_act) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = act_slowly(a.plain_act, v[i]);
+                for (int i = 0; i < 4; ++i) v[i] = act_slowly(plain_act, v[i]);
             }
-            const size_t at = (size_t)m * a.ldo + col;
+            const size_t at = (size_t)m * ldo + col;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (i >= count || col + i >= columns) break;
-                if (a.o_bf16) {
-                    reinterpret_cast<__nv_bfloat16*>(a.out)[at + i] = __float2bfloat16_rn(v[i]);
+                if (o_bf16) {
+                    reinterpret_cast<__nv_bfloat16*>(out)[at + i] = __float2bfloat16_rn(v[i]);
                 } else {
-                    float* o = reinterpret_cast<float*>(a.out) + at + i;
-                    *o = a.accumulate ? *o + v[i] : v[i];
+                    float* o = reinterpret_cast<float*>(out) + at + i;
+                    *o = accumulate ? *o + v[i] : v[i];
                 }
             }
         }
@@ -330,6 +331,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         return w;
     };
+    // CTAs of neighbouring row tiles want the same rows: each begins at another place along K, or they would all ask for the same few
+    // lines of L2 at once.
+    auto first_tile = [&](const Unit& w) { return GROUPED ? w.nt / TILES % w.n_kb : 0; };
     auto after = [&](long item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
 
     if (warp == 0) {
@@ -340,6 +344,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             for (long u = first; u < last && !bailed();) {
                 const Unit w = unit_at(u);
                 const uint8_t* src = a.W + (size_t)w.group * a.w_group + ((size_t)w.nt * a.kb + w.kb0) * MX_TILE_BYTES;
+                int k = first_tile(w);
                 // (a pair's second tile that is none of the matrix is its first one again: nobody stores what comes of it)
                 const size_t next = w.nt + 1 < a.tiles_n ? (size_t)a.kb * MX_TILE_BYTES : 0;
                 bool ok = true;
@@ -347,8 +352,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     ok = wait(&w_empty[s], phase);
                     if (!ok) break;
                     mbar_expect_tx(smem_u32(&w_full[s]), MX_TILE_BYTES);
-                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES), src + (size_t)(i / TILES) * MX_TILE_BYTES + (i % TILES) * next,
+                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES), src + (size_t)k * MX_TILE_BYTES + (i % TILES) * next,
                                   MX_TILE_BYTES, smem_u32(&w_full[s]));
+                    if (i % TILES == TILES - 1 && ++k == w.n_kb) k = 0;
                     if (++s == WS) { s = 0; phase ^= 1u; }
                 }
                 if (!ok) *bail = 1;
@@ -365,6 +371,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             for (long u = first; u < last && !bailed();) {
                 const Unit w = unit_at(u);
                 const int boxes = GROUPED ? w.n_tok / a.tile : 1, box = GROUPED ? a.tile : a.bn;
+                int k = first_tile(w);
                 for (int i = 0; i < w.n_kb; ++i) {
                     if (!wait(&done[s], phase)) { *bail = 1; break; }
                     const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES);
@@ -373,11 +380,12 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     for (int b = 0; b < boxes; ++b) {
 #pragma unroll
                         for (int p = 0; p < 2; ++p)          // (rows beyond M are the other part's, or zeros: nobody stores them)
-                            tma_load_2d(dst + (uint32_t)(p * w.n_tok + b * box) * 128, &map_x, bar, (w.kb0 + i) * 64, p * a.M + w.m0 + b * box);
+                            tma_load_2d(dst + (uint32_t)(p * w.n_tok + b * box) * 128, &map_x, bar, (w.kb0 + k) * 64, p * a.M + w.m0 + b * box);
                     }
                     const size_t tiles = GROUPED ? a.n_tiles : a.tiles_m, tile = w.m0 / (GROUPED ? a.tile : a.bn);
-                    const size_t at = ((size_t)(w.kb0 + i) * tiles + tile) * a.scale_bytes;
+                    const size_t at = ((size_t)(w.kb0 + k) * tiles + tile) * a.scale_bytes;
                     bulk_copy_g2s(dst + TOK * 256, a.x_scales + at, scale_bytes, bar);
+                    if (++k == w.n_kb) k = 0;
                     if (++s == R) { s = 0; phase ^= 1u; }
                 }
                 u = after(u, w);
@@ -455,18 +463,19 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                         if (++s == R) { s = 0; phase ^= 1u; }
                     }
                 }
-                while (i < w.n_kb && ok) {
-                    static_assert(R == 3 || R == 4 || R == 8, "blocks of three or four places");
-                    if (R == 3 && s == 0 && i + 3 <= w.n_kb) {
-                        ok = stage(0, i == 0) && stage(1, false) && stage(2, false);
-                        s = 3; i += 3;
-                    } else if (R != 3 && s == 0 && i + 4 <= w.n_kb) {
-                        ok = stage(0, i == 0) && stage(1, false) && stage(2, false) && stage(3, false);
-                        s = 4; i += 4;
-                    } else if (R == 8 && s == 4 && i + 4 <= w.n_kb) {
-                        ok = stage(4, i == 0) && stage(5, false) && stage(6, false) && stage(7, false);
-                        s = 8; i += 4;
-                    } else {
+                while (ok && i < w.n_kb) {
+                    constexpr int B = R % 4 == 0 ? 4 : 3;
+                    static_assert(R % B == 0, "blocks of three or four places");
+                    const int before = i;
+#pragma unroll
+                    for (int p = 0; p < R; p += B) {
+                        if (!ok || s != p || i + B > w.n_kb) continue;
+#pragma unroll
+                        for (int q = 0; q < B; ++q) ok = ok && stage(p + q, q == 0 && i == 0);
+                        s = p + B;
+                        i += B;
+                    }
+                    if (i == before) {
                         ok = stage(s, i == 0);
                         ++s; ++i;
                     }
@@ -598,7 +607,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 asm volatile("bar.sync 1, %0;" ::"n"(EPI) : "memory");
                 if (*flag == 1) {
                     __threadfence();
-                    join_shares<EPI>(a, w, tid, rows, a.partials + (size_t)w.id * a.max_segments * (size_t)(a.bn * MX_ROWS));
+                    join_shares<EPI>(reinterpret_cast<const float4*>(a.partials) + (size_t)w.id * a.max_segments * (size_t)(a.bn * (MX_ROWS / 4)),
+                                     (size_t)a.bn * (MX_ROWS / 4), w.shares, rows * (MX_ROWS / 4), tid, raise, a.out, a.ldo, w.m0, n0, a.N,
+                                     a.gate.act, a.gate.limit, a.gate.slope, a.plain_act, a.o_bf16, a.accumulate);
                 }
             } else {
                 const int slab = a.slabs ? w.share : 0;
@@ -721,7 +732,7 @@ int segments_of(long tiles_n, long kb, long grid) {           // the most stretc
 // more than `limit`.
 // Where shares have to meet (`join`), row tiles stay whole if the longest stretch and the meeting take longer.  In cycles: STAGE for
 // a tile of an SM, JOIN for the partial sums' way through L2 and back.
-constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 4000;
+constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 6000;
 struct Cut { int grid, segments; };
 Cut cut_of(int tiles_n, int kb, int limit, bool join) {
     static std::map<std::tuple<int, int, int, int>, Cut> known;              // (counting through the tiles takes microseconds)
@@ -747,9 +758,14 @@ int narrow_tokens(int M) { return (M + 7) / 8 * 8; }
 struct Plan { int bn, splits; bool pair; };
 constexpr int MORE_TILES = 2;
 constexpr double L2_BYTES = 62.0;                 // what an SM gets from L2 a cycle when all of them ask
-// The cheapest of the choices in cycles of an SM.  A stage costs its MMAs (2 cycles a column, at least 46 an instruction) or its
-// decoding or its way from L2, whichever is most; all CTAs together no less than the weights from HBM.  A share of K costs a copy of the output, written
-// and read.
+// The cheapest of the choices in cycles of an SM.  A stage costs its MMAs (2 cycles a column, twice for two parts of more than 64
+// tokens), its way from L2 or its decoding, whichever is most; all CTAs together no less than the weights from HBM.  Decoding's
+// cost grows with the CTAs: products that follow one another overlap on the SMs that the first leaves free (67 x 6,144 x 5,120 one after the
+// other: 96 CTAs 12.9 us, 144 of fewer tokens 17.2; each by itself about 19.5).  A pair's epilogue overlaps little of the next
+// one's products (100 cycles a token for both tiles), of a single tile's only the last one's shows.  Shares of K cost a copy of the output,
+// written and read, and where they meet the adding, which nothing overlaps (67 x 6,144 x 5,120: three shares 21 us, whole 15.6 with
+// the same tiles).  Where it decides for or against pairs: 301 x 28,672 x 4,096 68 us single, 80 in pairs; 2,048 x 4,096 x 14,336
+// 225 single, 200 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.
 Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
     const long sms = fb_sm_count(), tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     Plan best = {WIDE_TOKENS, 1, false};
@@ -762,14 +778,14 @@ Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int 
             if (pair && bn <= SIDE_BY_SIDE) continue;
             const long units_n = pair ? (tiles_n + 1) / 2 : tiles_n;
             const double l2 = (bn * 256.0 + (pair ? 2 : 1) * (double)MX_TILE_BYTES) / L2_BYTES;
-            const double stage = fmax(fmax((pair ? 8.0 : 4.0) * bn, l2) + 30.0, pair ? 520.0 : 300.0);
             for (int splits = 1; splits <= max_splits && splits <= kb; ++splits) {
                 if (!slabs && splits > 1 && (tiles * tiles_n > n_counters || tiles * tiles_n * splits * bn * MX_ROWS > partial_floats)) break;
-                const long rounds = (tiles * units_n * splits + sms - 1) / sms;
-                // (a pair's epilogue does not overlap the products of the next one)
-                double cost = fmax((double)rounds * ((kb + splits - 1) / splits * stage + (pair ? 35.0 * bn : 500.0)),
+                const long units = tiles * units_n * splits, rounds = (units + sms - 1) / sms;
+                const double stage = fmax(fmax((pair ? 8.0 : 4.0) * bn, l2), pair ? 490.0 : 300.0 + (double)(units < sms ? units : sms)) + 30.0;
+                double cost = fmax((double)rounds * ((kb + splits - 1) / splits * stage + (pair ? 100.0 * bn : 500.0)) + (pair ? 0.0 : 45.0 * bn),
                                    (double)tiles_n * kb * MX_TILE_BYTES / (23.0 * sms));
-                cost += (splits - 1) * (double)M * N * 8.0 / (24.0 * sms) + (splits > 1 && !slabs ? 3000.0 : 0.0);
+                cost += (splits - 1) * (double)M * N * 8.0 / (24.0 * sms);
+                if (splits > 1 && !slabs) cost += (double)rounds * (4000.0 + (pair ? 190.0 : 150.0) * bn);
                 if (cost < best_cost * (1.0 - 1e-9)) { best_cost = cost; best = Plan{bn, splits, pair != 0}; }
             }
         }
