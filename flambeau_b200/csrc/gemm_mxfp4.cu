@@ -43,7 +43,8 @@ constexpr int CHUNK = 16;                         // tokens that a group of four
 constexpr int OUT_BYTES = 4096, OUT_BUFFERS = 3;  // a staged box of the output: 16 tokens, 8 of ungated float32
 constexpr int FLAGS = 640;                        // bytes of barriers and flags
 constexpr int CONTROL = FLAGS + 4 * LIST;         // and the list
-constexpr int NARROW_TOKENS = 32, WIDE_TOKENS = 128;      // most tokens of a tile of either form
+constexpr int FEW_TOKENS = 8, NARROW_TOKENS = 32, WIDE_TOKENS = 128;      // most tokens of a tile of each form
+constexpr int SPLITTERS = 8;                      // warps that make the parts of few rows
 constexpr int SIDE_BY_SIDE = 64;                  // most tokens whose two parts are one operand
 constexpr int ATOM = 512;                         // scales of 128 rows for a stage, as tcgen05.cp brings them to tensor memory
 constexpr int TMEM = 512, SMEM = 227 * 1024;
@@ -55,13 +56,14 @@ constexpr int TMEM = 512, SMEM = 227 * 1024;
 // those of successive units.  Many tokens want it: a CTA's rows come from L2, whose bandwidth was the bound (82 bytes a cycle and SM
 // for 128 x 128, like this 49).
 template <int TOK, bool PAIR> struct Form {
-    static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow form cuts the line of tiles, and stores directly)
+    static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow forms cut the line of tiles, and store directly)
+    static constexpr bool FEW = TOK <= FEW_TOKENS;
     static constexpr int TILES = PAIR ? 2 : 1;
     static constexpr int R = TOK <= NARROW_TOKENS ? 8 : TOK <= SIDE_BY_SIDE ? 6 : PAIR ? 3 : 4;
-    static constexpr int GROUPS = TOK <= NARROW_TOKENS ? 4 : PAIR ? 2 : 3;
-    static constexpr int EPI_GROUPS = PAIR ? 4 : 2, EPI = 128 * EPI_GROUPS;   // groups of four warps, threads of the epilogue
+    static constexpr int GROUPS = FEW ? 3 : TOK <= NARROW_TOKENS ? 4 : PAIR ? 2 : 3;
+    static constexpr int EPI_GROUPS = FEW ? 1 : PAIR ? 4 : 2, EPI = 128 * EPI_GROUPS;   // groups of four warps, threads of the epilogue
     static constexpr int TURNS = GROUPS / TILES;                         // groups that take a feature tile's stages in turn
-    static constexpr int EPI_WARP = 4 + 4 * GROUPS, THREADS = 32 * EPI_WARP + EPI;
+    static constexpr int EPI_WARP = 4 + 4 * GROUPS, SPLIT_WARP = EPI_WARP + EPI / 32, THREADS = 32 * (SPLIT_WARP + (FEW ? SPLITTERS : 0));
     static constexpr int ATOMS = TOK <= SIDE_BY_SIDE ? 1 : 2 * ((TOK + 127) / 128);
     static constexpr int ACC_COLS = TOK <= SIDE_BY_SIDE ? 2 * TOK : TOK;
     static constexpr int W_COLS = A_COLS + SFA_COLS;
@@ -363,8 +365,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         __syncwarp();
     } else if (warp == 2) {
-        // ---------------- the rows' parts and their scales ----------------
-        if (elect_one()) {
+        // ---------------- the rows' parts and their scales (of few rows: see the last warps) ----------------
+        if (!F::FEW && elect_one()) {
             fb_pdl_wait();
             int s = 0;
             uint32_t phase = 1;
@@ -549,7 +551,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             u = after(u, w);
         }
         if (!ok) *bail = 1;
-    } else if (warp >= EPI_WARP) {
+    } else if (warp >= EPI_WARP && warp < F::SPLIT_WARP) {
         // ---------------- epilogue: lanes are features, the two groups of four warps take 16 tokens in turn ----------------
         fb_pdl_wait();
         const int quarter = warp & 3, half = (warp - EPI_WARP) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 32 * EPI_WARP;
@@ -709,6 +711,52 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             u = following;
         }
         if (WIDE && leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");        // the boxes it sent are in memory
+    } else if (F::FEW && warp >= F::SPLIT_WARP) {
+        // ---------------- few rows' parts: stages it = turn, turn + SPLITTERS, ..., a lane a block of 32 of row lane / 4 ----------------
+        fb_pdl_wait();
+        const int turn = warp - F::SPLIT_WARP, block = lane & 3, r = lane >> 2;
+        const __nv_bfloat16* row = r < a.M ? a.rows.x + (size_t)r * a.rows.ld : nullptr;
+        int s = turn;
+        uint32_t phase = 1, it = 0;
+        bool ok = true;
+        for (long u = first; u < last && ok;) {
+            const Unit w = unit_at(u);
+            uint4 raw[4];
+            auto load = [&](int i) {                                     // what the lane splits of the unit's i-th stage
+                const int k = (w.kb0 + i) * MX_COLS + block * MX_BLOCK;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) raw[q] = row ? mx_load8(row, k + 8 * q, a.K, a.rows.aligned != 0) : make_uint4(0, 0, 0, 0);
+            };
+            int i = turn - (int)it;                                      // the warp's first stage of the unit
+            if (i < 0) i += SPLITTERS;
+            if (i < w.n_kb) load(i);
+            for (; i < w.n_kb; i += SPLITTERS) {
+                uint2 one[4], two[4];
+                const uint32_t word = mx_split_block(raw, one, two);
+                if (i + SPLITTERS < w.n_kb) load(i + SPLITTERS);
+                if (lane == 0) ok = wait(&done[s], phase);               // the MMAs that read this place are done
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                uint8_t* stage = smem + s * F::STAGE_BYTES;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {                            // rows of 128 bytes, their sixteens swizzled by the row's place in eight
+                    const int at = r + p * w.n_tok;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint2 lo = p ? two[2 * h] : one[2 * h], hi = p ? two[2 * h + 1] : one[2 * h + 1];
+                        *reinterpret_cast<uint4*>(stage + at * 128 + (((2 * block + h) ^ (at & 7)) << 4)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    }
+                    if (block == 0) *reinterpret_cast<uint32_t*>(stage + TOK * 256 + mx_scale_place(at)) = p ? mx_second_scales(word) : word;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&full[s]));
+                if ((s += SPLITTERS) >= R) { s -= R; phase ^= 1u; }
+            }
+            it = (it + (uint32_t)w.n_kb) % SPLITTERS;
+            u = after(u, w);
+        }
+        if (!ok) *bail = 1;
     }
     tmem_fence_before();
     __syncthreads();
@@ -814,9 +862,16 @@ long long scale_bytes_of(int M, int kb, int tile) {
     return kb * tiles * ATOM * (tile == 16 || (!tile && M <= SIDE_BY_SIDE) ? 1 : 2);
 }
 
+// Whether the form of few rows takes the product (tile: the grouped form's row tile, 0: not grouped).  A CTA splits what it multiplies: that
+// spares a kernel that 8 rows spent 4 to 8 us in, behind the weights that the product had on their way by then, and one until the
+// first MMA (8 x 4,096 x 14,336 17.3 us with that kernel, FEWUS without).  With 16 rows the splitting warps were too slow (16 x 28,672 x
+// 4,096 gated 30.8 us, with the kernel 23.9), and so they were where many row tiles share the rows of a group (93 us, 65).
+bool few_rows(int M, int tile) { return tile == 0 && M <= FEW_TOKENS; }
+
 // The rows' parts and scales in `scratch`, their map, the output's map.
 int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, int box_rows, cudaStream_t stream) {
     const bool grouped = a.tile_group != nullptr;
+    if (few_rows(a.M, a.tile)) return 0;                 // (the product splits them itself, and stores directly)
     const long Kp = (long)a.kb * MX_COLS, parts = 2L * a.M * Kp;
     a.x_scales = (const uint8_t*)scratch + parts;
     a.scale_bytes = atoms_of(a.bn) * ATOM;
@@ -853,7 +908,7 @@ int check_operands(const void* X, long long lda, const void* W, const int* shift
 
 // What the rows' parts and their scales take, a multiple of 256 bytes (tile: the grouped form's row tile, 0: not grouped).
 static long long rows_bytes(int M, int K, int tile) {
-    if (M <= 0 || K <= 0) return 0;
+    if (M <= 0 || K <= 0 || few_rows(M, tile)) return 0;
     const long long kb = (K + MX_COLS - 1) / MX_COLS;
     return (2LL * M * kb * MX_COLS + scale_bytes_of(M, (int)kb, tile) + 255) / 256 * 256;
 }
@@ -916,7 +971,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
             if (splits_used) *splits_used = cut.segments;
         }
         if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
-        return launch<32, false, false>(a, mx, mo, cut.grid, stream);
+        return few_rows(M, 0) ? launch<FEW_TOKENS, false, false>(a, mx, mo, cut.grid, stream) : launch<32, false, false>(a, mx, mo, cut.grid, stream);
     }
     const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, SHARE_FLOATS,
                                 n_counters, slabs);

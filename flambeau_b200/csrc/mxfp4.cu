@@ -280,26 +280,21 @@ split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t*
             for (int i = 0; i < 4; ++i) v[i] = mx_times(v[i], share);
         }
     }
-    const uint32_t two = __vmaxu2(__vmaxu2(mx_top8(v[0]), mx_top8(v[1])), __vmaxu2(mx_top8(v[2]), mx_top8(v[3])));
-    const uint32_t scale = mx_row_scale(max(two & 0xffffu, two >> 16));
-    const uint32_t half = scale | __shfl_down_sync(0xffffffffu, scale, 1) << 8, word = half | __shfl_down_sync(0xffffffffu, half, 2) << 16;
+    uint2 one[4], two[4];
+    const uint32_t word = mx_split_block(v, one, two);
     if (!mine) return;
     uint4* to_first = reinterpret_cast<uint4*>(parts + (size_t)m * Kp + k);
     uint4* to_second = reinterpret_cast<uint4*>(parts + ((size_t)M + m) * Kp + k);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        uint2 one[2], two[2];
-        mx_split8(v[2 * h], scale, one[0], two[0]);
-        mx_split8(v[2 * h + 1], scale, one[1], two[1]);
-        to_first[h] = make_uint4(one[0].x, one[0].y, one[1].x, one[1].y);
-        to_second[h] = make_uint4(two[0].x, two[0].y, two[1].x, two[1].y);
+        to_first[h] = make_uint4(one[2 * h].x, one[2 * h].y, one[2 * h + 1].x, one[2 * h + 1].y);
+        to_second[h] = make_uint4(two[2 * h].x, two[2 * h].y, two[2 * h + 1].x, two[2 * h + 1].y);
     }
     if ((lane & 3) == 0) {
         const int apart = tokens <= 64 ? tokens : (tokens + 127) / 128 * 128;
         uint8_t* to = scales + ((size_t)(k >> 7) * tiles + unit) * layout.tile_bytes;
-        auto place = [](int row) { return (row >> 7) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4; };
-        *reinterpret_cast<uint32_t*>(to + place(at + q)) = word;
-        *reinterpret_cast<uint32_t*>(to + place(apart + at + q)) = mx_second_scales(word);
+        *reinterpret_cast<uint32_t*>(to + mx_scale_place(at + q)) = word;
+        *reinterpret_cast<uint32_t*>(to + mx_scale_place(apart + at + q)) = mx_second_scales(word);
     }
 }
 

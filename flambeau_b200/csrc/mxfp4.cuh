@@ -90,6 +90,19 @@ __device__ __forceinline__ uint32_t mx_top8(const uint4& v) {
     return __vmaxu2(__vmaxu2(v.x & MAGNITUDES, v.y & MAGNITUDES), __vmaxu2(v.z & MAGNITUDES, v.w & MAGNITUDES));
 }
 
+// A block of 32 numbers of a row, of which four neighbouring lanes have the four of 128 columns: its parts, and for the first of the
+// four lanes their scales.
+__device__ __forceinline__ uint32_t mx_split_block(const uint4 (&v)[4], uint2 (&one)[4], uint2 (&two)[4]) {
+    const uint32_t top = __vmaxu2(__vmaxu2(mx_top8(v[0]), mx_top8(v[1])), __vmaxu2(mx_top8(v[2]), mx_top8(v[3])));
+    const uint32_t scale = mx_row_scale(max(top & 0xffffu, top >> 16));
+    const uint32_t half = scale | __shfl_down_sync(0xffffffffu, scale, 1) << 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx_split8(v[i], scale, one[i], two[i]);
+    return half | __shfl_down_sync(0xffffffffu, half, 2) << 16;
+}
+// Where a row's word of scales lies among those of a tile.
+__device__ __forceinline__ int mx_scale_place(int row) { return (row >> 7) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4; }
+
 // Rows that a product reads: row m is x[m], or x[index[m]] (negative: zeros), times share[pair[m]] (rounded to bfloat16) where
 // there are shares.
 struct MxRows {
