@@ -37,7 +37,7 @@ namespace {
 
 constexpr int A_COLS = MX_COLS / 4;               // tensor-memory columns of a stage's weights, then of their scales
 constexpr int SFA_COLS = 4;
-constexpr int MAX_W = 16, MAX_R = 8;              // most stages of packed weights / of rows and decoded weights
+constexpr int MAX_W = 24, MAX_R = 8;              // most stages of packed weights / of rows and decoded weights
 constexpr int LIST = 512;                         // units of the grouped form that are kept in shared memory
 constexpr int CHUNK = 16;                         // tokens that a group of four epilogue warps takes at a time
 constexpr int OUT_BYTES = 4096, OUT_BUFFERS = 3;  // a staged box of the output: 16 tokens, 8 of ungated float32
@@ -72,7 +72,8 @@ template <int TOK, bool PAIR> struct Form {
     static constexpr int OUT = WIDE ? EPI_GROUPS * OUT_BUFFERS * OUT_BYTES : 0;
     static constexpr int RING = SMEM - 1024 - CONTROL - OUT;             // for the rings of stages
     static constexpr int FIT = (RING - R * STAGE_BYTES) / MX_TILE_BYTES;
-    static constexpr int WS = FIT < MAX_W ? FIT : MAX_W;
+    static constexpr int PRODUCERS = WIDE ? 1 : 2;                       // threads that ask for weights, each for places of its own
+    static constexpr int WS = (FIT < MAX_W ? FIT : MAX_W) / PRODUCERS * PRODUCERS;
     static_assert(2 * ACC_COLS + R * RING_COLS <= TMEM, "tensor memory");
     static_assert(TURNS <= R && WS >= GROUPS + TILES * R, "a wait names a phase by its parity: see the decoding warps");
 };
@@ -81,7 +82,7 @@ template <int TOK, bool PAIR> struct Form {
 __host__ __device__ constexpr int atoms_of(int tokens) { return tokens <= SIDE_BY_SIDE ? 1 : 2 * ((tokens + 127) / 128); }
 
 struct MxArgs {
-    const uint8_t* W; long w_group; const int* shifts;    // tiles, bytes of one group's, what each group's results are raised by
+    const uint8_t* W; long w_group;                       // tiles, bytes of one group's
     MxRows rows;                                          // what X's parts, which come by map_x, are made from
     const uint8_t* x_scales; int scale_bytes;             // their scales, bytes of a tile's
     void* out; long ldo, slab_stride;
@@ -104,8 +105,8 @@ __device__ __forceinline__ void mma_mx(uint32_t d, uint32_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], [%1], %2, %3, [%4], [%5], p;\n\t}"
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
 }
-// e4m3 x e4m3 -> f32 under E8M0 scales, M = 128; the k-th block of 32 of a stage takes byte k of the scales' words.
-__device__ __forceinline__ uint32_t mx_idesc(int n) { return ((uint32_t)(n >> 3) << 17) | (1u << 23) | (8u << 24); }
+// e2m1 x e4m3 -> f32 under E8M0 scales, M = 128; the k-th block of 32 of a stage takes byte k of the scales' words.
+__device__ __forceinline__ uint32_t mx_idesc(int n) { return (5u << 7) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (8u << 24); }
 __device__ __forceinline__ constexpr uint32_t mx_block(int k) { return ((uint32_t)k << 4) | ((uint32_t)k << 29); }
 // 512 bytes of scales, [lane i][j] words of row 32 j + i, into four columns, the same in every quarter of the lanes; in order with the
 // MMAs of the same thread.
@@ -180,7 +181,7 @@ __device__ __forceinline__ void st_shared(uint32_t addr, __nv_bfloat16 v) {
 // The shares of a row tile, `step` float4 apart, added in order; a thread has four neighbouring features of a token, n .. n + 3 of row
 // m0 + e / 32.  (What it needs comes by value: read through a reference again and again, behind every store, it made this ten times as long.)
 template <int EPI>
-__device__ __noinline__ void join_shares(const float4* __restrict__ base, size_t step, int shares, int all, int tid, float raise, void* out,
+__device__ __noinline__ void join_shares(const float4* __restrict__ base, size_t step, int shares, int all, int tid, void* out,
                                          long ldo, int m0, int n0, int N, int act, float limit, float slope, int plain_act, int o_bf16,
                                          int accumulate) {
     constexpr int U = 4;                         // sums of a thread at a time, two shares of each on their way
@@ -209,7 +210,7 @@ __device__ __noinline__ void join_shares(const float4* __restrict__ base, size_t
             const int e = e0 + q * EPI;
             if (e >= all) break;
             const int m = m0 + e / (MX_ROWS / 4), n = n0 + 4 * (e % (MX_ROWS / 4));
-            float v[4] = {sum[q].x * raise, sum[q].y * raise, sum[q].z * raise, sum[q].w * raise};
+            float v[4] = {sum[q].x, sum[q].y, sum[q].z, sum[q].w};
             int count = 4, columns = N, col = n;
             if (act) {                           // features alternate gate, up
                 float g[2] = {v[0], v[2]};
@@ -338,28 +339,30 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     auto first_tile = [&](const Unit& w) { return GROUPED ? w.nt / TILES % w.n_kb : 0; };
     auto after = [&](long item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
 
-    if (warp == 0) {
+    if (warp == 0 || (F::PRODUCERS == 2 && warp == 3)) {
         // ---------------- weights: no other kernel writes them, so they are requested at once ----------------
         if (elect_one()) {
-            int s = 0;
+            const int turn = warp == 0 ? 0 : 1;
+            int s = turn, i = turn;                  // i: the thread's first tile of the unit
             uint32_t phase = 1;
             for (long u = first; u < last && !bailed();) {
                 const Unit w = unit_at(u);
                 const uint8_t* src = a.W + (size_t)w.group * a.w_group + ((size_t)w.nt * a.kb + w.kb0) * MX_TILE_BYTES;
-                int k = first_tile(w);
                 // (a pair's second tile that is none of the matrix is its first one again: nobody stores what comes of it)
                 const size_t next = w.nt + 1 < a.tiles_n ? (size_t)a.kb * MX_TILE_BYTES : 0;
+                const int begin = first_tile(w), tiles = TILES * w.n_kb;
                 bool ok = true;
-                for (int i = 0; i < TILES * w.n_kb && ok; ++i) {
+                for (; i < tiles; i += F::PRODUCERS) {
                     ok = wait(&w_empty[s], phase);
                     if (!ok) break;
+                    const int k = begin + i / TILES;
                     mbar_expect_tx(smem_u32(&w_full[s]), MX_TILE_BYTES);
-                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES), src + (size_t)k * MX_TILE_BYTES + (i % TILES) * next,
-                                  MX_TILE_BYTES, smem_u32(&w_full[s]));
-                    if (i % TILES == TILES - 1 && ++k == w.n_kb) k = 0;
-                    if (++s == WS) { s = 0; phase ^= 1u; }
+                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES),
+                                  src + (size_t)(k < w.n_kb ? k : k - w.n_kb) * MX_TILE_BYTES + (i % TILES) * next, MX_TILE_BYTES, smem_u32(&w_full[s]));
+                    if ((s += F::PRODUCERS) >= WS) { s -= WS; phase ^= 1u; }
                 }
                 if (!ok) *bail = 1;
+                i -= tiles;
                 u = after(u, w);
             }
         }
@@ -565,8 +568,6 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             Unit w = unit_at(u);
             const long following = after(u, w);
             bool stop = false;
-            const int shift = a.shifts[w.group];
-            const float raise = shift > 0 ? ldexpf(1.0f, shift) : 1.0f;
 #pragma unroll 1
             for (int h = 0; h < TILES; ++h, ++w.nt, ++w.id) {
             const bool both = w.n_tok <= SIDE_BY_SIDE, join = !GROUPED && w.shares > 1 && a.slabs == 0;
@@ -610,7 +611,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 if (*flag == 1) {
                     __threadfence();
                     join_shares<EPI>(reinterpret_cast<const float4*>(a.partials) + (size_t)w.id * a.max_segments * (size_t)(a.bn * (MX_ROWS / 4)),
-                                     (size_t)a.bn * (MX_ROWS / 4), w.shares, rows * (MX_ROWS / 4), tid, raise, a.out, a.ldo, w.m0, n0, a.N,
+                                     (size_t)a.bn * (MX_ROWS / 4), w.shares, rows * (MX_ROWS / 4), tid, a.out, a.ldo, w.m0, n0, a.N,
                                      a.gate.act, a.gate.limit, a.gate.slope, a.plain_act, a.o_bf16, a.accumulate);
                 }
             } else {
@@ -619,10 +620,6 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 for (int c = half * CHUNK; c < rows; c += STEP) {
                     float v[16];
                     sums(c, v);
-                    if (__builtin_expect(shift > 0, 0)) {
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) v[q] *= raise;
-                    }
                     if (__builtin_expect(a.plain_act != 0, 0)) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) v[q] = act_slowly(a.plain_act, v[q]);
@@ -793,8 +790,9 @@ Cut cut_of(int tiles_n, int kb, int limit, bool join) {
     long grid = most < slots ? most : slots;
     int segments = segments_of(tiles_n, kb, grid);
     while (segments > limit && grid > 1) segments = segments_of(tiles_n, kb, --grid);
-    if (join && segments > 1 && tiles_n <= slots && ((long)tiles_n * kb + grid - 1) / grid * STAGE + JOIN >= (long)kb * STAGE) {
-        grid = tiles_n;
+    const long rounds = (tiles_n + slots - 1) / slots;
+    if (join && segments > 1 && tiles_n % rounds == 0 && ((long)tiles_n * kb + grid - 1) / grid * STAGE + JOIN >= rounds * kb * STAGE) {
+        grid = tiles_n / rounds;
         segments = 1;
     }
     if (known.size() > 4096) known.clear();
@@ -890,7 +888,7 @@ int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, int box_
     return rc < 0 ? rc : 0;
 }
 
-int check_operands(const void* X, long long lda, const void* W, const int* shifts, const void* out, int o_dtype, long long ldo, int M, int N,
+int check_operands(const void* X, long long lda, const void* W, const void* out, int o_dtype, long long ldo, int M, int N,
                    int K, FbGate gate, int plain_act, int* status) {
     FB_REQUIRE(M >= 0 && N > 0 && K > 0, "gemm_mxfp4: bad sizes M=%d N=%d K=%d", M, N, K);
     FB_REQUIRE(o_dtype == FB_F32 || o_dtype == FB_BF16, "gemm_mxfp4: unknown output dtype code %d", o_dtype);
@@ -898,8 +896,8 @@ int check_operands(const void* X, long long lda, const void* W, const int* shift
                "gemm_mxfp4: a gate needs a known activation, an even number of stacked rows and no plain activation beside it");
     FB_REQUIRE(fb_plain_act_known(plain_act), "gemm_mxfp4: unknown activation code %d", plain_act);
     FB_REQUIRE(lda >= K && ldo >= (gate.act ? N / 2 : N), "gemm_mxfp4: a row stride is shorter than its row");
-    FB_REQUIRE(((uintptr_t)X & 1) == 0 && W && ((uintptr_t)W & 15) == 0 && shifts && status,
-               "gemm_mxfp4: unaligned rows or weights, or no shifts, or no status word");
+    FB_REQUIRE(((uintptr_t)X & 1) == 0 && W && ((uintptr_t)W & 15) == 0 && status,
+               "gemm_mxfp4: unaligned rows or weights, or no status word");
     FB_REQUIRE(((uintptr_t)out & (o_dtype == FB_F32 ? 3 : 1)) == 0, "gemm_mxfp4: unaligned output");
     return 0;
 }
@@ -931,25 +929,25 @@ FB_API long long fb_gemm_mxfp4_scratch_bytes(int M, int N, int K, int n_counters
     return rows_bytes(M, K, tile) + (slabs || tile ? 0 : 4 * share_floats(M, N, K, n_counters));
 }
 
-// X [M,K] bfloat16, W one matrix in tiles with its shift (fb_mxfp4_tiles).  `act` (an FbAct code with its constants): W stacks gate
+// X [M,K] bfloat16, W one matrix in tiles (fb_mxfp4_tiles).  `act` (an FbAct code with its constants): W stacks gate
 // and up rows alternately and out[m, c] = act(g_c) u_c has N / 2 columns; `plain_act` (an FbPlainAct code): out = act(product);
 // `accumulate` (float32): the product is added to what `out` holds.  Shares of K: with slab_stride > 0 (float32, neither activation
 // nor accumulate) share s goes to out + s * slab_stride and *splits_used says how many there are (at most max_slabs); else they
 // meet in `scratch` and at `counters` (zero before the call and after it).  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a
 // 128-byte border, of calls that run one after the other.
-FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int* shifts, void* out, int o_dtype, long long ldo,
+FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out, int o_dtype, long long ldo,
                          long long slab_stride, int max_slabs, int* splits_used, int M, int N, int K, int act, float limit,
                          float slope, int plain_act, int accumulate, int* counters, int n_counters, void* scratch,
                          long long scratch_bytes, int* status, cudaStream_t stream) {
     const FbGate gate = {act, limit, slope};
-    if (const int rc = check_operands(X, lda, W, shifts, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
+    if (const int rc = check_operands(X, lda, W, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
     FB_REQUIRE(slab_stride == 0 || (o_dtype == FB_F32 && max_slabs >= 1 && slab_stride >= (long long)M * ldo && !act && !plain_act && !accumulate),
                "gemm_mxfp4: slabs must be float32, at least one, not overlap, and hold plain shares");
     FB_REQUIRE(!accumulate || (o_dtype == FB_F32 && !act && !plain_act), "gemm_mxfp4: only a float32 product can be added to its output");
     if (splits_used) *splits_used = 1;
     if (M == 0) return 0;
     MxArgs a = {};
-    a.W = (const uint8_t*)W; a.shifts = shifts; a.out = out; a.ldo = (long)ldo; a.slab_stride = (long)slab_stride;
+    a.W = (const uint8_t*)W; a.out = out; a.ldo = (long)ldo; a.slab_stride = (long)slab_stride;
     a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, nullptr, nullptr, nullptr};
     a.o_bf16 = o_dtype == FB_BF16; a.accumulate = accumulate; a.counters = counters;
     a.M = M; a.N = N; a.K = K; a.kb = (K + MX_COLS - 1) / MX_COLS; a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
@@ -991,17 +989,17 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, const int*
     return a.bn <= 64 ? launch<64, false, false>(a, mx, mo, grid, stream) : launch<128, false, false>(a, mx, mo, grid, stream);
 }
 
-// The grouped form: W holds `groups` matrices [N, K] in tiles with a shift each; the M rows of `out` come in tiles of `tile` (a
+// The grouped form: W holds `groups` matrices [N, K] in tiles; the M rows of `out` come in tiles of `tile` (a
 // multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are).  Row m is
 // X[m], or with row_index X[row_index[m]] (negative: zeros), with row_share times row_share[row_pair[m]].  `scratch`:
 // at least
 // fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
 FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_index, const float* row_share, const int* row_pair,
-                                 const void* W, const int* shifts, int groups, const int* tile_group, int tile, void* out, int o_dtype,
+                                 const void* W, int groups, const int* tile_group, int tile, void* out, int o_dtype,
                                  long long ldo, int M, int N, int K, int act, float limit, float slope, int plain_act, void* scratch,
                                  long long scratch_bytes, int* status, cudaStream_t stream) {
     const FbGate gate = {act, limit, slope};
-    if (const int rc = check_operands(X, lda, W, shifts, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
+    if (const int rc = check_operands(X, lda, W, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
     FB_REQUIRE(groups > 0 && tile_group, "gemm_mxfp4_grouped: no groups");
     FB_REQUIRE(tile >= 16 && tile <= 128 && tile % 16 == 0 && M % tile == 0 && M / tile < (1 << 24),
                "gemm_mxfp4_grouped: the rows must be whole tiles of 16 to 128, not tiles of %d", tile);
@@ -1011,7 +1009,7 @@ FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_in
     MxArgs a = {};
     a.kb = (K + MX_COLS - 1) / MX_COLS;
     a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
-    a.W = (const uint8_t*)W; a.w_group = (long)a.tiles_n * a.kb * MX_TILE_BYTES; a.shifts = shifts; a.out = out; a.ldo = (long)ldo;
+    a.W = (const uint8_t*)W; a.w_group = (long)a.tiles_n * a.kb * MX_TILE_BYTES; a.out = out; a.ldo = (long)ldo;
     a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, row_index, row_share, row_pair};
     a.o_bf16 = o_dtype == FB_BF16; a.M = M; a.N = N; a.K = K; a.tiles_m = 1; a.splits = a.max_segments = 1;
     a.gate = gate; a.plain_act = plain_act; a.status = status;

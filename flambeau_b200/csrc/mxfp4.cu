@@ -177,27 +177,11 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     }
 }
 
-// The two kernels that write the tiles let no kernel behind them in before they end: the product asks for its first weights ahead of
-// its wait for the kernel before it, and that kernel may have come in early itself.
-// shifts[g] = how far the scales of matrix g have to be lowered (one block a matrix; scales of 255 do not count).
-__global__ void __launch_bounds__(1024)
-shift_kernel(const uint8_t* __restrict__ scales, long per_group, int* __restrict__ shifts) {
-    fb_pdl_wait();
-    __shared__ float scratch[32];
-    const uint8_t* s = scales + (size_t)blockIdx.x * per_group;
-    int top = 0;
-    for (long i = threadIdx.x; i < per_group; i += 1024) {
-        const int v = s[i];
-        if (v != 255) top = max(top, v);
-    }
-    const float all = fb_block_max((float)top, scratch);
-    if (threadIdx.x == 0) shifts[blockIdx.x] = max(0, (int)all - MX_TOP_SCALE);
-}
-
-// A thread a row and block of 32 columns: its 16 bytes of codes in the tiles' order, its scale lowered by the matrix's shift.
+// The kernel that writes the tiles lets no kernel behind it in before it ends: the product asks for its first weights ahead of its
+// wait for the kernel before it, and that kernel may have come in early itself.
+// A thread a row and block of 32 columns: its 16 bytes of codes in the tiles' order, its scale.
 __global__ void __launch_bounds__(128)
-tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int N, int blocks, int tiles_k,
-             const int* __restrict__ shifts, uint8_t* __restrict__ tiles) {
+tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int N, int blocks, int tiles_k, uint8_t* __restrict__ tiles) {
     fb_pdl_wait();
     const int row = threadIdx.x, b = blockIdx.x, n = blockIdx.y * MX_ROWS + row, group = blockIdx.z;
     const size_t tile = ((size_t)group * gridDim.y + blockIdx.y) * tiles_k + b / 4;
@@ -213,13 +197,6 @@ tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scal
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[i] |= mx_place(in[i] >> (4 * j) & 15u, j);
         s = scales[at];
-        if (s != 255) {
-            s += MX_RAISE - shifts[group];
-            if (s < 0) {                 // 2^248 below the largest scale: nothing is left of it
-                s = 0;
-                w[0] = w[1] = w[2] = w[3] = 0;
-            }
-        }
     }
     reinterpret_cast<uint4*>(dst)[(b & 3) * MX_ROWS + row] = make_uint4(w[0], w[1], w[2], w[3]);
     dst[MX_CODE_BYTES + ((row & 31) * 4 + (row >> 5)) * 4 + (b & 3)] = (uint8_t)s;
@@ -358,15 +335,13 @@ FB_API long long fb_mxfp4_tile_bytes(int N, int K) {
     return (long long)((N + MX_ROWS - 1) / MX_ROWS) * ((K + MX_COLS - 1) / MX_COLS) * MX_TILE_BYTES;
 }
 
-// `groups` matrices [N, K] from rows (codes, scales as fb_quantize_mxfp4 writes them) into tiles, and shifts[groups] (int32).
-FB_API int fb_mxfp4_tiles(const void* codes, const void* scales, int groups, int N, int K, void* tiles, int* shifts,
-                          cudaStream_t stream) {
+// `groups` matrices [N, K] from rows (codes, scales as fb_quantize_mxfp4 writes them) into tiles.
+FB_API int fb_mxfp4_tiles(const void* codes, const void* scales, int groups, int N, int K, void* tiles, cudaStream_t stream) {
     FB_REQUIRE(groups > 0 && N > 0 && K > 0 && groups <= 65535 && N <= 65535 * MX_ROWS, "mxfp4_tiles: bad sizes");
     FB_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)tiles & 15) == 0, "mxfp4_tiles: operands must be 16-byte aligned");
     const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK, tiles_k = (K + MX_COLS - 1) / MX_COLS;
-    fb_launch(shift_kernel, dim3(groups), dim3(1024), 0, stream, (const uint8_t*)scales, (long)N * blocks, shifts);
     fb_launch(tiles_kernel, dim3(4 * tiles_k, (N + MX_ROWS - 1) / MX_ROWS, groups), dim3(128), 0, stream, (const uint8_t*)codes,
-              (const uint8_t*)scales, N, blocks, tiles_k, shifts, (uint8_t*)tiles);
+              (const uint8_t*)scales, N, blocks, tiles_k, (uint8_t*)tiles);
     return fb_check_launch("mxfp4_tiles");
 }
 

@@ -16,24 +16,17 @@ constexpr int MX_LAST_SCALE = 252;                                       // the 
 constexpr int MX_ROWS = 128, MX_COLS = 128;                              // a tile
 constexpr int MX_CODE_BYTES = MX_ROWS * MX_COLS / 2;
 constexpr int MX_TILE_BYTES = MX_CODE_BYTES + MX_ROWS * MX_COLS / MX_BLOCK;
-// A code becomes an e4m3 number (sign, four bits of exponent, three of mantissa) by putting its magnitude bits where they are the
-// end of the exponent and the first bit of the mantissa: the number times 2^-6, subnormal ones included.  The tiles' scales make
-// up for it; where that passes their largest, a matrix carries a shift that they are lowered by, and results are raised by.
-constexpr int MX_RAISE = 6, MX_TOP_SCALE = 254 - MX_RAISE;
 
-// Eight codes in a 32-bit word of a tile.  Columns 0..3: bits 7 (sign), 4, 3, 2 of its bytes, where they are wanted.  Columns 4..7: bits 5
-// (sign), 1 (the exponent's lower bit) of its bytes, two places away, and 0 (the upper one), 6 of the byte before (the mantissa's), four
-// places away in a word that turns: two rotations and two operations for the four.
+// tcgen05.mma takes such numbers (e2m1) from tensor memory in bytes, the code in bits 5 to 2, zeros around it.  Eight codes in a
+// 32-bit word of a tile: columns 0..3 where they are wanted, columns 4..7 in the bits between, four places further in a word that turns.
 __host__ __device__ __forceinline__ uint32_t mx_place(uint32_t code, int column) {
-    const uint32_t s = code >> 3, e1 = code >> 2 & 1u, e0 = code >> 1 & 1u, m = code & 1u;
-    const int byte = 8 * (column & 3);
-    if (column < 4) return (s << 7 | e1 << 4 | e0 << 3 | m << 2) << byte;
-    return (s << 5 | e0 << 1 | e1) << byte | m << ((byte + 30) & 31);
+    const int to = 8 * (column & 3) + (column < 4 ? 2 : 30) & 31;
+    return code << to | (to > 28 ? code >> (32 - to) : 0u);
 }
-// The e4m3 numbers of columns 0..3 and 4..7, packed.
+// The bytes of columns 0..3 and 4..7.
 __device__ __forceinline__ void mx_decode(uint32_t w, uint32_t& first, uint32_t& second) {
-    first = w & 0x9C9C9C9Cu;
-    second = (__funnelshift_l(w, w, 2) & 0x88888888u) | (__funnelshift_l(w, w, 4) & 0x14141414u);
+    first = w & 0x3C3C3C3Cu;
+    second = __funnelshift_l(w, w, 4) & 0x3C3C3C3Cu;
 }
 // 2^(S - 127) in float32.
 __device__ __forceinline__ float mx_scale_f32(uint32_t s) {

@@ -62,11 +62,11 @@ _SIGNATURES = {
     "fb_quantize_mxfp4": (I, [P, I, L, L, I, P, P, STREAM]),
     "fb_dequantize_mxfp4": (I, [P, P, L, I, P, I, L, STREAM]),
     "fb_mxfp4_tile_bytes": (L, [I, I]),
-    "fb_mxfp4_tiles": (I, [P, P, I, I, I, P, P, STREAM]),
+    "fb_mxfp4_tiles": (I, [P, P, I, I, I, P, STREAM]),
     # gemm_mxfp4.cu
     "fb_gemm_mxfp4_scratch_bytes": (L, [I, I, I, I, I, I]),
-    "fb_gemm_mxfp4": (I, [P, L, P, P, P, I, L, L, I, P, I, I, I, I, F, F, I, I, P, I, P, L, P, STREAM]),
-    "fb_gemm_mxfp4_grouped": (I, [P, L, P, P, P, P, P, I, P, I, P, I, L, I, I, I, I, F, F, I, P, L, P, STREAM]),
+    "fb_gemm_mxfp4": (I, [P, L, P, P, I, L, L, I, P, I, I, I, I, F, F, I, I, P, I, P, L, P, STREAM]),
+    "fb_gemm_mxfp4_grouped": (I, [P, L, P, P, P, P, I, P, I, P, I, L, I, I, I, I, F, F, I, P, L, P, STREAM]),
     # attention_simt.cu
     "fb_paged_attention_simt": (I, [P, L, P, L, I, P, P, I, I, P, I, P, I, P, P, I, I, I, I, I, I, I, F, F, P, P, P, L, I, L, P, STREAM]),
     # attention_tc.cu

@@ -1671,7 +1671,7 @@ class Mxfp4Weight(PackedWeight):
 
     `shape`, `dtype` (of the rows that it multiplies), `device`, `nbytes` are those of a weight tensor.  Every number of such a
     weight is a bfloat16 number: the products give what bfloat16 products with `dequantize_mxfp4`'s numbers give, up to the order of
-    their float32 sums.  (Numbers below 2^-127 of 3 times a matrix's largest scale, where that is above 2, count as zeros.)"""
+    their float32 sums."""
     dtype = torch.bfloat16
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, inputs: int):
@@ -1685,10 +1685,9 @@ class Mxfp4Weight(PackedWeight):
             raise KernelError("mxfp4 weight: no outputs")
         self.device = codes.device
         self.tiles = torch.empty(groups * lib().fb_mxfp4_tile_bytes(outputs, int(inputs)), dtype=torch.uint8, device=codes.device)
-        self.shifts = torch.empty(groups, dtype=torch.int32, device=codes.device)
-        self._tiles, self._shifts, self._scratch = self.tiles.data_ptr(), self.shifts.data_ptr(), {}
+        self._tiles, self._scratch = self.tiles.data_ptr(), {}
         check(lib().fb_mxfp4_tiles(codes.data_ptr(), scales.data_ptr(), groups, outputs, int(inputs), self.tiles.data_ptr(),
-                                   self.shifts.data_ptr(), _stream()), "mxfp4_tiles")
+                                   _stream()), "mxfp4_tiles")
 
     @classmethod
     def from_dense(cls, weight: torch.Tensor) -> "Mxfp4Weight":
@@ -1697,7 +1696,7 @@ class Mxfp4Weight(PackedWeight):
 
     @property
     def nbytes(self) -> int:
-        return self.tiles.numel() + 4 * self.shifts.numel()
+        return self.tiles.numel()
 
     def dim(self) -> int:
         return len(self.shape)
@@ -1729,7 +1728,7 @@ class Mxfp4Weight(PackedWeight):
         nbytes = self._scratch_bytes(M, counters.numel(), slabs is not None, 0)
         mark = ws.mark()
         try:
-            check(lib().fb_gemm_mxfp4(a.data_ptr(), a.stride(0), self._tiles, self._shifts, out.data_ptr(), _CODES[out.dtype], out.stride(0),
+            check(lib().fb_gemm_mxfp4(a.data_ptr(), a.stride(0), self._tiles, out.data_ptr(), _CODES[out.dtype], out.stride(0),
                                       slabs.stride(0) if slabs is not None else 0, slabs.shape[0] if slabs is not None else 0,
                                       _SPLITS_USED_REF, M, N, K, *gate, plain_act, accumulate, counters.data_ptr(), counters.numel(),
                                       ws.reserve(nbytes), nbytes, ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
@@ -1805,8 +1804,7 @@ class Mxfp4Weight(PackedWeight):
         nbytes = self._scratch_bytes(M, 0, False, int(tile))
         mark = ws.mark()
         try:
-            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), _ptr(row_index), _ptr(row_share), _ptr(row_pair), self._tiles,
-                                              self._shifts, self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(),
+            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), _ptr(row_index), _ptr(row_share), _ptr(row_pair), self._tiles, self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(),
                                               dtype_code(out), _rows(out), M, N, K, *gate_args,
                                               plain_activation_code(activation_name), ws.reserve(nbytes), nbytes,
                                               ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4_grouped", (M, N, K))
