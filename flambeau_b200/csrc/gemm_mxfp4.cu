@@ -854,22 +854,29 @@ template <int TOK, bool GROUPED, bool PAIR> int launch(const MxArgs& a, const CU
     return fb_check_launch("gemm_mxfp4");
 }
 
+// Whether the form of few rows takes the product (tile: the grouped form's row tile, 0: not grouped).  A CTA splits what it multiplies: that
+// spares a kernel that 8 rows spent 4 to 8 us in, behind the weights that the product had on their way by then, and one until the
+// first MMA (shares to slabs, 8 x 4,096 x 14,336, 24 stages a CTA: 17.3 us with that kernel, 11.9 without; 8 x 7,168 x 18,432, 55: 21.7 and
+// 18.2).  But its warps share the issue slots with the decoding: longer stretches are faster with the kernel (8 x 28,672 x 4,096 gated,
+// 64 stages: 14.9 us, 17.5), and so are 16 rows (15.1 us, 30.8) and products whose row tiles share a group's rows (65 us, 93).
+constexpr int FEW_STAGES = 60;
+bool few_rows(int M, int N, int K, int tile, bool slabs) {
+    if (tile || M > FEW_TOKENS) return false;
+    const long tiles_n = (N + MX_ROWS - 1) / MX_ROWS, kb = (K + MX_COLS - 1) / MX_COLS;
+    const long grid = slabs ? fb_sm_count() : cut_of((int)tiles_n, (int)kb, ANY, true).grid;
+    return tiles_n * kb <= FEW_STAGES * grid;
+}
+
 // (Token tiles are at most MORE_TILES more than the rows need; the grouped form has a place for every row tile.)
 long long scale_bytes_of(int M, int kb, int tile) {
     const long long tiles = tile ? M / tile : (M + WIDE_TOKENS - 1) / WIDE_TOKENS + MORE_TILES;
     return kb * tiles * ATOM * (tile == 16 || (!tile && M <= SIDE_BY_SIDE) ? 1 : 2);
 }
 
-// Whether the form of few rows takes the product (tile: the grouped form's row tile, 0: not grouped).  A CTA splits what it multiplies: that
-// spares a kernel that 8 rows spent 4 to 8 us in, behind the weights that the product had on their way by then, and one until the
-// first MMA (8 x 4,096 x 14,336 17.3 us with that kernel, FEWUS without).  With 16 rows the splitting warps were too slow (16 x 28,672 x
-// 4,096 gated 30.8 us, with the kernel 23.9), and so they were where many row tiles share the rows of a group (93 us, 65).
-bool few_rows(int M, int tile) { return tile == 0 && M <= FEW_TOKENS; }
-
 // The rows' parts and scales in `scratch`, their map, the output's map.
 int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, int box_rows, cudaStream_t stream) {
     const bool grouped = a.tile_group != nullptr;
-    if (few_rows(a.M, a.tile)) return 0;                 // (the product splits them itself, and stores directly)
+    if (few_rows(a.M, a.N, a.K, a.tile, a.slabs > 0)) return 0;                 // (the product splits them itself, and stores directly)
     const long Kp = (long)a.kb * MX_COLS, parts = 2L * a.M * Kp;
     a.x_scales = (const uint8_t*)scratch + parts;
     a.scale_bytes = atoms_of(a.bn) * ATOM;
@@ -905,8 +912,8 @@ int check_operands(const void* X, long long lda, const void* W, const void* out,
 }  // namespace
 
 // What the rows' parts and their scales take, a multiple of 256 bytes (tile: the grouped form's row tile, 0: not grouped).
-static long long rows_bytes(int M, int K, int tile) {
-    if (M <= 0 || K <= 0 || few_rows(M, tile)) return 0;
+static long long rows_bytes(int M, int N, int K, int tile, bool slabs) {
+    if (M <= 0 || N <= 0 || K <= 0 || few_rows(M, N, K, tile, slabs)) return 0;
     const long long kb = (K + MX_COLS - 1) / MX_COLS;
     return (2LL * M * kb * MX_COLS + scale_bytes_of(M, (int)kb, tile) + 255) / 256 * 256;
 }
@@ -926,7 +933,7 @@ static long long share_floats(int M, int N, int K, int n_counters) {
 // Bytes of `scratch` that the products below want for M rows, with `n_counters` counters.  slabs: shares of K go to slabs; tile: the
 // grouped form's row tile (0: not grouped).
 FB_API long long fb_gemm_mxfp4_scratch_bytes(int M, int N, int K, int n_counters, int slabs, int tile) {
-    return rows_bytes(M, K, tile) + (slabs || tile ? 0 : 4 * share_floats(M, N, K, n_counters));
+    return rows_bytes(M, N, K, tile, slabs != 0) + (slabs || tile ? 0 : 4 * share_floats(M, N, K, n_counters));
 }
 
 // X [M,K] bfloat16, W one matrix in tiles (fb_mxfp4_tiles).  `act` (an FbAct code with its constants): W stacks gate
@@ -953,7 +960,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
     a.M = M; a.N = N; a.K = K; a.kb = (K + MX_COLS - 1) / MX_COLS; a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
     const bool slabs = slab_stride > 0;
-    const long long need = fb_gemm_mxfp4_scratch_bytes(M, N, K, n_counters, slabs, 0), rows = rows_bytes(M, K, 0);
+    const long long need = fb_gemm_mxfp4_scratch_bytes(M, N, K, n_counters, slabs, 0), rows = rows_bytes(M, N, K, 0, slabs);
     FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= need && (slabs || (counters && n_counters > 0)),
                "gemm_mxfp4: %lld bytes of scratch wanted, and counters", need);
     a.partials = need > rows ? (float*)((uint8_t*)scratch + rows) : nullptr;
@@ -969,7 +976,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
             if (splits_used) *splits_used = cut.segments;
         }
         if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
-        return few_rows(M, 0) ? launch<FEW_TOKENS, false, false>(a, mx, mo, cut.grid, stream) : launch<32, false, false>(a, mx, mo, cut.grid, stream);
+        return few_rows(M, N, K, 0, slabs) ? launch<FEW_TOKENS, false, false>(a, mx, mo, cut.grid, stream) : launch<32, false, false>(a, mx, mo, cut.grid, stream);
     }
     const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, SHARE_FLOATS,
                                 n_counters, slabs);
@@ -1004,7 +1011,7 @@ FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_in
     FB_REQUIRE(tile >= 16 && tile <= 128 && tile % 16 == 0 && M % tile == 0 && M / tile < (1 << 24),
                "gemm_mxfp4_grouped: the rows must be whole tiles of 16 to 128, not tiles of %d", tile);
     FB_REQUIRE(!row_share || (row_index && row_pair), "gemm_mxfp4_grouped: shares need the rows' index and pairs");
-    FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= rows_bytes(M, K, tile), "gemm_mxfp4_grouped: scratch missing");
+    FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= rows_bytes(M, N, K, tile, false), "gemm_mxfp4_grouped: scratch missing");
     if (M == 0) return 0;
     MxArgs a = {};
     a.kb = (K + MX_COLS - 1) / MX_COLS;
