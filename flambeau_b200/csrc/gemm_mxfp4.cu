@@ -1,15 +1,14 @@
 // out[M,N] = X[M,K] * W[N,K]^T with X in bfloat16 and W in four bits (mxfp4.cuh) on the 5th-generation tensor cores.
 //
-// tcgen05.mma.kind::mxf8f6f4 multiplies 8-bit numbers whose blocks of 32 along K carry power-of-two scales, and sums in float32.
-// A four-bit weight is such a number as it is.  A row's bfloat16 numbers become two e4m3 numbers each, the second what the first left
-// (mxfp4.cuh: what is lost is below 2^-22 of a block's largest number, far below what bfloat16 itself has rounded), so the
+// tcgen05.mma.kind::mxf8f6f4 multiplies numbers of up to 8 bits whose blocks of 32 along K carry power-of-two scales, and sums in
+// float32.  A four-bit weight is such a number as it is.  A row's bfloat16 numbers become two e4m3 numbers each, the second what the
+// first left (mxfp4.cuh: what is lost is at most 2^-22 of a block's largest number, far below what bfloat16 itself has rounded), so the
 // product is that of bfloat16 rows with the weights' numbers, summed in float32; only infinities among the rows end as NaN.
 //
 // Why this instruction, on one SM, for 128 features x 128 of K (a tile of 8,704 bytes, which HBM brings every 370 cycles): kind::f16
 // takes 8 instructions of 70 cycles at least, whatever the number of tokens up to 128, and its weights have to be decoded to
 // bfloat16 (19 instructions for eight: shifts, masks, multiplications); this kind takes 4 of 35 cycles up to 32 tokens (N = 64: both
-// parts side by side), and decoding is moving bits (7 instructions for eight), since the scales go to the tensor core as
-// they are.
+// parts side by side), and decoding is moving bits (3 instructions for eight), since the scales go to the tensor core as they are.
 //
 // Layout.  A CTA owns 128 output features x a tile of tokens ("swap-AB": the weight is the 128-row operand, the tokens are N).  A stage
 // is 128 of K: one bulk copy brings a weight tile as it lies in memory, groups of four warps take the stages in turn and decode, a
@@ -17,13 +16,18 @@
 // once for all CTAs by a kernel of their own, come by TMA (K-major, 128-byte swizzle), their scales by tcgen05.cp.  Up to 64 tokens the
 // two parts are N's two halves, which the epilogue adds; with more they are two instructions into one accumulator.
 //
-// The narrow form (up to 32 tokens: decoding, experts' few rows): the tiles of all row tiles form one line that the CTAs cut into
-// equal stretches.  The wide form sends its output through shared memory.  Shares of K go to slabs that the next kernel adds, or
-// meet in scratch, where the CTA that arrives last (a counter a row tile, no waiting) adds them in order.  Grouped (routed
-// experts): row tiles of one group each; a unit is a run of neighbouring ones.
+// Forms.  Few (up to 8 tokens, the CTA splits the rows itself) and narrow (up to 32): the tiles of all row tiles form one line that the
+// CTAs cut into equal stretches.  Wide: token tiles of up to 64 or 128, the output through shared memory.  Shares of K go to slabs
+// that the next kernel adds, or meet in scratch, where the CTA that arrives last (a counter a row tile, no waiting) adds them in
+// order.  Grouped (routed experts): row tiles of one group each; a unit is a run of neighbouring ones.
 //
-// full[s]: a stage's rows (by bytes) and its decoded weights (by arrivals) are there; done[s]: its MMAs are.  Two accumulators, so that the epilogue of one
-// unit overlaps the products of the next.  Every mbarrier wait is bounded as in gemm_tc.cu.
+// full[s]: a stage's rows (by bytes) and its decoded weights (by arrivals) are there; done[s]: its MMAs are.  Two accumulators, so that
+// the epilogue of one unit overlaps the products of the next.  Every mbarrier wait is bounded as in gemm_tc.cu.
+//
+// What bounds it.  A few rows: instructions.  Decoding a stage takes 150 of a scheduler's slots of the 370 cycles that HBM has it
+// under way, its barriers and the thread that issues MMAs another 100; before that a launch and the way from the first weights to the
+// first MMA, about 4 us (8 x 28,672 x 4,096: 14.9 us in a graph, 64% of HBM's rate).  Many rows: the MMAs, 512 cycles for 128 x 128 x
+// 128 in two parts, at the clock that the power limit leaves (2,048 x 28,672 x 4,096: 355 us, 1,350 TFLOP/s at 1.6 GHz).
 #include "group_units.cuh"
 #include "mxfp4.cuh"
 #include "tensor_map.cuh"
@@ -50,11 +54,11 @@ constexpr int ATOM = 512;                         // scales of 128 rows for a st
 constexpr int TMEM = 512, SMEM = 227 * 1024;
 
 // TOK: most tokens of a tile.  R stages of rows and decoded weights, GROUPS of four decoding warps: a stage is 1,500 cycles on its way
-// from the first look at its weights to the end of its MMAs, of which a group works on it for half, so that it takes
-// four groups and eight stages to keep up with memory where the MMAs are short.
+// from the first look at its weights to the end of its MMAs, of which a group works on it for half, so that it takes four groups
+// and eight stages to keep up with memory where the MMAs are short.
 // PAIR: a unit is two neighbouring feature tiles, which share the stages of rows; their accumulators are the two that are otherwise
-// those of successive units.  Many tokens want it: a CTA's rows come from L2, whose bandwidth was the bound (82 bytes a cycle and SM
-// for 128 x 128, like this 49).
+// those of successive units, and sixteen warps store them.  It halves the reading of rows, and one round of pairs can replace two
+// of single tiles (128 x 28,672 x 4,096: 30 us, 34 single); see plan_wide.
 template <int TOK, bool PAIR> struct Form {
     static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow forms cut the line of tiles, and store directly)
     static constexpr bool FEW = TOK <= FEW_TOKENS;
@@ -334,9 +338,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         return w;
     };
-    // CTAs of neighbouring row tiles want the same rows: each begins at another place along K, or they would all ask for the same few
-    // lines of L2 at once.
-    auto first_tile = [&](const Unit& w) { return GROUPED ? w.nt / TILES % w.n_kb : 0; };
+    // CTAs of neighbouring row tiles of a group want the same rows: each begins at another place along K, or they would all ask for the same
+    // few lines of L2 at once (8 tokens on 6 of 64 experts, 3,584 x 4,096: 68 us, like this 64).
+    auto first_tile = [&](const Unit& w) { return GROUPED ? w.nt % w.n_kb : 0; };
     auto after = [&](long item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
 
     if (warp == 0 || (F::PRODUCERS == 2 && warp == 3)) {
@@ -400,8 +404,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     } else if (warp == 1) {
         // ---------------- MMA ----------------
         // (What an instruction's operands are made of is brought to uniform registers first.  Where a stage's place in the ring is counted
-        // out, that takes 300 cycles a stage of four instructions; with four places as constants it is done once, and a stage
-        // takes 140 with its wait and commit, 57 to 260 of them MMAs.)
+        // out, that takes 300 cycles a stage of four instructions; with three or four places as constants it is done once, and a
+        // stage takes 140 with its wait and commit, 57 to 260 of them MMAs.)
         if (elect_one()) {
             int s = 0, j = 0;
             uint32_t phase = 0;
@@ -555,7 +559,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         if (!ok) *bail = 1;
     } else if (warp >= EPI_WARP && warp < F::SPLIT_WARP) {
-        // ---------------- epilogue: lanes are features, the two groups of four warps take 16 tokens in turn ----------------
+        // ---------------- epilogue: lanes are features, the groups of four warps take 16 tokens in turn ----------------
         fb_pdl_wait();
         const int quarter = warp & 3, half = (warp - EPI_WARP) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 32 * EPI_WARP;
         const bool leader = quarter == 0 && lane == 0;
@@ -774,9 +778,9 @@ int segments_of(long tiles_n, long kb, long grid) {           // the most stretc
     return (int)most;
 }
 // CTAs, one an SM, each with a few tiles at least, and the most stretches that they cut a row tile into: as many CTAs as leave no
-// more than `limit`.
-// Where shares have to meet (`join`), row tiles stay whole if the longest stretch and the meeting take longer.  In cycles: STAGE for
-// a tile of an SM, JOIN for the partial sums' way through L2 and back.
+// more than `limit`.  Where shares have to meet (`join`), row tiles stay whole if they come out even and the longest stretch and the
+// meeting take longer (16 x 28,672 x 4,096 gated: 23.0 us in 148 stretches, 16.7 in 112 of two whole tiles).  In cycles: STAGE for a
+// tile of an SM, JOIN for the partial sums' way through L2 and back.
 constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 6000;
 struct Cut { int grid, segments; };
 Cut cut_of(int tiles_n, int kb, int limit, bool join) {
@@ -810,8 +814,8 @@ constexpr double L2_BYTES = 62.0;                 // what an SM gets from L2 a c
 // other: 96 CTAs 12.9 us, 144 of fewer tokens 17.2; each by itself about 19.5).  A pair's epilogue overlaps little of the next
 // one's products (100 cycles a token for both tiles), of a single tile's only the last one's shows.  Shares of K cost a copy of the output,
 // written and read, and where they meet the adding, which nothing overlaps (67 x 6,144 x 5,120: three shares 21 us, whole 15.6 with
-// the same tiles).  Where it decides for or against pairs: 301 x 28,672 x 4,096 68 us single, 80 in pairs; 2,048 x 4,096 x 14,336
-// 225 single, 200 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.
+// the same tiles).  Where it decides for or against pairs: 301 x 28,672 x 4,096 68 us single, 80 in pairs; 128 x 28,672 x 4,096
+// 34 single, 30 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.
 Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
     const long sms = fb_sm_count(), tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     Plan best = {WIDE_TOKENS, 1, false};
@@ -867,7 +871,7 @@ bool few_rows(int M, int N, int K, int tile, bool slabs) {
     return tiles_n * kb <= FEW_STAGES * grid;
 }
 
-// (Token tiles are at most MORE_TILES more than the rows need; the grouped form has a place for every row tile.)
+// Bytes of the rows' scales.  (Token tiles are at most MORE_TILES more than the rows need; the grouped form has a place for every row tile.)
 long long scale_bytes_of(int M, int kb, int tile) {
     const long long tiles = tile ? M / tile : (M + WIDE_TOKENS - 1) / WIDE_TOKENS + MORE_TILES;
     return kb * tiles * ATOM * (tile == 16 || (!tile && M <= SIDE_BY_SIDE) ? 1 : 2);
@@ -998,9 +1002,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
 
 // The grouped form: W holds `groups` matrices [N, K] in tiles; the M rows of `out` come in tiles of `tile` (a
 // multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are).  Row m is
-// X[m], or with row_index X[row_index[m]] (negative: zeros), with row_share times row_share[row_pair[m]].  `scratch`:
-// at least
-// fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
+// X[m], or with row_index X[row_index[m]] (negative: zeros), with row_share times row_share[row_pair[m]].  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
 FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_index, const float* row_share, const int* row_pair,
                                  const void* W, int groups, const int* tile_group, int tile, void* out, int o_dtype,
                                  long long ldo, int M, int N, int K, int act, float limit, float slope, int plain_act, void* scratch,

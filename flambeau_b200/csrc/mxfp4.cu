@@ -55,7 +55,7 @@ __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& sca
 }
 
 // Rows of whole blocks, one behind the other on 16-byte borders: UNROLL quarters a thread, all fetched before the first is used.
-// (28,672 x 4,096 bfloat16 with the form below: 94 us, of which 45 are memory's; like this QUANTUS.)
+// (28,672 x 4,096 bfloat16 with the form below: 94 us, of which 45 are memory's; like this 49.)
 constexpr int UNROLL = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -203,7 +203,8 @@ tiles_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scal
 }
 
 // A thread a block of 32 numbers, SPLIT_ROWS rows (of one tile) a group of blocks: parts[p][m][k] (bytes, rows of Kp, a multiple of 128,
-// zeros behind K), their scales as `layout` says.
+// zeros behind K), their scales as `layout` says.  (14,336 x 4,096 numbers, 117 MB in and out each: 45 us, memory's 36; a thread eight
+// numbers, where what is not conversion outweighs it, took 61.)
 constexpr int SPLIT_ROWS = 4;
 template <bool GROUPED>
 __global__ void __launch_bounds__(256)

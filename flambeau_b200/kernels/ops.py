@@ -1723,12 +1723,14 @@ class Mxfp4Weight(PackedWeight):
     def _product(self, a, out, ctx, columns: int, what: str, gate=(0, 0.0, 0.0), plain_act: int = 0, accumulate: bool = False,
                  slabs=None) -> int:
         M, N, K = self._matrix(a, out, columns, what)
-        ws = ctx.ws
+        ws = getattr(ctx, "ws", None)
+        if ws is None:
+            raise KernelError(f"{what}: four-bit weights need the step's scratch (ctx)")
         counters = ws.counters
         nbytes = self._scratch_bytes(M, counters.numel(), slabs is not None, 0)
         mark = ws.mark()
         try:
-            check(lib().fb_gemm_mxfp4(a.data_ptr(), a.stride(0), self._tiles, out.data_ptr(), _CODES[out.dtype], out.stride(0),
+            check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self._tiles, out.data_ptr(), _CODES[out.dtype], out.stride(0),
                                       slabs.stride(0) if slabs is not None else 0, slabs.shape[0] if slabs is not None else 0,
                                       _SPLITS_USED_REF, M, N, K, *gate, plain_act, accumulate, counters.data_ptr(), counters.numel(),
                                       ws.reserve(nbytes), nbytes, ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
