@@ -93,7 +93,7 @@ struct MxArgs {
     int o_bf16, accumulate, boxed, slabs;                 // boxed: tokens of a box, 0: stored directly
     float* partials; int* counters; int max_segments;
     int M, N, K, kb, bn, tiles_m, tiles_n, units_n, splits;      // units_n: feature tiles, or pairs of them
-    long items;                                           // narrow, not grouped: tiles_n * kb; wide, not grouped: units
+    uint32_t items;                                       // narrow, not grouped: tiles_n * kb; wide, not grouped: units
     const int* tile_group; int tile, n_tiles;
     FbGate gate; int plain_act;
     int* status;
@@ -290,7 +290,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // The CTA's part of the work: items first .. last of the line.  Narrow, not grouped: an item is a tile along K of a row tile; else a
     // unit, and the CTAs take turns.
     constexpr bool LINE = !WIDE && !GROUPED;
-    long first = blockIdx.x, last = a.items;
+    // (32 bits hold items x CTAs: a matrix of 2^38 weights fills the memory.  Twenty warps divide for every unit.)
+    uint32_t first = blockIdx.x, last = a.items;
     if constexpr (GROUPED) {
         if (warp == EPI_WARP) {
             fb_pdl_wait();                       // which weights a tile wants is the work of the kernels before this one
@@ -298,41 +299,41 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             if (lane == 0) *unit_count = found;
         }
         __syncthreads();
-        last = (long)*unit_count * a.units_n;
+        last = (uint32_t)*unit_count * a.units_n;
     } else if constexpr (LINE) {
         first = blockIdx.x * a.items / gridDim.x;
         last = (blockIdx.x + 1) * a.items / gridDim.x;
     }
     GroupWalk walk = {0, 0u};
-    auto unit_at = [&](long item) {              // (asked for ascending items only)
+    auto unit_at = [&](uint32_t item) {              // (asked for ascending items only)
         Unit w;
         if constexpr (GROUPED) {                 // feature tiles vary fastest: the CTAs that run together share few units' rows
-            const int i = (int)(item / a.units_n);
+            const int i = (int)(item / (uint32_t)a.units_n);
             const uint32_t entry = group_unit<LIST>(a.tile_group, a.n_tiles, most, list, i, walk);
             const int t = (int)(entry & 0xffffffu);
             w.m0 = t * a.tile;
             w.n_tok = (int)(entry >> 24) * a.tile;
             w.group = a.tile_group[t];
-            w.nt = TILES * (int)(item - (long)i * a.units_n);
+            w.nt = TILES * ((int)item - i * a.units_n);
             w.kb0 = 0; w.n_kb = a.kb; w.share = 0; w.shares = 1; w.id = 0;
         } else if constexpr (WIDE) {             // token tiles vary fastest: the CTAs that run together share weight tiles
-            const long units = (long)a.tiles_m * a.units_n;
+            const uint32_t units = (uint32_t)a.tiles_m * a.units_n;
             w.share = (int)(item / units);
             w.shares = a.splits;
-            const int u = (int)(item - w.share * units), mt = u % a.tiles_m;
-            w.m0 = mt * a.bn;
-            w.nt = TILES * (u / a.tiles_m);
-            w.id = mt * a.tiles_n + w.nt;
+            const uint32_t u = item - w.share * units, mt = u % (uint32_t)a.tiles_m;
+            w.m0 = (int)mt * a.bn;
+            w.nt = TILES * (int)(u / (uint32_t)a.tiles_m);
+            w.id = (int)mt * a.tiles_n + w.nt;
             w.n_tok = a.bn;
             w.group = 0;
-            w.kb0 = (int)((long)w.share * a.kb / a.splits);
-            w.n_kb = (int)((long)(w.share + 1) * a.kb / a.splits) - w.kb0;
+            w.kb0 = (int)((uint32_t)(w.share * a.kb) / (uint32_t)a.splits);
+            w.n_kb = (int)((uint32_t)((w.share + 1) * a.kb) / (uint32_t)a.splits) - w.kb0;
         } else {
-            w.nt = (int)(item / a.kb);
-            w.kb0 = (int)(item - (long)w.nt * a.kb);
-            w.n_kb = (int)(last - item < a.kb - w.kb0 ? last - item : a.kb - w.kb0);
+            w.nt = (int)(item / (uint32_t)a.kb);
+            w.kb0 = (int)item - w.nt * a.kb;
+            w.n_kb = min((int)(last - item), a.kb - w.kb0);
             w.m0 = 0; w.n_tok = a.bn; w.group = 0; w.id = w.nt;
-            const long from = (long)w.nt * a.kb, begin = ((from + 1) * gridDim.x - 1) / a.items;
+            const uint32_t from = (uint32_t)(w.nt * a.kb), begin = ((from + 1) * gridDim.x - 1) / a.items;
             w.share = (int)(blockIdx.x - begin);
             w.shares = (int)(((from + a.kb) * gridDim.x - 1) / a.items - begin) + 1;
         }
@@ -341,7 +342,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // CTAs of neighbouring row tiles of a group want the same rows: each begins at another place along K, or they would all ask for the same
     // few lines of L2 at once (8 tokens on 6 of 64 experts, 3,584 x 4,096: 68 us, like this 64).
     auto first_tile = [&](const Unit& w) { return GROUPED ? w.nt % w.n_kb : 0; };
-    auto after = [&](long item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
+    auto after = [&](uint32_t item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
 
     if (warp == 0 || (F::PRODUCERS == 2 && warp == 3)) {
         // ---------------- weights: no other kernel writes them, so they are requested at once ----------------
@@ -349,7 +350,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             const int turn = warp == 0 ? 0 : 1;
             int s = turn, i = turn;                  // i: the thread's first tile of the unit
             uint32_t phase = 1;
-            for (long u = first; u < last && !bailed();) {
+            for (uint32_t u = first; u < last && !bailed();) {
                 const Unit w = unit_at(u);
                 const uint8_t* src = a.W + (size_t)w.group * a.w_group + ((size_t)w.nt * a.kb + w.kb0) * MX_TILE_BYTES;
                 // (a pair's second tile that is none of the matrix is its first one again: nobody stores what comes of it)
@@ -377,7 +378,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             fb_pdl_wait();
             int s = 0;
             uint32_t phase = 1;
-            for (long u = first; u < last && !bailed();) {
+            for (uint32_t u = first; u < last && !bailed();) {
                 const Unit w = unit_at(u);
                 const int boxes = GROUPED ? w.n_tok / a.tile : 1, box = GROUPED ? a.tile : a.bn;
                 int k = first_tile(w);
@@ -412,7 +413,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             bool ok = true;
             const uint32_t x_base = smem_u32(smem), full_base = smem_u32(full), done_base = smem_u32(done);
             const uint64_t desc = umma_desc(x_base), desc_scales = scales_desc(x_base + TOK * 256);
-            for (long u = first; u < last && ok && !bailed(); ++j) {
+            for (uint32_t u = first; u < last && ok && !bailed(); ++j) {
                 const Unit w = unit_at(u);
                 const bool both = w.n_tok <= SIDE_BY_SIDE;               // both parts in one operand
                 const int b = PAIR ? 0 : j & 1;
@@ -510,7 +511,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         uint32_t w_phase = 0, r_phase = 0, it = 0;       // it: stages ahead of the unit, modulo TURNS
         int round = 0;
         bool ok = true;
-        for (long u = first; u < last && ok;) {                 // (not `bailed`, which the four warps might see at different times)
+        for (uint32_t u = first; u < last && ok;) {                 // (not `bailed`, which the four warps might see at different times)
             const Unit w = unit_at(u);
             int i = turn - (int)it;                                      // the group's first stage of the unit
             if (i < 0) i += TURNS;
@@ -568,9 +569,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         const uint32_t box_last = box_first + (OUT_BUFFERS - 1) * OUT_BYTES;
         uint32_t box_at = box_first;
         int j = 0;
-        for (long u = first; u < last; ++j) {
+        for (uint32_t u = first; u < last; ++j) {
             Unit w = unit_at(u);
-            const long following = after(u, w);
+            const uint32_t following = after(u, w);
             bool stop = false;
 #pragma unroll 1
             for (int h = 0; h < TILES; ++h, ++w.nt, ++w.id) {
@@ -720,7 +721,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         int s = turn;
         uint32_t phase = 1, it = 0;
         bool ok = true;
-        for (long u = first; u < last && ok;) {
+        for (uint32_t u = first; u < last && ok;) {
             const Unit w = unit_at(u);
             uint4 raw[4];
             auto load = [&](int i) {                                     // what the lane splits of the unit's i-th stage
@@ -906,6 +907,7 @@ int check_operands(const void* X, long long lda, const void* W, const void* out,
     FB_REQUIRE(!gate.act || (fb_gate_known(gate) && N % 2 == 0 && !plain_act),
                "gemm_mxfp4: a gate needs a known activation, an even number of stacked rows and no plain activation beside it");
     FB_REQUIRE(fb_plain_act_known(plain_act), "gemm_mxfp4: unknown activation code %d", plain_act);
+    FB_REQUIRE((long)((N + MX_ROWS - 1) / MX_ROWS) * ((K + MX_COLS - 1) / MX_COLS) < (1L << 24), "gemm_mxfp4: too many weights, %d x %d", N, K);
     FB_REQUIRE(lda >= K && ldo >= (gate.act ? N / 2 : N), "gemm_mxfp4: a row stride is shorter than its row");
     FB_REQUIRE(((uintptr_t)X & 1) == 0 && W && ((uintptr_t)W & 15) == 0 && status,
                "gemm_mxfp4: unaligned rows or weights, or no status word");
@@ -973,7 +975,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
     if (M <= NARROW_TOKENS) {
         const Cut cut = cut_of(a.tiles_n, a.kb, slabs ? max_slabs : join ? ANY : 1, !slabs);
         a.bn = narrow_tokens(M);
-        a.tiles_m = 1; a.splits = 1; a.items = (long)a.tiles_n * a.kb;
+        a.tiles_m = 1; a.splits = 1; a.items = (uint32_t)a.tiles_n * a.kb;
         a.max_segments = cut.segments;
         if (slabs) {
             a.slabs = cut.segments;
@@ -992,10 +994,11 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
         a.slabs = plan.splits;
         if (splits_used) *splits_used = plan.splits;
     }
-    a.items = (long)a.tiles_m * a.units_n * a.splits;
-    if (a.items > 2000000000L) return fb_fail(-1, "gemm_mxfp4: too many tiles (M=%d N=%d)", M, N);
+    const long items = (long)a.tiles_m * a.units_n * a.splits;
+    a.items = (uint32_t)items;
+    if (items > 2000000000L) return fb_fail(-1, "gemm_mxfp4: too many tiles (M=%d N=%d)", M, N);
     if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
-    const long grid = a.items < fb_sm_count() ? a.items : fb_sm_count();
+    const long grid = items < fb_sm_count() ? items : fb_sm_count();
     if (plan.pair) return launch<128, false, true>(a, mx, mo, grid, stream);
     return a.bn <= 64 ? launch<64, false, false>(a, mx, mo, grid, stream) : launch<128, false, false>(a, mx, mo, grid, stream);
 }
