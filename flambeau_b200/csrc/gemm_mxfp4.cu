@@ -63,7 +63,8 @@ template <int TOK, bool PAIR> struct Form {
     static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow forms cut the line of tiles, and store directly)
     static constexpr bool FEW = TOK <= FEW_TOKENS;
     static constexpr int TILES = PAIR ? 2 : 1;
-    static constexpr int R = TOK <= NARROW_TOKENS ? 8 : TOK <= SIDE_BY_SIDE ? 6 : PAIR ? 3 : 4;
+    static constexpr int KT = WIDE ? 1 : 2;                              // tiles along K of a stage
+    static constexpr int R = TOK <= NARROW_TOKENS ? 4 : TOK <= SIDE_BY_SIDE ? 6 : PAIR ? 3 : 4;
     static constexpr int GROUPS = FEW ? 3 : TOK <= NARROW_TOKENS ? 4 : PAIR ? 2 : 3;
     static constexpr int EPI_GROUPS = FEW ? 1 : PAIR ? 4 : 2, EPI = 128 * EPI_GROUPS;   // groups of four warps, threads of the epilogue
     static constexpr int TURNS = GROUPS / TILES;                         // groups that take a feature tile's stages in turn
@@ -71,15 +72,19 @@ template <int TOK, bool PAIR> struct Form {
     static constexpr int ATOMS = TOK <= SIDE_BY_SIDE ? 1 : 2 * ((TOK + 127) / 128);
     static constexpr int ACC_COLS = TOK <= SIDE_BY_SIDE ? 2 * TOK : TOK;
     static constexpr int W_COLS = A_COLS + SFA_COLS;
-    static constexpr int RING_COLS = (TILES * W_COLS + 4 * ATOMS + 7) / 8 * 8;         // [weights | their scales] a tile, the rows' scales
-    static constexpr int STAGE_BYTES = (TOK * 256 + ATOMS * ATOM + 1023) / 1024 * 1024;
+    static constexpr int TILE_COLS = (TILES * W_COLS + 4 * ATOMS + 7) / 8 * 8;         // [weights | their scales] a feature tile, the rows' scales
+    static constexpr int TILE_BYTES = (TOK * 256 + ATOMS * ATOM + 1023) / 1024 * 1024; // the rows' parts, their scales
+    static constexpr int RING_COLS = KT * TILE_COLS, STAGE_BYTES = KT * TILE_BYTES;
     static constexpr int OUT = WIDE ? EPI_GROUPS * OUT_BUFFERS * OUT_BYTES : 0;
     static constexpr int RING = SMEM - 1024 - CONTROL - OUT;             // for the rings of stages
     static constexpr int FIT = (RING - R * STAGE_BYTES) / MX_TILE_BYTES;
     static constexpr int PRODUCERS = WIDE ? 1 : 2;                       // threads that ask for weights, each for places of its own
     static constexpr int WS = (FIT < MAX_W ? FIT : MAX_W) / PRODUCERS * PRODUCERS;
+    static constexpr int ARRIVALS = 4 * TILES + (FEW ? KT : 1);          // at full[s]: of the decoding warps, and of who brings the rows
     static_assert(2 * ACC_COLS + R * RING_COLS <= TMEM, "tensor memory");
-    static_assert(TURNS <= R && WS >= GROUPS + TILES * R, "a wait names a phase by its parity: see the decoding warps");
+    static_assert(TURNS <= R && WS % KT == 0 && WS >= KT * (GROUPS + TILES * R) && (!FEW || SPLITTERS / KT <= R),
+                  "a wait names a phase by its parity: see the decoding warps");
+    static_assert(PRODUCERS == 1 || KT == 2, "each has places of its own");
 };
 
 // Atoms of scales that the rows of a tile have: of both parts side by side, or of either part.
@@ -248,7 +253,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                   const __grid_constant__ MxArgs a) {
     using F = Form<TOK, PAIR>;
     constexpr bool WIDE = F::WIDE;
-    constexpr int WS = F::WS, R = F::R, G = F::GROUPS, EPI = F::EPI, EPI_WARP = F::EPI_WARP, TILES = F::TILES;
+    constexpr int WS = F::WS, R = F::R, G = F::GROUPS, KT = F::KT, EPI = F::EPI, EPI_WARP = F::EPI_WARP, TILES = F::TILES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* w_base = smem + R * F::STAGE_BYTES;                         // [stages of rows | weight stages | output boxes | control]
@@ -271,7 +276,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     if (threadIdx.x == 0) {
         for (int s = 0; s < MAX_W; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4); }
         for (int s = 0; s < R; ++s) {
-            mbar_init(smem_u32(&full[s]), 4 * TILES + 1);
+            mbar_init(smem_u32(&full[s]), F::ARRIVALS);
             mbar_init(smem_u32(&done[s]), 1);
         }
         for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&acc_full[s]), 1); mbar_init(smem_u32(&acc_empty[s]), EPI); }
@@ -342,6 +347,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // CTAs of neighbouring row tiles of a group want the same rows: each begins at another place along K, or they would all ask for the same
     // few lines of L2 at once (8 tokens on 6 of 64 experts, 3,584 x 4,096: 68 us, like this 64).
     auto first_tile = [&](const Unit& w) { return GROUPED ? w.nt % w.n_kb : 0; };
+    auto stages_of = [&](const Unit& w) { return (w.n_kb + KT - 1) / KT; };
     auto after = [&](uint32_t item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
 
     if (warp == 0 || (F::PRODUCERS == 2 && warp == 3)) {
@@ -355,12 +361,13 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 const uint8_t* src = a.W + (size_t)w.group * a.w_group + ((size_t)w.nt * a.kb + w.kb0) * MX_TILE_BYTES;
                 // (a pair's second tile that is none of the matrix is its first one again: nobody stores what comes of it)
                 const size_t next = w.nt + 1 < a.tiles_n ? (size_t)a.kb * MX_TILE_BYTES : 0;
-                const int begin = first_tile(w), tiles = TILES * w.n_kb;
+                const int begin = first_tile(w), tiles = TILES * stages_of(w) * KT;
                 bool ok = true;
                 for (; i < tiles; i += F::PRODUCERS) {
                     ok = wait(&w_empty[s], phase);
                     if (!ok) break;
-                    const int k = begin + i / TILES;
+                    // (a stage's second tile that is none of the unit is the first one again: nothing is multiplied with it)
+                    const int k = begin + min(i / TILES, w.n_kb - 1);
                     mbar_expect_tx(smem_u32(&w_full[s]), MX_TILE_BYTES);
                     bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES),
                                   src + (size_t)(k < w.n_kb ? k : k - w.n_kb) * MX_TILE_BYTES + (i % TILES) * next, MX_TILE_BYTES, smem_u32(&w_full[s]));
@@ -382,20 +389,25 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 const Unit w = unit_at(u);
                 const int boxes = GROUPED ? w.n_tok / a.tile : 1, box = GROUPED ? a.tile : a.bn;
                 int k = first_tile(w);
-                for (int i = 0; i < w.n_kb; ++i) {
+                for (int i = 0; i < w.n_kb; i += KT) {
                     if (!wait(&done[s], phase)) { *bail = 1; break; }
-                    const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES);
+                    const uint32_t bar = smem_u32(&full[s]);
                     const uint32_t scale_bytes = (uint32_t)(atoms_of(w.n_tok) * ATOM);
-                    mbar_expect_tx(bar, (uint32_t)w.n_tok * 2 * 128 + scale_bytes);
-                    for (int b = 0; b < boxes; ++b) {
+                    mbar_expect_tx(bar, min(KT, w.n_kb - i) * ((uint32_t)w.n_tok * 2 * 128 + scale_bytes));
 #pragma unroll
-                        for (int p = 0; p < 2; ++p)          // (rows beyond M are the other part's, or zeros: nobody stores them)
-                            tma_load_2d(dst + (uint32_t)(p * w.n_tok + b * box) * 128, &map_x, bar, (w.kb0 + k) * 64, p * a.M + w.m0 + b * box);
+                    for (int t = 0; t < KT; ++t) {
+                        if (t && i + t >= w.n_kb) break;
+                        const uint32_t dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES + t * F::TILE_BYTES);
+                        for (int b = 0; b < boxes; ++b) {
+#pragma unroll
+                            for (int p = 0; p < 2; ++p)      // (rows beyond M are the other part's, or zeros: nobody stores them)
+                                tma_load_2d(dst + (uint32_t)(p * w.n_tok + b * box) * 128, &map_x, bar, (w.kb0 + k) * 64, p * a.M + w.m0 + b * box);
+                        }
+                        const size_t tiles = GROUPED ? a.n_tiles : a.tiles_m, tile = w.m0 / (GROUPED ? a.tile : a.bn);
+                        const size_t at = ((size_t)(w.kb0 + k) * tiles + tile) * a.scale_bytes;
+                        bulk_copy_g2s(dst + TOK * 256, a.x_scales + at, scale_bytes, bar);
+                        if (++k == w.n_kb) k = 0;
                     }
-                    const size_t tiles = GROUPED ? a.n_tiles : a.tiles_m, tile = w.m0 / (GROUPED ? a.tile : a.bn);
-                    const size_t at = ((size_t)(w.kb0 + k) * tiles + tile) * a.scale_bytes;
-                    bulk_copy_g2s(dst + TOK * 256, a.x_scales + at, scale_bytes, bar);
-                    if (++k == w.n_kb) k = 0;
                     if (++s == R) { s = 0; phase ^= 1u; }
                 }
                 u = after(u, w);
@@ -424,9 +436,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 if (!ok) break;
                 tmem_fence_after();
                 const uint32_t d = tmem + (uint32_t)(b * F::ACC_COLS);
-                auto products = [&](int at, int h, bool fresh) {         // of the stage in place `at` of the ring with the h-th feature tile
-                    const uint32_t A0 = ring + (uint32_t)(at * F::RING_COLS), sfb = A0 + TILES * F::W_COLS;
-                    const uint64_t x = desc + (uint64_t)(at * (F::STAGE_BYTES / 16));
+                auto products = [&](int at, int h, bool fresh) {         // of the tile along K in place `at` of the ring with the h-th feature tile
+                    const uint32_t A0 = ring + (uint32_t)(at * F::TILE_COLS), sfb = A0 + TILES * F::W_COLS;
+                    const uint64_t x = desc + (uint64_t)(at * (F::TILE_BYTES / 16));
                     const uint32_t A = A0 + h * F::W_COLS, to = d + h * F::ACC_COLS;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -437,29 +449,38 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                             mma_mx(to, A + 8 * k, x + second + 2 * k, idesc + mx_block(k), A + A_COLS, sfb + sfb_second, 1u);
                     }
                 };
-                auto begin = [&](int at) {
+                auto begin = [&](int at, bool whole) {                   // the stage in place `at`, of KT tiles or of one
                     if (!wait_long(full_base + 8 * at, phase, a.status)) return false;
                     tmem_fence_after();
-                    const uint32_t sfb = ring + (uint32_t)(at * F::RING_COLS) + TILES * F::W_COLS;
 #pragma unroll
-                    for (int t = 0; t < F::ATOMS; ++t)
-                        if (t == 0 || !both) copy_scales(sfb + 4 * t, desc_scales + (uint64_t)((at * F::STAGE_BYTES + t * ATOM) / 16));
+                    for (int k = 0; k < KT; ++k) {
+                        const uint32_t sfb = ring + (uint32_t)((KT * at + k) * F::TILE_COLS) + TILES * F::W_COLS;
+#pragma unroll
+                        for (int t = 0; t < F::ATOMS; ++t)
+                            if ((k == 0 || whole) && (t == 0 || !both))
+                                copy_scales(sfb + 4 * t, desc_scales + (uint64_t)(((KT * at + k) * F::TILE_BYTES + t * ATOM) / 16));
+                    }
                     return true;
                 };
-                auto stage = [&](int at, bool fresh) {
-                    if (!begin(at)) return false;
+                auto stage = [&](int at, bool fresh, bool whole) {
+                    if (!begin(at, whole)) return false;
 #pragma unroll
-                    for (int h = 0; h < TILES; ++h) products(at, h, fresh);
+                    for (int k = 0; k < KT; ++k)
+                        if (k == 0 || whole) {
+#pragma unroll
+                            for (int h = 0; h < TILES; ++h) products(KT * at + k, h, fresh && k == 0);
+                        }
                     umma_commit(done_base + 8 * at);
                     return true;
                 };
                 int i = 0;
+                const int stages = stages_of(w), whole = w.n_kb / KT;
                 if constexpr (PAIR) {
                     // the first tile's products of the stages that the ring holds run ahead, while the epilogue still has the other accumulator
                     const int s0 = s, ahead = w.n_kb < R ? w.n_kb : R;
                     const uint32_t phase0 = phase;
                     for (; i < ahead && ok; ++i) {
-                        ok = begin(s);
+                        ok = begin(s, true);
                         if (ok) products(s, 0, i == 0);
                         if (++s == R) { s = 0; phase ^= 1u; }
                     }
@@ -473,20 +494,20 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                         if (++s == R) { s = 0; phase ^= 1u; }
                     }
                 }
-                while (ok && i < w.n_kb) {
+                while (ok && i < stages) {
                     constexpr int B = R % 4 == 0 ? 4 : 3;
                     static_assert(R % B == 0, "blocks of three or four places");
                     const int before = i;
 #pragma unroll
                     for (int p = 0; p < R; p += B) {
-                        if (!ok || s != p || i + B > w.n_kb) continue;
+                        if (!ok || s != p || i + B > whole) continue;
 #pragma unroll
-                        for (int q = 0; q < B; ++q) ok = ok && stage(p + q, q == 0 && i == 0);
+                        for (int q = 0; q < B; ++q) ok = ok && stage(p + q, q == 0 && i == 0, true);
                         s = p + B;
                         i += B;
                     }
                     if (i == before) {
-                        ok = stage(s, i == 0);
+                        ok = stage(s, i == 0, i < whole);
                         ++s; ++i;
                     }
                     if (s == R) { s = 0; phase ^= 1u; }
@@ -507,55 +528,61 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         const uint32_t lanes = ring + ((uint32_t)(quarter * 32) << 16);
         constexpr int TURNS = F::TURNS;
         const int turn = group / TILES, tile = group % TILES;
-        int ws = group, r = turn;
+        int ws = KT * group, r = turn;
         uint32_t w_phase = 0, r_phase = 0, it = 0;       // it: stages ahead of the unit, modulo TURNS
         int round = 0;
         bool ok = true;
         for (uint32_t u = first; u < last && ok;) {                 // (not `bailed`, which the four warps might see at different times)
             const Unit w = unit_at(u);
+            const int stages = stages_of(w);
             int i = turn - (int)it;                                      // the group's first stage of the unit
             if (i < 0) i += TURNS;
-            for (; i < w.n_kb; i += TURNS) {
+            for (; i < stages; i += TURNS) {
                 // one of the four warps asks: twenty that ask at every barrier again and again take half of the issue slots
                 if (quarter == 0) {
-                    ok = wait(&w_full[ws], w_phase);
-                    if (ok) ok = wait(&done[r], r_phase ^ 1u);           // the MMAs that read this place are done
+                    ok = wait(&done[r], r_phase ^ 1u);                   // the MMAs that read this place are done
+#pragma unroll
+                    for (int t = 0; t < KT; ++t)
+                        if (ok) ok = wait(&w_full[ws + t], w_phase);
                     if (!ok) group_failed[2 * group + round] = 1;
                 }
                 asm volatile("bar.sync %0, 128;" ::"r"(6 + group) : "memory");
                 ok = *(volatile int*)&group_failed[2 * group + round] == 0;      // (two flags in turn: the next round's is not seen yet)
                 round ^= 1;
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                const uint8_t* src = w_base + (size_t)ws * MX_TILE_BYTES;
-                const uint4 scales = *reinterpret_cast<const uint4*>(src + MX_CODE_BYTES + lane * 16);
-                uint4 c[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) c[q] = *reinterpret_cast<const uint4*>(src + (q * MX_ROWS + row) * 16);
                 tmem_fence_after();
-                const uint32_t dst = lanes + (uint32_t)(r * F::RING_COLS + tile * F::W_COLS);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t v[16];
+                for (int t = 0; t < KT; ++t) {
+                    const uint8_t* src = w_base + (size_t)(ws + t) * MX_TILE_BYTES;
+                    const uint4 scales = *reinterpret_cast<const uint4*>(src + MX_CODE_BYTES + lane * 16);
+                    uint4 c[4];
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint32_t in[4] = {c[2 * h + q].x, c[2 * h + q].y, c[2 * h + q].z, c[2 * h + q].w};
+                    for (int q = 0; q < 4; ++q) c[q] = *reinterpret_cast<const uint4*>(src + (q * MX_ROWS + row) * 16);
+                    const uint32_t dst = lanes + (uint32_t)(r * F::RING_COLS + t * F::TILE_COLS + tile * F::W_COLS);
 #pragma unroll
-                        for (int p = 0; p < 4; ++p) mx_decode(in[p], v[8 * q + 2 * p], v[8 * q + 2 * p + 1]);
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t v[16];
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t in[4] = {c[2 * h + q].x, c[2 * h + q].y, c[2 * h + q].z, c[2 * h + q].w};
+#pragma unroll
+                            for (int p = 0; p < 4; ++p) mx_decode(in[p], v[8 * q + 2 * p], v[8 * q + 2 * p + 1]);
+                        }
+                        tmem_st16(dst + 16 * h, v);
                     }
-                    tmem_st16(dst + 16 * h, v);
+                    tmem_st4(dst + A_COLS, scales);
+                    // (behind the stores, which need every number of the row: see gemm_f32_tc.cu)
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&w_empty[ws + t]));
                 }
-                tmem_st4(dst + A_COLS, scales);
-                // (behind the stores, which need every number of the row: see gemm_f32_tc.cu)
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&w_empty[ws]));
                 tmem_wait_st();
                 tmem_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&full[r]));
-                if ((ws += G) >= WS) { ws -= WS; w_phase ^= 1u; }
+                if ((ws += KT * G) >= WS) { ws -= WS; w_phase ^= 1u; }
                 if ((r += TURNS) >= R) { r -= R; r_phase ^= 1u; }
             }
-            it = (it + (uint32_t)w.n_kb) % TURNS;
+            it = (it + (uint32_t)stages) % TURNS;
             u = after(u, w);
         }
         if (!ok) *bail = 1;
@@ -714,32 +741,33 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         if (WIDE && leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");        // the boxes it sent are in memory
     } else if (F::FEW && warp >= F::SPLIT_WARP) {
-        // ---------------- few rows' parts: stages it = turn, turn + SPLITTERS, ..., a lane a block of 32 of row lane / 4 ----------------
+        // ---------------- few rows' parts: tiles it = turn, turn + SPLITTERS, ..., a lane a block of 32 of row lane / 4 ----------------
         fb_pdl_wait();
         const int turn = warp - F::SPLIT_WARP, block = lane & 3, r = lane >> 2;
         const __nv_bfloat16* row = r < a.M ? a.rows.x + (size_t)r * a.rows.ld : nullptr;
-        int s = turn;
-        uint32_t phase = 1, it = 0;
+        int s = turn / KT;
+        uint32_t phase = 1, it = 0;              // it: tiles ahead of the unit, modulo SPLITTERS
         bool ok = true;
         for (uint32_t u = first; u < last && ok;) {
             const Unit w = unit_at(u);
+            const int tiles = stages_of(w) * KT;
             uint4 raw[4];
-            auto load = [&](int i) {                                     // what the lane splits of the unit's i-th stage
+            auto load = [&](int i) {                                     // what the lane splits of the unit's i-th tile
                 const int k = (w.kb0 + i) * MX_COLS + block * MX_BLOCK;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) raw[q] = row ? mx_load8(row, k + 8 * q, a.K, a.rows.aligned != 0) : make_uint4(0, 0, 0, 0);
             };
-            int i = turn - (int)it;                                      // the warp's first stage of the unit
+            int i = turn - (int)it;                                      // the warp's first tile of the unit
             if (i < 0) i += SPLITTERS;
             if (i < w.n_kb) load(i);
-            for (; i < w.n_kb; i += SPLITTERS) {
+            for (; i < tiles; i += SPLITTERS) {                          // (of a stage's second tile that is none of the unit nothing is read)
                 uint2 one[4], two[4];
                 const uint32_t word = mx_split_block(raw, one, two);
                 if (i + SPLITTERS < w.n_kb) load(i + SPLITTERS);
                 if (lane == 0) ok = wait(&done[s], phase);               // the MMAs that read this place are done
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
-                uint8_t* stage = smem + s * F::STAGE_BYTES;
+                uint8_t* stage = smem + s * F::STAGE_BYTES + (turn % KT) * F::TILE_BYTES;
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {                            // rows of 128 bytes, their sixteens swizzled by the row's place in eight
                     const int at = r + p * w.n_tok;
@@ -753,9 +781,9 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&full[s]));
-                if ((s += SPLITTERS) >= R) { s -= R; phase ^= 1u; }
+                if ((s += SPLITTERS / KT) >= R) { s -= R; phase ^= 1u; }
             }
-            it = (it + (uint32_t)w.n_kb) % SPLITTERS;
+            it = (it + (uint32_t)tiles) % SPLITTERS;
             u = after(u, w);
         }
         if (!ok) *bail = 1;
