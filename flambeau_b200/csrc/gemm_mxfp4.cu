@@ -53,9 +53,9 @@ constexpr int SIDE_BY_SIDE = 64;                  // most tokens whose two parts
 constexpr int ATOM = 512;                         // scales of 128 rows for a stage, as tcgen05.cp brings them to tensor memory
 constexpr int TMEM = 512, SMEM = 227 * 1024;
 
-// TOK: most tokens of a tile.  R stages of rows and decoded weights, GROUPS of four decoding warps: a stage is 1,500 cycles on its way
-// from the first look at its weights to the end of its MMAs, of which a group works on it for half, so that it takes four groups
-// and eight stages to keep up with memory where the MMAs are short.
+// TOK: most tokens of a tile.  R stages of KT tiles of rows and decoded weights, GROUPS of four decoding warps: a stage of one tile is
+// 1,500 cycles on its way from the first look at its weights to the end of its MMAs, of which a group works on it for half.  Where
+// the MMAs are short, instructions are the bound, and two tiles a stage spare half of its waits and barriers.
 // PAIR: a unit is two neighbouring feature tiles, which share the stages of rows; their accumulators are the two that are otherwise
 // those of successive units, and sixteen warps store them.  It halves the reading of rows, and one round of pairs can replace two
 // of single tiles (128 x 28,672 x 4,096: 30 us, 34 single); see plan_wide.
@@ -807,7 +807,9 @@ int segments_of(long tiles_n, long kb, long grid) {           // the most stretc
     return (int)most;
 }
 // CTAs, one an SM, each with a few tiles at least, and the most stretches that they cut a row tile into: as many CTAs as leave no
-// more than `limit`.  Where shares have to meet (`join`), row tiles stay whole if they come out even and the longest stretch and the
+// more than `limit`, or fewer that cut every row tile alike, down to two thirds of them: a CTA then has one unit, and SMs are left for
+// the next kernel (32 x 4,096 x 14,336 to slabs: 148 stretches 16.0 us, 128 quarters 12.2; 8 rows 10.6 and 10.0, added 13.9 and 11.6;
+// 32 x 6,400 x 4,096 12.9 and 7.5 in 100 halves; with 80 of 148 one row of 10,240 x 8,192 took 13.8 us instead of 12.1).  Where shares have to meet (`join`), row tiles stay whole if they come out even and the longest stretch and the
 // meeting take longer (16 x 28,672 x 4,096 gated: 23.0 us in 148 stretches, 16.7 in 112 of two whole tiles).  In cycles: STAGE for a
 // tile of an SM, JOIN for the partial sums' way through L2 and back.
 constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 6000;
@@ -821,6 +823,8 @@ Cut cut_of(int tiles_n, int kb, int limit, bool join) {
     if (it != known.end()) return it->second;
     const long most = ((long)tiles_n * kb + LEAST_ITEMS - 1) / LEAST_ITEMS, slots = fb_sm_count();
     long grid = most < slots ? most : slots;
+    const long even = grid / tiles_n * tiles_n;
+    if (even * 3 >= grid * 2) grid = even;
     int segments = segments_of(tiles_n, kb, grid);
     while (segments > limit && grid > 1) segments = segments_of(tiles_n, kb, --grid);
     const long rounds = (tiles_n + slots - 1) / slots;
