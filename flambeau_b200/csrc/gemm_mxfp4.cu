@@ -849,7 +849,7 @@ constexpr double L2_BYTES = 62.0;                 // what an SM gets from L2 a c
 // written and read, and where they meet the adding, which nothing overlaps (67 x 6,144 x 5,120: three shares 21 us, whole 15.6 with
 // the same tiles).  Where it decides for or against pairs: 301 x 28,672 x 4,096 68 us single, 80 in pairs; 128 x 28,672 x 4,096
 // 34 single, 30 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.
-Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
+Plan cheapest(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
     const long sms = fb_sm_count(), tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     Plan best = {WIDE_TOKENS, 1, false};
     double best_cost = 1e300;
@@ -878,6 +878,17 @@ Plan plan_wide(long M, long N, int kb, int max_splits, long partial_floats, int 
 
 constexpr long SHARE_FLOATS = 16L << 20;          // most that the shares of one product may take
 constexpr int MOST_SPLITS = 16;
+
+Plan plan_wide(int M, int N, int kb, int max_splits, int n_counters, bool slabs) {
+    static std::map<std::tuple<int, int, int, int, int, bool, int>, Plan> known;             // (looking for it takes microseconds)
+    static std::mutex mu;
+    const std::tuple<int, int, int, int, int, bool, int> key{M, N, kb, max_splits, n_counters, slabs, fb_sm_count()};
+    std::lock_guard<std::mutex> lock(mu);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    if (known.size() > 4096) known.clear();
+    return known[key] = cheapest(M, N, kb, max_splits, SHARE_FLOATS, n_counters, slabs);
+}
 
 template <int TOK, bool GROUPED, bool PAIR> int launch(const MxArgs& a, const CUtensorMap& mx, const CUtensorMap& mo, long grid, cudaStream_t stream) {
     auto kernel = gemm_mxfp4_kernel<TOK, GROUPED, PAIR>;
@@ -964,7 +975,7 @@ static long long share_floats(int M, int N, int K, int n_counters) {
         const int segments = tiles_n <= n_counters ? cut_of(tiles_n, kb, ANY, true).segments : 1;
         return segments > 1 ? (long long)tiles_n * segments * narrow_tokens(M) * MX_ROWS : 0;
     }
-    const Plan p = plan_wide(M, N, kb, MOST_SPLITS, SHARE_FLOATS, n_counters, false);
+    const Plan p = plan_wide(M, N, kb, MOST_SPLITS, n_counters, false);
     return p.splits == 1 ? 0 : (long long)((M + p.bn - 1) / p.bn) * tiles_n * p.splits * p.bn * MX_ROWS;
 }
 
@@ -999,7 +1010,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
     a.gate = gate; a.plain_act = plain_act; a.status = status;
     const bool slabs = slab_stride > 0;
     const long long need = fb_gemm_mxfp4_scratch_bytes(M, N, K, n_counters, slabs, 0), rows = rows_bytes(M, N, K, 0, slabs);
-    FB_REQUIRE(scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= need && (slabs || (counters && n_counters > 0)),
+    FB_REQUIRE((need == 0 || (scratch && ((uintptr_t)scratch & 127) == 0 && scratch_bytes >= need)) && (slabs || (counters && n_counters > 0)),
                "gemm_mxfp4: %lld bytes of scratch wanted, and counters", need);
     a.partials = need > rows ? (float*)((uint8_t*)scratch + rows) : nullptr;
     const bool join = a.partials != nullptr;
@@ -1016,8 +1027,8 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
         if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
         return few_rows(M, N, K, 0, slabs) ? launch<FEW_TOKENS, false, false>(a, mx, mo, cut.grid, stream) : launch<32, false, false>(a, mx, mo, cut.grid, stream);
     }
-    const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, SHARE_FLOATS,
-                                n_counters, slabs);
+    const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, n_counters,
+                                slabs);
     a.bn = plan.bn;
     a.tiles_m = (M + plan.bn - 1) / plan.bn;
     a.units_n = plan.pair ? (a.tiles_n + 1) / 2 : a.tiles_n;

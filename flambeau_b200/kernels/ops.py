@@ -1681,6 +1681,7 @@ class Mxfp4Weight(PackedWeight):
         self.shape = torch.Size((*codes.shape[:-1], int(inputs)))
         groups = codes.shape[0] if codes.dim() == 3 else 1
         outputs = codes.shape[-2]
+        self._outputs, self._inputs = int(outputs), int(inputs)
         if groups < 1 or outputs < 1:
             raise KernelError("mxfp4 weight: no outputs")
         self.device = codes.device
@@ -1708,17 +1709,16 @@ class Mxfp4Weight(PackedWeight):
 
     def _operands(self, a: torch.Tensor, out: torch.Tensor, columns: int, what: str, indexed: bool = False) -> tuple:
         """Checks what a product takes: a [M, K] bfloat16, out [M, columns] float32 or bfloat16, rows dense.  (M, N, K)."""
-        N, K = self.shape[-2:]
-        if a.dim() != 2 or out.dim() != 2 or a.shape[1] != K or out.shape[1] != columns \
-                or (out.shape[0] != a.shape[0] and not indexed):
-            raise KernelError(f"{what}: shapes a{tuple(a.shape)} w{tuple(self.shape)} out{tuple(out.shape)} do not agree")
-        if a.dtype != torch.bfloat16:
+        N, K = self._outputs, self._inputs
+        rows, outs = a.shape, out.shape
+        if len(rows) != 2 or len(outs) != 2 or rows[1] != K or outs[1] != columns or (outs[0] != rows[0] and not indexed):
+            raise KernelError(f"{what}: shapes a{tuple(rows)} w{tuple(self.shape)} out{tuple(outs)} do not agree")
+        if a.dtype is not torch.bfloat16:
             raise KernelError(f"{what}: four-bit weights multiply bfloat16 rows, not {a.dtype}")
         if a.device != self.device or out.device != self.device:
             raise KernelError(f"{what}: the weight is on {self.device}, the rows on {a.device}, the output on {out.device}")
         dtype_code(out)
-        _rows(out)
-        return a.shape[0], N, K
+        return rows[0], N, K
 
     def _product(self, a, out, ctx, columns: int, what: str, gate=(0, 0.0, 0.0), plain_act: int = 0, accumulate: bool = False,
                  slabs=None) -> int:
@@ -1730,10 +1730,11 @@ class Mxfp4Weight(PackedWeight):
         nbytes = self._scratch_bytes(M, counters.numel(), slabs is not None, 0)
         mark = ws.mark()
         try:
-            check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self._tiles, out.data_ptr(), _CODES[out.dtype], out.stride(0),
+            check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self._tiles, out.data_ptr(), _CODES[out.dtype], _rows(out),
                                       slabs.stride(0) if slabs is not None else 0, slabs.shape[0] if slabs is not None else 0,
                                       _SPLITS_USED_REF, M, N, K, *gate, plain_act, accumulate, counters.data_ptr(), counters.numel(),
-                                      ws.reserve(nbytes), nbytes, ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4", (M, N, K))
+                                      ws.reserve(nbytes) if nbytes else 0, nbytes, ctx.runtime.status.data_ptr(), _stream()),
+                  "gemm_mxfp4", (M, N, K))
         finally:
             ws.release(mark)
         return _SPLITS_USED.value
@@ -1745,11 +1746,11 @@ class Mxfp4Weight(PackedWeight):
         if nbytes is None:
             if len(self._scratch) > 4096:
                 self._scratch.clear()
-            nbytes = self._scratch[key] = lib().fb_gemm_mxfp4_scratch_bytes(M, *self.shape[-2:], counters, slabs, tile)
+            nbytes = self._scratch[key] = lib().fb_gemm_mxfp4_scratch_bytes(M, self._outputs, self._inputs, counters, slabs, tile)
         return nbytes
 
     def linear(self, a, out, ctx) -> None:
-        self._product(a, out, ctx, self.shape[-2], "linear")
+        self._product(a, out, ctx, self._outputs, "linear")
 
     def linear_slabs(self, a, slabs, ctx) -> int:
         if slabs.dim() != 3 or slabs.dtype != torch.float32 or slabs.shape[0] < 1:
@@ -1757,7 +1758,7 @@ class Mxfp4Weight(PackedWeight):
         if slabs.shape[0] == 1:
             self.linear(a, slabs[0], ctx)
             return 1
-        return self._product(a, slabs[0], ctx, self.shape[-2], "linear_slabs", slabs=slabs)
+        return self._product(a, slabs[0], ctx, self._outputs, "linear_slabs", slabs=slabs)
 
     def linear_add(self, a, acc, ctx) -> bool:
         if acc.dtype != torch.float32:
@@ -1765,16 +1766,16 @@ class Mxfp4Weight(PackedWeight):
         # up to 128 rows the shares of K are better left to the next norm, which fetches the stream anyway
         if a.shape[0] <= 128:
             return False
-        self._product(a, acc[:a.shape[0]], ctx, self.shape[-2], "linear_add", accumulate=True)
+        self._product(a, acc[:a.shape[0]], ctx, self._outputs, "linear_add", accumulate=True)
         return True
 
     def gated_linear(self, a, out, activation, ctx) -> None:
-        if self.shape[-2] % 2:
+        if self._outputs % 2:
             raise KernelError("gated_linear: gate and up rows alternate, their number is even")
-        self._product(a, out, ctx, self.shape[-2] // 2, "gated_linear", gate=gate_arguments(activation))
+        self._product(a, out, ctx, self._outputs // 2, "gated_linear", gate=gate_arguments(activation))
 
     def activated_linear(self, a, out, activation_name, ctx) -> None:
-        self._product(a, out, ctx, self.shape[-2], "activated_linear", plain_act=plain_activation_code(activation_name))
+        self._product(a, out, ctx, self._outputs, "activated_linear", plain_act=plain_activation_code(activation_name))
 
     def grouped(self, a, row_index, tile_group, tile: int, out, ctx, activation_name=None, gate=None, row_share=None,
                 row_pair=None) -> None:
