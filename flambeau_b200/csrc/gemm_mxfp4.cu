@@ -26,8 +26,8 @@
 //
 // What bounds it.  A few rows: instructions.  Decoding a stage takes 150 of a scheduler's slots of the 370 cycles that HBM has it
 // under way, its barriers and the thread that issues MMAs another 100; before that a launch and the way from the first weights to the
-// first MMA, about 4 us (8 x 28,672 x 4,096: 14.9 us in a graph, 64% of HBM's rate).  Many rows: the MMAs, 512 cycles for 128 x 128 x
-// 128 in two parts, at the clock that the power limit leaves (2,048 x 28,672 x 4,096: 355 us, 1,350 TFLOP/s at 1.6 GHz).
+// first MMA, 3 to 4 us (8 x 28,672 x 4,096: 13.8 us in a graph, 69% of HBM's rate).  Many rows: the MMAs, 512 cycles for 128 x 128 x
+// 128 in two parts, at the clock that the power limit leaves (2,048 x 28,672 x 4,096: 353 us in bursts at 1.63 GHz, 413 at 1.35).
 #include "group_units.cuh"
 #include "mxfp4.cuh"
 #include "tensor_map.cuh"
