@@ -91,7 +91,7 @@ template <int TOK, bool PAIR> struct Form {
 __host__ __device__ constexpr int atoms_of(int tokens) { return tokens <= SIDE_BY_SIDE ? 1 : 2 * ((tokens + 127) / 128); }
 
 struct MxArgs {
-    const uint8_t* W; long w_group;                       // tiles, bytes of one group's
+    const uint8_t* W; long w_group; int groups;           // tiles, bytes of one group's
     MxRows rows;                                          // what X's parts, which come by map_x, are made from
     const uint8_t* x_scales; int scale_bytes;             // their scales, bytes of a tile's
     void* out; long ldo, slab_stride;
@@ -318,7 +318,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             const int t = (int)(entry & 0xffffffu);
             w.m0 = t * a.tile;
             w.n_tok = (int)(entry >> 24) * a.tile;
-            w.group = a.tile_group[t];
+            w.group = min(a.tile_group[t], a.groups - 1);            // (no weights lie beyond the last group's)
             w.nt = TILES * ((int)item - i * a.units_n);
             w.kb0 = 0; w.n_kb = a.kb; w.share = 0; w.shares = 1; w.id = 0;
         } else if constexpr (WIDE) {             // token tiles vary fastest: the CTAs that run together share weight tiles
@@ -1004,7 +1004,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
     if (M == 0) return 0;
     MxArgs a = {};
     a.W = (const uint8_t*)W; a.out = out; a.ldo = (long)ldo; a.slab_stride = (long)slab_stride;
-    a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, nullptr, nullptr, nullptr};
+    a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, M, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, nullptr, nullptr, nullptr};
     a.o_bf16 = o_dtype == FB_BF16; a.accumulate = accumulate; a.counters = counters;
     a.M = M; a.N = N; a.K = K; a.kb = (K + MX_COLS - 1) / MX_COLS; a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
@@ -1048,14 +1048,15 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
 
 // The grouped form: W holds `groups` matrices [N, K] in tiles; the M rows of `out` come in tiles of `tile` (a
 // multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are).  Row m is
-// X[m], or with row_index X[row_index[m]] (negative: zeros), with row_share times row_share[row_pair[m]].  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
-FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_index, const float* row_share, const int* row_pair,
+// X[m], or with row_index X[row_index[m]] (zeros where that is none of the x_rows), with row_share times row_share[row_pair[m]].  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
+FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, int x_rows, const int* row_index, const float* row_share, const int* row_pair,
                                  const void* W, int groups, const int* tile_group, int tile, void* out, int o_dtype,
                                  long long ldo, int M, int N, int K, int act, float limit, float slope, int plain_act, void* scratch,
                                  long long scratch_bytes, int* status, cudaStream_t stream) {
     const FbGate gate = {act, limit, slope};
     if (const int rc = check_operands(X, lda, W, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
     FB_REQUIRE(groups > 0 && tile_group, "gemm_mxfp4_grouped: no groups");
+    FB_REQUIRE(x_rows >= (row_index ? 0 : M), "gemm_mxfp4_grouped: %d rows are fewer than the %d of the output", x_rows, M);
     FB_REQUIRE(tile >= 16 && tile <= 128 && tile % 16 == 0 && M % tile == 0 && M / tile < (1 << 24),
                "gemm_mxfp4_grouped: the rows must be whole tiles of 16 to 128, not tiles of %d", tile);
     FB_REQUIRE(!row_share || (row_index && row_pair), "gemm_mxfp4_grouped: shares need the rows' index and pairs");
@@ -1065,7 +1066,8 @@ FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, const int* row_in
     a.kb = (K + MX_COLS - 1) / MX_COLS;
     a.tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     a.W = (const uint8_t*)W; a.w_group = (long)a.tiles_n * a.kb * MX_TILE_BYTES; a.out = out; a.ldo = (long)ldo;
-    a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, row_index, row_share, row_pair};
+    a.groups = groups;
+    a.rows = MxRows{(const __nv_bfloat16*)X, (long)lda, x_rows, lda % 8 == 0 && ((uintptr_t)X & 15) == 0, row_index, row_share, row_pair};
     a.o_bf16 = o_dtype == FB_BF16; a.M = M; a.N = N; a.K = K; a.tiles_m = 1; a.splits = a.max_segments = 1;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
     a.tile_group = tile_group; a.tile = tile; a.n_tiles = M / tile;

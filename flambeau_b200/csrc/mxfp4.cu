@@ -248,7 +248,7 @@ split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t*
     uint4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = make_uint4(0, 0, 0, 0);
-    if (from >= 0) {
+    if (from >= 0 && from < rows.count) {
         const __nv_bfloat16* row = rows.x + (size_t)from * rows.ld;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = mx_load8(row, k + 8 * i, K, rows.aligned != 0);

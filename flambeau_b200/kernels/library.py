@@ -66,7 +66,7 @@ _SIGNATURES = {
     # gemm_mxfp4.cu
     "fb_gemm_mxfp4_scratch_bytes": (L, [I, I, I, I, I, I]),
     "fb_gemm_mxfp4": (I, [P, L, P, P, I, L, L, I, P, I, I, I, I, F, F, I, I, P, I, P, L, P, STREAM]),
-    "fb_gemm_mxfp4_grouped": (I, [P, L, P, P, P, P, I, P, I, P, I, L, I, I, I, I, F, F, I, P, L, P, STREAM]),
+    "fb_gemm_mxfp4_grouped": (I, [P, L, I, P, P, P, P, I, P, I, P, I, L, I, I, I, I, F, F, I, P, L, P, STREAM]),
     # attention_simt.cu
     "fb_paged_attention_simt": (I, [P, L, P, L, I, P, P, I, I, P, I, P, I, P, P, I, I, I, I, I, I, I, F, F, P, P, P, L, I, L, P, STREAM]),
     # attention_tc.cu

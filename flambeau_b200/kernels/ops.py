@@ -611,7 +611,6 @@ def tc_supported(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> bool:
 
 
 _SPLITS_USED = ctypes.c_int(1)
-_SPLITS_USED_REF = ctypes.byref(_SPLITS_USED)
 
 
 def gemm_tc(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, status: torch.Tensor, splits: int = 0,
@@ -1623,8 +1622,9 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple:
     """(codes, scales) of x [..., columns], float32 or bfloat16 (a 2-d x may have rows apart, more dimensions are contiguous).
 
     A block's scale is the smallest power of two, not below 2^-127, under which its largest magnitude stays below 7 (where
-    rounding still ends at 6), but at most 2^125, so that every number is a finite float32; numbers go to the nearest of the grid, ties to the even code.  A block with an infinity or a NaN
-    becomes NaN as a whole.  The columns behind the last one of a row's last block count as zeros."""
+    rounding still ends at 6), but at most 2^125, so that every number is a finite float32; numbers go to the nearest of the
+    grid, ties to the even code.  A block with an infinity or a NaN becomes NaN as a whole.  The columns behind the last one of
+    a row's last block count as zeros."""
     _cuda(x)
     code = dtype_code(x)
     if x.dim() < 2 or x.shape[-1] < 1:
@@ -1728,16 +1728,17 @@ class Mxfp4Weight(PackedWeight):
             raise KernelError(f"{what}: four-bit weights need the step's scratch (ctx)")
         counters = ws.counters
         nbytes = self._scratch_bytes(M, counters.numel(), slabs is not None, 0)
+        splits = ctypes.c_int(1) if slabs is not None else None
         mark = ws.mark()
         try:
             check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self._tiles, out.data_ptr(), _CODES[out.dtype], _rows(out),
                                       slabs.stride(0) if slabs is not None else 0, slabs.shape[0] if slabs is not None else 0,
-                                      _SPLITS_USED_REF, M, N, K, *gate, plain_act, accumulate, counters.data_ptr(), counters.numel(),
+                                      ctypes.byref(splits) if splits is not None else None, M, N, K, *gate, plain_act, accumulate, counters.data_ptr(), counters.numel(),
                                       ws.reserve(nbytes) if nbytes else 0, nbytes, ctx.runtime.status.data_ptr(), _stream()),
                   "gemm_mxfp4", (M, N, K))
         finally:
             ws.release(mark)
-        return _SPLITS_USED.value
+        return splits.value if splits is not None else 1
 
     def _scratch_bytes(self, M: int, counters: int, slabs: bool, tile: int) -> int:
         """What the products want of the arena for M rows (asked of the library once per number of rows)."""
@@ -1807,7 +1808,8 @@ class Mxfp4Weight(PackedWeight):
         nbytes = self._scratch_bytes(M, 0, False, int(tile))
         mark = ws.mark()
         try:
-            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), _ptr(row_index), _ptr(row_share), _ptr(row_pair), self._tiles, self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(),
+            check(lib().fb_gemm_mxfp4_grouped(a.data_ptr(), _rows(a), a.shape[0], _ptr(row_index), _ptr(row_share), _ptr(row_pair),
+                                              self._tiles, self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(),
                                               dtype_code(out), _rows(out), M, N, K, *gate_args,
                                               plain_activation_code(activation_name), ws.reserve(nbytes), nbytes,
                                               ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4_grouped", (M, N, K))

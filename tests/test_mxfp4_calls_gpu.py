@@ -294,6 +294,31 @@ def test_offsets_past_32_bits():
     ctx.runtime.check_status()
 
 
+def test_indexes_that_name_no_row_and_no_group():
+    """A row that is none of the input's counts as zeros, as a negative one does; a group beyond the last one reads no weights of others."""
+    from flambeau_b200.kernels import ops
+    ctx = step()
+    w, codes, scales = drawn((3, 96), 64, 18)
+    dense = numbers(codes, scales)
+    x = rows(10, 64, 19)
+    for tile in (16, 32):
+        M = 3 * tile
+        tiles = torch.tensor([0, 2, 1], dtype=torch.int32, device="cuda")
+        index = (torch.arange(M, device="cuda") % 10).int()
+        index[1], index[tile + 2], index[2 * tile + 3] = 10, 2 ** 31 - 1, -2 ** 31
+        a = torch.where(((index >= 0) & (index < 10)).unsqueeze(1), x[index.clamp(0, 9).long()], 0)
+        out = torch.empty(M, 96, device="cuda")
+        ops.grouped_linear(x, index, w, tiles, tile, out, None, ctx)
+        for i, g in enumerate((0, 2, 1)):
+            part = slice(i * tile, (i + 1) * tile)
+            want, sums = product(a[part], dense[g])
+            assert close(out[part], want, sums)
+        ops.grouped_linear(x, index, w, torch.tensor([0, 7, 1], dtype=torch.int32, device="cuda"), tile, out, None, ctx)
+        want, sums = product(a[:tile], dense[0])
+        assert close(out[:tile], want, sums)
+    ctx.runtime.check_status()
+
+
 def test_what_products_refuse():
     from flambeau_b200.kernels import ops
     from flambeau_b200.kernels.library import KernelError
