@@ -299,7 +299,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     uint32_t first = blockIdx.x, last = a.items;
     if constexpr (GROUPED) {
         if (warp == EPI_WARP) {
-            fb_pdl_wait();                       // which weights a tile wants is the work of the kernels before this one
+            // (Which weights a tile wants is the work of kernels that have ended: the one that splits the rows lets this one in behind
+            // its own wait.  8 tokens on 6 of 64 experts, 3,584 x 4,096, with a wait here: 60 us, like this 57.)
             const int found = group_units<LIST>(a.tile_group, a.n_tiles, most, list);
             if (lane == 0) *unit_count = found;
         }

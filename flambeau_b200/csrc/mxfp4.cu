@@ -210,8 +210,11 @@ template <bool GROUPED>
 __global__ void __launch_bounds__(256)
 split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t* __restrict__ parts, uint8_t* __restrict__ scales,
              const __grid_constant__ MxScaleLayout layout) {
-    fb_pdl_launch_dependents();
+    // (grouped: the product comes in behind the wait, and so behind the kernels that order the rows: it looks up its weights and asks
+    // for them while the rows are split)
+    if constexpr (!GROUPED) fb_pdl_launch_dependents();
     fb_pdl_wait();
+    if constexpr (GROUPED) fb_pdl_launch_dependents();
     const int blocks = Kp / MX_BLOCK, lane = threadIdx.x & 31, first = blockIdx.x * SPLIT_ROWS;
     const int item = blockIdx.y * 256 + threadIdx.x, q = item / blocks, m = first + q, k = (item - q * blocks) * MX_BLOCK;
     int unit, tokens, at, tiles;                         // the scales' tile, its tokens, the first row's place in it, all tiles
