@@ -33,10 +33,6 @@
 #include "tensor_map.cuh"
 #include "umma.cuh"
 
-#include <map>
-#include <mutex>
-#include <tuple>
-
 namespace {
 
 constexpr int A_COLS = MX_COLS / 4;               // tensor-memory columns of a stage's weights, then of their scales
@@ -815,13 +811,23 @@ int segments_of(long tiles_n, long kb, long grid) {           // the most stretc
 // tile of an SM, JOIN for the partial sums' way through L2 and back.
 constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 6000;
 struct Cut { int grid, segments; };
+// What was last asked for in a place of a thread's table, and the answer to it (neither allocates nor locks).
+constexpr int REMEMBERED = 256;
+template <typename Value, int N> struct Remembered {
+    int asked[N];
+    Value value;
+    bool is(const int (&key)[N]) {               // else it is so from now on, and its value wanted
+        bool same = true;
+        for (int i = 0; i < N; ++i) same = same && asked[i] == key[i];
+        if (!same)
+            for (int i = 0; i < N; ++i) asked[i] = key[i];
+        return same;
+    }
+};
 Cut cut_of(int tiles_n, int kb, int limit, bool join) {
-    static std::map<std::tuple<int, int, int, int>, Cut> known;              // (counting through the tiles takes microseconds)
-    static std::mutex mu;
-    const std::tuple<int, int, int, int> key{tiles_n, kb, join ? -limit : limit, fb_sm_count()};
-    std::lock_guard<std::mutex> lock(mu);
-    const auto it = known.find(key);
-    if (it != known.end()) return it->second;
+    static thread_local Remembered<Cut, 4> known[REMEMBERED];                // (counting through the tiles takes microseconds)
+    Remembered<Cut, 4>& was = known[(uint32_t)(tiles_n + 37 * kb + 101 * limit + join) % REMEMBERED];
+    if (was.is({tiles_n, kb, join ? -limit : limit, fb_sm_count()})) return was.value;
     const long most = ((long)tiles_n * kb + LEAST_ITEMS - 1) / LEAST_ITEMS, slots = fb_sm_count();
     long grid = most < slots ? most : slots;
     const long even = grid / tiles_n * tiles_n;
@@ -833,8 +839,7 @@ Cut cut_of(int tiles_n, int kb, int limit, bool join) {
         grid = tiles_n / rounds;
         segments = 1;
     }
-    if (known.size() > 4096) known.clear();
-    return known[key] = Cut{(int)grid, segments};
+    return was.value = Cut{(int)grid, segments};
 }
 int narrow_tokens(int M) { return (M + 7) / 8 * 8; }
 
@@ -881,14 +886,10 @@ constexpr long SHARE_FLOATS = 16L << 20;          // most that the shares of one
 constexpr int MOST_SPLITS = 16;
 
 Plan plan_wide(int M, int N, int kb, int max_splits, int n_counters, bool slabs) {
-    static std::map<std::tuple<int, int, int, int, int, bool, int>, Plan> known;             // (looking for it takes microseconds)
-    static std::mutex mu;
-    const std::tuple<int, int, int, int, int, bool, int> key{M, N, kb, max_splits, n_counters, slabs, fb_sm_count()};
-    std::lock_guard<std::mutex> lock(mu);
-    const auto it = known.find(key);
-    if (it != known.end()) return it->second;
-    if (known.size() > 4096) known.clear();
-    return known[key] = cheapest(M, N, kb, max_splits, SHARE_FLOATS, n_counters, slabs);
+    static thread_local Remembered<Plan, 7> known[REMEMBERED];                               // (looking for it takes microseconds)
+    Remembered<Plan, 7>& was = known[(uint32_t)(M + 37 * N + 101 * kb + 211 * max_splits + slabs) % REMEMBERED];
+    if (was.is({M, N, kb, max_splits, n_counters, slabs ? 1 : 0, fb_sm_count()})) return was.value;
+    return was.value = cheapest(M, N, kb, max_splits, SHARE_FLOATS, n_counters, slabs);
 }
 
 template <int TOK, bool GROUPED, bool PAIR> int launch(const MxArgs& a, const CUtensorMap& mx, const CUtensorMap& mo, long grid, cudaStream_t stream) {
