@@ -1627,16 +1627,16 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple:
     a row's last block count as zeros."""
     _cuda(x)
     code = dtype_code(x)
-    if x.dim() < 2 or x.shape[-1] < 1:
+    *lead, columns = x.shape if x.dim() else (0,)
+    if not lead or columns < 1:
         raise KernelError(f"quantize_mxfp4: rows wanted, not a tensor of shape {tuple(x.shape)}")
-    if x.dim() > 2 and not x.is_contiguous():
+    if len(lead) > 1 and not x.is_contiguous():
         raise KernelError("quantize_mxfp4: more than two dimensions must be contiguous")
-    flat = x if x.dim() == 2 else x.view(-1, x.shape[-1])
-    rows, columns = flat.shape
+    flat = x if len(lead) == 1 else x.view(-1, columns)
+    rows = flat.shape[0]
     stride = _rows(flat) if rows > 1 or flat.stride(1) != 1 else columns
     blocks = -(-columns // MXFP4_BLOCK)
-    codes = torch.empty((*x.shape[:-1], 16 * blocks), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device)
+    codes, scales = x.new_empty((*lead, 16 * blocks), dtype=torch.uint8), x.new_empty((*lead, blocks), dtype=torch.uint8)
     check(lib().fb_quantize_mxfp4(flat.data_ptr(), code, stride, rows, columns, codes.data_ptr(), scales.data_ptr(), _stream()),
           "quantize_mxfp4")
     return codes, scales
@@ -1646,8 +1646,8 @@ def _mxfp4_blocks(codes: torch.Tensor, scales: torch.Tensor, columns: int, what:
     """The number of blocks of a row."""
     _cuda(codes, scales)
     blocks = -(-int(columns) // MXFP4_BLOCK)
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or columns < 1 or codes.dim() < 2 \
-            or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * blocks or scales.shape[-1] != blocks:
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or columns < 1 or codes.dim() < 2 \
+            or (*codes.shape[:-1], blocks) != tuple(scales.shape) or codes.shape[-1] != 16 * blocks:
         raise KernelError(f"{what}: uint8 codes [..., {16 * blocks}] and scales [..., {blocks}] wanted for {columns} columns, not "
                           f"{tuple(codes.shape)} and {tuple(scales.shape)}")
     if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
@@ -1658,7 +1658,7 @@ def _mxfp4_blocks(codes: torch.Tensor, scales: torch.Tensor, columns: int, what:
 def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, columns: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The numbers that codes and scales stand for, [..., columns] in float32 or bfloat16 (which holds them exactly)."""
     blocks = _mxfp4_blocks(codes, scales, columns, "dequantize_mxfp4")
-    out = torch.empty((*codes.shape[:-1], columns), dtype=dtype, device=codes.device)
+    out = codes.new_empty((*codes.shape[:-1], columns), dtype=dtype)
     code = dtype_code(out)
     check(lib().fb_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), scales.numel() // blocks, int(columns), out.data_ptr(), code,
                                     int(columns), _stream()), "dequantize_mxfp4")
