@@ -54,13 +54,13 @@ constexpr int TMEM = 512, SMEM = 227 * 1024;
 // the MMAs are short, instructions are the bound, and two tiles a stage spare half of its waits and barriers.
 // PAIR: a unit is two neighbouring feature tiles, which share the stages of rows; their accumulators are the two that are otherwise
 // those of successive units, and sixteen warps store them.  It halves the reading of rows, and one round of pairs can replace two
-// of single tiles (128 x 28,672 x 4,096: 30 us, 34 single); see plan_wide.
+// of single tiles (128 x 28,672 x 4,096: 30 us, 34 single; 64 rows 20.8 and 22.2); see plan_wide.
 template <int TOK, bool PAIR> struct Form {
     static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow forms cut the line of tiles, and store directly)
     static constexpr bool FEW = TOK <= FEW_TOKENS;
     static constexpr int TILES = PAIR ? 2 : 1;
     static constexpr int KT = WIDE ? 1 : 2;                              // tiles along K of a stage
-    static constexpr int R = TOK <= NARROW_TOKENS ? 4 : TOK <= SIDE_BY_SIDE ? 6 : PAIR ? 3 : 4;
+    static constexpr int R = TOK <= NARROW_TOKENS ? 4 : PAIR ? 3 : TOK <= SIDE_BY_SIDE ? 6 : 4;
     static constexpr int GROUPS = FEW ? 3 : TOK <= NARROW_TOKENS ? 4 : PAIR ? 2 : 3;
     static constexpr int EPI_GROUPS = FEW ? 1 : PAIR ? 4 : 2, EPI = 128 * EPI_GROUPS;   // groups of four warps, threads of the epilogue
     static constexpr int TURNS = GROUPS / TILES;                         // groups that take a feature tile's stages in turn
@@ -76,6 +76,10 @@ template <int TOK, bool PAIR> struct Form {
     static constexpr int FIT = (RING - R * STAGE_BYTES) / MX_TILE_BYTES;
     static constexpr int PRODUCERS = WIDE ? 1 : 2;                       // threads that ask for weights, each for places of its own
     static constexpr int WS = (FIT < MAX_W ? FIT : MAX_W) / PRODUCERS * PRODUCERS;
+    // Threads that ask for rows, each for places of its own.  (Groups of 64 rows at most, 180 tokens on 6 of 64 experts, 3,584 x 4,096: one
+    // 114 us, two 104.)
+    static constexpr int ROW_PRODUCERS = WIDE && TOK <= SIDE_BY_SIDE && !PAIR ? 2 : 1;
+    static_assert(R % ROW_PRODUCERS == 0 && PRODUCERS + ROW_PRODUCERS <= 3, "places of their own, warps 0, 2 and 3");
     static constexpr int ARRIVALS = 4 * TILES + (FEW ? KT : 1);          // at full[s]: of the decoding warps, and of who brings the rows
     static_assert(2 * ACC_COLS + R * RING_COLS <= TMEM, "tensor memory");
     static_assert(TURNS <= R && WS % KT == 0 && WS >= KT * (GROUPS + TILES * R) && (!FEW || SPLITTERS / KT <= R),
@@ -376,37 +380,41 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             }
         }
         __syncwarp();
-    } else if (warp == 2) {
+    } else if (warp == 2 || (F::ROW_PRODUCERS == 2 && warp == 3)) {
         // ---------------- the rows' parts and their scales (of few rows: see the last warps) ----------------
         if (!F::FEW && elect_one()) {
             fb_pdl_wait();
-            int s = 0;
+            const int turn = warp == 2 ? 0 : 1;
+            int s = turn, i = turn;                  // i: the thread's first stage of the unit
             uint32_t phase = 1;
             for (uint32_t u = first; u < last && !bailed();) {
                 const Unit w = unit_at(u);
-                const int boxes = GROUPED ? w.n_tok / a.tile : 1, box = GROUPED ? a.tile : a.bn;
-                int k = first_tile(w);
-                for (int i = 0; i < w.n_kb; i += KT) {
+                const int boxes = GROUPED ? w.n_tok / a.tile : 1, box = GROUPED ? a.tile : a.bn, stages = stages_of(w), begin = first_tile(w);
+                const uint32_t scale_bytes = (uint32_t)(atoms_of(w.n_tok) * ATOM);
+                const size_t step = (size_t)(GROUPED ? a.n_tiles : a.tiles_m) * a.scale_bytes;       // scales of a tile along K
+                const uint8_t* scales = a.x_scales + (size_t)(w.m0 / (GROUPED ? a.tile : a.bn)) * a.scale_bytes + w.kb0 * step;
+                int k = begin + KT * i;
+                if (k >= w.n_kb) k -= w.n_kb;
+                for (; i < stages; i += F::ROW_PRODUCERS) {
                     if (!wait(&done[s], phase)) { *bail = 1; break; }
                     const uint32_t bar = smem_u32(&full[s]);
-                    const uint32_t scale_bytes = (uint32_t)(atoms_of(w.n_tok) * ATOM);
-                    mbar_expect_tx(bar, min(KT, w.n_kb - i) * ((uint32_t)w.n_tok * 2 * 128 + scale_bytes));
+                    mbar_expect_tx(bar, min(KT, w.n_kb - KT * i) * ((uint32_t)w.n_tok * 2 * 128 + scale_bytes));
 #pragma unroll
                     for (int t = 0; t < KT; ++t) {
-                        if (t && i + t >= w.n_kb) break;
+                        if (t && KT * i + t >= w.n_kb) break;
                         const uint32_t dst = smem_u32(smem) + (uint32_t)(s * F::STAGE_BYTES + t * F::TILE_BYTES);
                         for (int b = 0; b < boxes; ++b) {
 #pragma unroll
                             for (int p = 0; p < 2; ++p)      // (rows beyond M are the other part's, or zeros: nobody stores them)
                                 tma_load_2d(dst + (uint32_t)(p * w.n_tok + b * box) * 128, &map_x, bar, (w.kb0 + k) * 64, p * a.M + w.m0 + b * box);
                         }
-                        const size_t tiles = GROUPED ? a.n_tiles : a.tiles_m, tile = w.m0 / (GROUPED ? a.tile : a.bn);
-                        const size_t at = ((size_t)(w.kb0 + k) * tiles + tile) * a.scale_bytes;
-                        bulk_copy_g2s(dst + TOK * 256, a.x_scales + at, scale_bytes, bar);
+                        bulk_copy_g2s(dst + TOK * 256, scales + k * step, scale_bytes, bar);
                         if (++k == w.n_kb) k = 0;
                     }
-                    if (++s == R) { s = 0; phase ^= 1u; }
+                    if (F::ROW_PRODUCERS == 2 && ++k == w.n_kb) k = 0;                       // (the other thread's)
+                    if ((s += F::ROW_PRODUCERS) >= R) { s -= R; phase ^= 1u; }
                 }
+                i -= stages;
                 u = after(u, w);
             }
         }
@@ -864,7 +872,6 @@ Plan cheapest(long M, long N, int kb, int max_splits, long partial_floats, int n
         const int bn = (int)(((M + tiles_m - 1) / tiles_m + 15) / 16 * 16);
         const long tiles = (M + bn - 1) / bn;
         for (int pair = 0; pair <= 1; ++pair) {
-            if (pair && bn <= SIDE_BY_SIDE) continue;
             const long units_n = pair ? (tiles_n + 1) / 2 : tiles_n;
             const double l2 = (bn * 256.0 + (pair ? 2 : 1) * (double)MX_TILE_BYTES) / L2_BYTES;
             for (int splits = 1; splits <= max_splits && splits <= kb; ++splits) {
@@ -1044,7 +1051,7 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
     if (items > 2000000000L) return fb_fail(-1, "gemm_mxfp4: too many tiles (M=%d N=%d)", M, N);
     if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
     const long grid = items < fb_sm_count() ? items : fb_sm_count();
-    if (plan.pair) return launch<128, false, true>(a, mx, mo, grid, stream);
+    if (plan.pair) return a.bn <= 64 ? launch<64, false, true>(a, mx, mo, grid, stream) : launch<128, false, true>(a, mx, mo, grid, stream);
     return a.bn <= 64 ? launch<64, false, false>(a, mx, mo, grid, stream) : launch<128, false, false>(a, mx, mo, grid, stream);
 }
 

@@ -107,6 +107,30 @@ def test_an_odd_number_of_feature_tiles_in_pairs():
     assert int(ctx.ws.counters.abs().sum()) == 0
 
 
+@pytest.mark.parametrize("M", [40, 64])
+def test_pairs_of_feature_tiles_and_up_to_64_rows(M):
+    """Both parts of the rows side by side, two feature tiles a unit, the last one alone."""
+    from flambeau_b200.kernels import ops
+    ctx = step()
+    N, K = 28790, 4096 + 64
+    w, codes, scales = drawn((N,), K, 31)
+    a = rows(M, K, M)
+    want, sums = product(a, numbers(codes, scales))
+    for dtype, rounding in ((torch.float32, 0.0), (torch.bfloat16, 2.0 ** -8)):
+        out = torch.full((M, N + 2), 7.0, dtype=dtype, device="cuda")
+        ops.linear(a, w, out[:, :N], ctx)
+        assert close(out[:, :N], want, sums, rounding) and bool((out[:, N:] == 7.0).all())
+        act = torch.empty(M, N // 2, dtype=dtype, device="cuda")
+        ops.gated_linear(a, w, act, "silu", ctx)
+        ref, allowed = gated(want, sums, rounding + 2.0 ** -20)
+        assert close(act, ref, allowed)
+    slabs = torch.full((3, M, N), 7.0, device="cuda")
+    k = ops.linear_slabs(a, w, slabs, ctx)
+    assert close(slabs[:k].double().sum(0), want, sums) and bool((slabs[k:] == 7.0).all())
+    ctx.runtime.check_status()
+    assert int(ctx.ws.counters.abs().sum()) == 0
+
+
 @pytest.mark.parametrize("M,N,K", [(48, 384, 14336), (100, 256, 8192), (130, 200, 16384)])
 def test_shares_of_many_rows_meet(M, N, K):
     """So few tiles that K is split, by rows that leave the last tile of tokens open."""
