@@ -862,7 +862,8 @@ constexpr double L2_BYTES = 62.0;                 // what an SM gets from L2 a c
 // one's products (100 cycles a token for both tiles), of a single tile's only the last one's shows.  Shares of K cost a copy of the output,
 // written and read, and where they meet the adding, which nothing overlaps (67 x 6,144 x 5,120: three shares 21 us, whole 15.6 with
 // the same tiles).  Where it decides for or against pairs: 301 x 28,672 x 4,096 68 us single, 80 in pairs; 128 x 28,672 x 4,096
-// 34 single, 30 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.
+// 34 single, 30 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.  (Pairs of up to 64 tokens have three stages in flight for the
+// way to L2 and back, 690 cycles: 64 x 28,672 x 4,096 22.2 single, 20.8 in pairs, 301 in tiles of 64 74.)
 Plan cheapest(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
     const long sms = fb_sm_count(), tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     Plan best = {WIDE_TOKENS, 1, false};
@@ -877,7 +878,7 @@ Plan cheapest(long M, long N, int kb, int max_splits, long partial_floats, int n
             for (int splits = 1; splits <= max_splits && splits <= kb; ++splits) {
                 if (!slabs && splits > 1 && (tiles * tiles_n > n_counters || tiles * tiles_n * splits * bn * MX_ROWS > partial_floats)) break;
                 const long units = tiles * units_n * splits, rounds = (units + sms - 1) / sms;
-                const double stage = fmax(fmax((pair ? 8.0 : 4.0) * bn, l2), pair ? 490.0 : 300.0 + (double)(units < sms ? units : sms)) + 30.0;
+                const double stage = fmax(fmax((pair ? 8.0 : 4.0) * bn, l2), pair ? (bn <= SIDE_BY_SIDE ? 690.0 : 490.0) : 300.0 + (double)(units < sms ? units : sms)) + 30.0;
                 double cost = fmax((double)rounds * ((kb + splits - 1) / splits * stage + (pair ? 100.0 * bn : 500.0)) + (pair ? 0.0 : 45.0 * bn),
                                    (double)tiles_n * kb * MX_TILE_BYTES / (23.0 * sms));
                 cost += (splits - 1) * (double)M * N * 8.0 / (24.0 * sms);
