@@ -11,7 +11,7 @@
 // parts side by side), and decoding is moving bits (3 instructions for eight), since the scales go to the tensor core as they are.
 //
 // Layout.  A CTA owns 128 output features x a tile of tokens ("swap-AB": the weight is the 128-row operand, the tokens are N).  A stage
-// is 128 of K: one bulk copy brings a weight tile as it lies in memory, groups of four warps take the stages in turn and decode, a
+// is 128 of K (256 up to 32 tokens): one bulk copy brings a weight tile as it lies in memory, groups of four warps take the stages in turn and decode, a
 // thread a feature, into tensor memory, where the MMA takes its A operand and both operands' scales from; the rows' parts, made
 // once for all CTAs by a kernel of their own, come by TMA (K-major, 128-byte swizzle), their scales by tcgen05.cp.  Up to 64 tokens the
 // two parts are N's two halves, which the epilogue adds; with more they are two instructions into one accumulator.
@@ -24,7 +24,7 @@
 // full[s]: a stage's rows (by bytes) and its decoded weights (by arrivals) are there; done[s]: its MMAs are.  Two accumulators, so that
 // the epilogue of one unit overlaps the products of the next.  Every mbarrier wait is bounded as in gemm_tc.cu.
 //
-// What bounds it.  A few rows: instructions.  Decoding a stage takes 150 of a scheduler's slots of the 370 cycles that HBM has it
+// What bounds it.  A few rows: instructions.  Decoding a tile takes 150 of a scheduler's slots of the 370 cycles that HBM has it
 // under way, its barriers and the thread that issues MMAs another 100; before that a launch and the way from the first weights to the
 // first MMA, 3 to 4 us (8 x 28,672 x 4,096: 13.8 us in a graph, 69% of HBM's rate).  Many rows: the MMAs, 512 cycles for 128 x 128 x
 // 128 in two parts, at the clock that the power limit leaves (2,048 x 28,672 x 4,096: 353 us in bursts at 1.63 GHz, 413 at 1.35).
@@ -528,7 +528,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         // ---------------- decode: a thread a feature; weight tiles it = group, group + G, ... (of a pair, always the same one) ----------------
         // (A wait names a phase by its parity alone, and a group does not come to every slot in every round of a ring.  It comes every
         // TURNS stages and has seen the MMAs of the stage TURNS + R ago done, so with TURNS <= R no slot of that ring is two rounds
-        // behind, and with WS >= GROUPS + TILES R none of the weights'.)
+        // behind, and with WS >= KT (GROUPS + TILES R) none of the weights'.)
         const int quarter = warp & 3, row = quarter * 32 + lane, group = (warp - 4) >> 2;
         const uint32_t lanes = ring + ((uint32_t)(quarter * 32) << 16);
         constexpr int TURNS = F::TURNS;
