@@ -2,8 +2,11 @@
 //
 // tcgen05.mma.kind::mxf8f6f4 multiplies numbers of up to 8 bits whose blocks of 32 along K carry power-of-two scales, and sums in
 // float32.  A four-bit weight is such a number as it is.  A row's bfloat16 numbers become two e4m3 numbers each, the second what the
-// first left (mxfp4.cuh: what is lost is at most 2^-22 of a block's largest number, far below what bfloat16 itself has rounded), so the
-// product is that of bfloat16 rows with the weights' numbers, summed in float32; only infinities among the rows end as NaN.
+// first left, under one scale a block of 32 (mxfp4.cuh): numbers down to 2^-14 of the block's largest are held exactly, smaller ones to
+// 2^-22 of it.  So the product is that of bfloat16 rows with the weights' numbers, summed in float32, but for rows with numbers so far
+// above their neighbours: what those lose is what a float32 sum with the largest among its terms loses, and shows where the largest meets a
+// weight of zero (one of 2^13 in every block: 8e-4 of such sums).  A third part would be half as many MMAs again.  An infinity or a NaN
+// among a row's numbers makes all its sums NaN.
 //
 // Why this instruction, on one SM, for 128 features x 128 of K (a tile of 8,704 bytes, which HBM brings every 370 cycles): kind::f16
 // takes 8 instructions of 70 cycles at least, whatever the number of tokens up to 128, and its weights have to be decoded to

@@ -35,9 +35,12 @@ __device__ __forceinline__ float mx_scale_f32(uint32_t s) {
 
 // ---- rows of bfloat16 numbers as two e4m3 numbers each ----
 // With 2^e <= amax < 2^(e + 1) the largest magnitude of a block of 32, y = x 2^(7 - e) lies below 2^8; its first part is y rounded
-// to e4m3, its second what that left, times 2^5.  Eight bits of mantissa go into four and four: what is lost is 2^-22 of amax at most.
+// to e4m3, its second what that left, times 2^5.  Eight bits of mantissa go into four and four where |y| >= 2^-7: such numbers, down to
+// 2^-14 of 2^e, are held exactly.  Below, the second part's last place, 2^-14, rounds them: what is lost is at most 2^-15, or 2^-22 of
+// amax.  That is a rounding to fewer bits than bfloat16 has, of numbers that stand beside one 2^14 times as large.
 // Scales: MX_FIRST less than the exponent's field for the first part, 5 less again for the second; blocks below 2^-115 use that
-// exponent's.  A block with an infinity or a NaN gets scales of 255, and so do the sums that it is part of.
+// exponent's, and lose 2^-137 at most (nothing of a bfloat16 number).  A block with an infinity or a NaN gets scales of 255, and so do
+// the sums that it is part of.
 constexpr int MX_LEAST_FIELD = 12, MX_FIRST = 7, MX_SECOND_LESS = 5;
 // `top`: the largest magnitude's 15 bits of the block.
 __device__ __forceinline__ uint32_t mx_row_scale(uint32_t top) {

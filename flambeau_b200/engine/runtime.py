@@ -115,8 +115,10 @@ class Workspace:
 
 class Runtime:
     """`weights`: how the large maps of attention and feed-forwards hold their weights, 'stored' (as the model folder and the
-    dtype rule say) or 'mxfp4' (quantised to four bits when they are bound; embedding, head, norms, routers and the maps
-    whose outputs are rates of a recurrence stay as stored)."""
+    dtype rule say) or 'mxfp4' (quantised to four bits when they are bound; embedding, head, norms, routers, the
+    maps per head of latent attention and every map that a recurrence reads, its queries, keys, values, gates and
+    rates, stay as stored; a recurrence's output map is among the four-bit ones).  The bfloat16 rows that four-bit
+    weights multiply are held to 2^-22 of the largest number among 32 neighbours (kernels.ops.Mxfp4Weight)."""
 
     def __init__(self, device="cuda:0", dtype="bfloat16", page_size: int = 16, workspace_bytes: int = 1 << 24,
                  weights: str = "stored"):

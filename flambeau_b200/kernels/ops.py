@@ -1671,7 +1671,9 @@ class Mxfp4Weight(PackedWeight):
 
     `shape`, `dtype` (of the rows that it multiplies), `device`, `nbytes` are those of a weight tensor.  Every number of such a
     weight is a bfloat16 number: the products give what bfloat16 products with `dequantize_mxfp4`'s numbers give, up to the order of
-    their float32 sums."""
+    their float32 sums and a rounding of the rows: a number below 2^-14 of the largest among its row's block of 32 columns is held
+    to 2^-22 of that largest one.  A float32 sum with the largest among its terms loses as much anyway; where the largest meets a
+    weight of zero, the smaller ones' products are off by up to that much.  A row with an infinity or a NaN gives NaN."""
     dtype = torch.bfloat16
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, inputs: int):
