@@ -162,14 +162,22 @@ __device__ __forceinline__ void store_box(const void* map, uint32_t src, int x, 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
-// g sigmoid(g) u by the approximate exponential and reciprocal (relative errors of 2^-22 and 2^-23; the exponential's argument is
-// rounded to 2^-24 of itself): within 3e-7 (2 + |g|) of the result.  The exact ones made the epilogue of 160 tokens longer than the
-// products of K = 4,096.
+// g sigmoid(g) u with h = e^(-|g| / 2): g u / (1 + h h), below zero with h h above the line, one h a factor, so that nothing
+// overflows and nothing vanishes before the result does (g < -174: zero).  The exponential and the reciprocal are the approximate ones
+// (2^-22 and 2^-23 of themselves); what the exponential's argument -|g| log2(e) / 2 loses by rounding is computed with the constant in
+// two parts, as Cody and Waite reduce arguments, and comes back as the first term of e^x.  17 x 2^-24 of the result at most, whatever g.
+// expf and a division made the epilogue of 160 tokens longer than the products of K = 4,096.
 __device__ __forceinline__ float silu_times(float g, float u) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * g));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));          // (e = inf: 0)
-    return g * r * u;
+    constexpr double HALF_LOG2E = 0.72134752044448170368, LN2 = 0.69314718055994530942;
+    constexpr float HI = (float)HALF_LOG2E, LO = (float)(HALF_LOG2E - (double)HI);
+    const float m = fminf(fabsf(g), 512.0f), t = -HI * m;                  // (an infinity would make a NaN of what t loses)
+    const float rest = fmaf(-LO, m, fmaf(-HI, m, -t)) * (float)LN2;
+    float h, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(t));
+    h = fmaf(h, rest, h);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.0f)));
+    const float p = g < 0.0f ? h : 1.0f;
+    return g * p * u * (p * r);
 }
 
 // The epilogue's code is walked a few times a tile only, so that its instructions come from far: every 128 bytes of them cost
