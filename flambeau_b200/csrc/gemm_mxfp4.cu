@@ -330,7 +330,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             const int t = (int)(entry & 0xffffffu);
             w.m0 = t * a.tile;
             w.n_tok = (int)(entry >> 24) * a.tile;
-            w.group = min(a.tile_group[t], a.groups - 1);            // (no weights lie beyond the last group's)
+            w.group = min(a.tile_group[t], a.groups - 1);            // (none lie beyond the last group's: such a tile's rows are NaN)
             w.nt = TILES * ((int)item - i * a.units_n);
             w.kb0 = 0; w.n_kb = a.kb; w.share = 0; w.shares = 1; w.id = 0;
         } else if constexpr (WIDE) {             // token tiles vary fastest: the CTAs that run together share weight tiles
@@ -951,7 +951,7 @@ int prepare(MxArgs& a, CUtensorMap& mx, CUtensorMap& mo, void* scratch, int box_
     a.scale_bytes = atoms_of(a.bn) * ATOM;
     const int most = grouped ? a.bn / a.tile : 0;
     int rc = fb_mxfp4_split_rows(a.rows, a.M, a.K, scratch, (uint8_t*)scratch + parts,
-                                 MxScaleLayout{a.bn, a.scale_bytes, a.tile_group, a.tile, most, a.n_tiles}, stream);
+                                 MxScaleLayout{a.bn, a.scale_bytes, a.tile_group, a.tile, most, a.n_tiles, a.groups}, stream);
     if (rc) return rc;
     rc = fb_tensor_map_bf16(&mx, scratch, 2L * a.M, Kp / 2, Kp / 2, 64, box_rows);       // (bytes, two at a time)
     if (rc) return rc;
@@ -1068,7 +1068,8 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
 }
 
 // The grouped form: W holds `groups` matrices [N, K] in tiles; the M rows of `out` come in tiles of `tile` (a
-// multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are).  Row m is
+// multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are; beyond the last:
+// its products are NaN, and what the activation makes of that).  Row m is
 // X[m], or with row_index X[row_index[m]] (zeros where that is none of the x_rows), with row_share times row_share[row_pair[m]].  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
 FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, int x_rows, const int* row_index, const float* row_share, const int* row_pair,
                                  const void* W, int groups, const int* tile_group, int tile, void* out, int o_dtype,

@@ -218,9 +218,11 @@ split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t*
     const int blocks = Kp / MX_BLOCK, lane = threadIdx.x & 31, first = blockIdx.x * SPLIT_ROWS;
     const int item = blockIdx.y * 256 + threadIdx.x, q = item / blocks, m = first + q, k = (item - q * blocks) * MX_BLOCK;
     int unit, tokens, at, tiles;                         // the scales' tile, its tokens, the first row's place in it, all tiles
+    bool no_group = false;                               // (the tile's group is beyond the weights: its sums are to be NaN)
     if constexpr (GROUPED) {
         const int t = first / layout.tile, g = layout.tile_group[t];
         if (g < 0) return;                               // (rows of tiles without a group are not multiplied, whatever they hold)
+        no_group = g >= layout.groups;
         unit = t;
         int n = 1;
         if (layout.most > 1) {
@@ -262,7 +264,8 @@ split_kernel(const __grid_constant__ MxRows rows, int M, int K, int Kp, uint8_t*
         }
     }
     uint2 one[4], two[4];
-    const uint32_t word = mx_split_block(v, one, two);
+    uint32_t word = mx_split_block(v, one, two);
+    if (GROUPED && no_group) word = 0xffffffffu;
     if (!mine) return;
     uint4* to_first = reinterpret_cast<uint4*>(parts + (size_t)m * Kp + k);
     uint4* to_second = reinterpret_cast<uint4*>(parts + ((size_t)M + m) * Kp + k);

@@ -118,5 +118,6 @@ __device__ __forceinline__ uint4 mx_times(uint4 v, float f) {
 // Where the rows' scales go: [K / 128][token tile][tile_bytes], for a tile of n tokens the first parts as rows 0 .. and the second ones
 // up to 64 tokens as rows n .., else from the next multiple of 128 on, by 128 rows as [lane i][j] words of row 32 j + i.  A tile is
 // `tokens` rows; grouped: up to `most` neighbouring row tiles of `tile` rows of one group, in the place of the first of them.
-struct MxScaleLayout { int tokens, tile_bytes; const int* tile_group; int tile, most, n_tiles; };
+// Rows of a tile whose group is none of the `groups` get scales of 255.
+struct MxScaleLayout { int tokens, tile_bytes; const int* tile_group; int tile, most, n_tiles, groups; };
 int fb_mxfp4_split_rows(const MxRows& rows, int M, int K, void* parts, void* scales, const MxScaleLayout& layout, cudaStream_t stream);

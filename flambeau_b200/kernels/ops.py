@@ -1782,7 +1782,8 @@ class Mxfp4Weight(PackedWeight):
 
     def grouped(self, a, row_index, tile_group, tile: int, out, ctx, activation_name=None, gate=None, row_share=None,
                 row_pair=None) -> None:
-        """grouped_linear, or with `gate` grouped_gated_linear."""
+        """grouped_linear, or with `gate` grouped_gated_linear.  A tile whose group is negative is skipped (its rows of `out` stay),
+        one whose group is beyond the last has products of NaN; a row whose index is none of a's counts as zeros."""
         what = "grouped product"
         if ctx is None:
             raise KernelError(f"{what}: four-bit weights need the step's scratch (ctx)")

@@ -95,3 +95,28 @@ def test_a_row_with_an_infinity_or_a_nan(M, N, K, what):
     for name, out in products(a, codes, scales, ctx):
         assert bool(out[bad].isnan().all()) and torch.equal(out[~bad].double(), want[~bad]), name
     ctx.runtime.check_status()
+
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128])
+def test_a_tile_whose_group_is_none_of_the_weights(tile):
+    """Its rows of the output become NaN, and those of the other tiles are what they are without it."""
+    from flambeau_b200.kernels import ops
+    N, K = 130, 320
+    codes, scales = whole.weight_codes((3, N), K, 7)
+    w, dense = ops.Mxfp4Weight(codes, scales, K), whole.numbers(codes, scales)
+    order = [0, 3, 1, 1, 2 ** 31 - 1, -1, 2, 2, 70]
+    M = tile * len(order)
+    a = whole.rows(M, K, 8)
+    tiles = torch.tensor(order, dtype=torch.int32, device="cuda")
+    of = tiles.repeat_interleave(tile)
+    ctx = step()
+    for index in (None, torch.arange(M, dtype=torch.int32, device="cuda")):
+        for dtype in (torch.float32, torch.bfloat16):
+            out, act = torch.full((M, N), 7.0, dtype=dtype, device="cuda"), torch.full((M, N // 2), 7.0, dtype=dtype, device="cuda")
+            ops.grouped_linear(a, index, w, tiles, tile, out, None, ctx)
+            ops.grouped_gated_linear(a, index, w, tiles, tile, act, "silu", ctx)
+            for g in range(3):
+                assert torch.equal(out[of == g], whole.product(a[of == g], dense[g]).to(dtype)) and bool(act[of == g].isfinite().all())
+            assert bool(out[of > 2].isnan().all()) and bool(act[of > 2].isnan().all())
+            assert bool((out[of < 0] == 7.0).all()) and bool((act[of < 0] == 7.0).all())
+    ctx.runtime.check_status()
