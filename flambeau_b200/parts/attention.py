@@ -123,19 +123,19 @@ class PagedAttention(Mixer):
 
     def own_tensor_specs(self):
         p, init = self.prefix, ("normal", self.init_std)
-        nm = self.names
+        nm, packs = self.names, self._packs_qkv()
         specs = {
-            p + nm["q"]: TensorSpec((self.qw, self.width), init=init),
-            p + nm["k"]: TensorSpec((self.kvw, self.width), init=init),
-            p + nm["o"]: TensorSpec((self.width, self.nh * self.vd), init=init),
+            p + nm["q"]: TensorSpec((self.qw, self.width), init=init, packs=packs),
+            p + nm["k"]: TensorSpec((self.kvw, self.width), init=init, packs=packs),
+            p + nm["o"]: TensorSpec((self.width, self.nh * self.vd), init=init, packs=True),
         }
         if not self.values_from_keys:
-            specs[p + nm["v"]] = TensorSpec((self.vw, self.width), init=init)
+            specs[p + nm["v"]] = TensorSpec((self.vw, self.width), init=init, packs=packs)
         if self.sink:
             specs[p + nm["sink"]] = TensorSpec((self.nh,), init=("normal", 1.0))
         if self.gate:
             specs[p + nm["g"]] = TensorSpec((self.nh * self.vd if self.gate == "element" else self.nh, self.width),
-                                            init=init)
+                                            init=init, packs=packs)
         return specs
 
     def own_bind(self, tensors):
@@ -149,14 +149,18 @@ class PagedAttention(Mixer):
             # rows of zeros up to a multiple of 8, so that the product's float32 rows stay 16-byte aligned
             stack.append(torch.zeros((8 - rows % 8, self.width), dtype=stack[0].dtype, device=stack[0].device))
         qkv = concat_rows(stack)
-        # (query/key norms without the fused kernel multiply with row slices of the weight, which stays a tensor then)
-        self.qkv = Linear(qkv if self.q_norm is not None and not self._fused_norm_kernel() else held(self.runtime, qkv))
+        self.qkv = Linear(held(self.runtime, qkv) if self._packs_qkv() else qkv)
         self.o = Linear(held(self.runtime, tensors[p + nm["o"]]))
         if self.sink:
             self.sinks = tensors[p + nm["sink"]].float().contiguous()      # scores are float32 in both modes
 
     def own_weights(self):
         return [self.qkv.weight, self.o.weight]
+
+    def _packs_qkv(self) -> bool:
+        """Whether the map of queries, keys and values is held in the runtime's weight format: query/key norms without the
+        fused kernel multiply with row slices of the weight, which stays a tensor then."""
+        return self.q_norm is None or self._fused_norm_kernel()
 
     def _wants_norm_kernel(self) -> bool:
         """Whether the mixer needs what only the kernel of _fused_norm_kernel does: a norm of q and k, values of their

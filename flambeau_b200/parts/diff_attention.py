@@ -71,10 +71,10 @@ class DifferentialAttention(Mixer):
     def own_tensor_specs(self):
         p, init = self.prefix, ("normal", self.init_std)
         specs = {
-            p + "q": TensorSpec((self.qw, self.width), init=init),
-            p + "k": TensorSpec((self.kw, self.width), init=init),
-            p + "v": TensorSpec((self.vw, self.width), init=init),
-            p + "o": TensorSpec((self.width, self.nh * self.vd), init=init),
+            p + "q": TensorSpec((self.qw, self.width), init=init, packs=True),
+            p + "k": TensorSpec((self.kw, self.width), init=init, packs=True),
+            p + "v": TensorSpec((self.vw, self.width), init=init, packs=True),
+            p + "o": TensorSpec((self.width, self.nh * self.vd), init=init, packs=True),
         }
         for name in ("lq1", "lk1", "lq2", "lk2"):
             specs[p + name] = TensorSpec((self.kd,), init=("normal", 0.1))
@@ -88,7 +88,7 @@ class DifferentialAttention(Mixer):
             specs[p + "q.norm"] = TensorSpec((self.kd,), init=("one_plus_normal", 0.1))
             specs[p + "k.norm"] = TensorSpec((self.kd,), init=("one_plus_normal", 0.1))
         if self.head_gate:
-            specs[p + "g"] = TensorSpec((self.nh, self.width), init=init)
+            specs[p + "g"] = TensorSpec((self.nh, self.width), init=init, packs=True)
         return specs
 
     def own_bind(self, tensors):

@@ -41,9 +41,9 @@ class GatedMLP(FeedForward):
         p, init = self.prefix, ("normal", self.init_std)
         gate, up, down = self.names
         return {
-            p + gate: TensorSpec((self.inner, self.width), init=init),
-            p + up: TensorSpec((self.inner, self.width), init=init),
-            p + down: TensorSpec((self.width, self.inner), init=init),
+            p + gate: TensorSpec((self.inner, self.width), init=init, packs=True),
+            p + up: TensorSpec((self.inner, self.width), init=init, packs=True),
+            p + down: TensorSpec((self.width, self.inner), init=init, packs=True),
         }
 
     def own_bind(self, tensors):
@@ -108,8 +108,8 @@ class PlainMLP(FeedForward):
     def own_tensor_specs(self):
         p, init = self.prefix, ("normal", self.init_std)
         up, down = self.names
-        return {p + up: TensorSpec((self.inner, self.width), init=init),
-                p + down: TensorSpec((self.width, self.inner), init=init)}
+        return {p + up: TensorSpec((self.inner, self.width), init=init, packs=True),
+                p + down: TensorSpec((self.width, self.inner), init=init, packs=True)}
 
     def own_bind(self, tensors):
         up, down = self.names

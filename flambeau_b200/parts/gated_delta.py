@@ -76,7 +76,7 @@ class GatedDeltaRule(Mixer):
             p + "A_log": TensorSpec((self.H,), init=("normal", 0.5)),
             p + "dt_bias": TensorSpec((self.H * (self.dk if self.by_channel else 1),), init=("normal", 0.5)),
             p + "norm": TensorSpec((self.dv,), init=("one_plus_normal", 0.1)),
-            p + "o": TensorSpec((self.width, self.vw), init=init),
+            p + "o": TensorSpec((self.width, self.vw), init=init, packs=True),
         }
         if self.by_channel:
             specs[p + "a1"] = TensorSpec((self.rank, self.width), init=init, free_axes=(0,))

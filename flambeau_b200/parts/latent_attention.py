@@ -66,20 +66,20 @@ class LatentAttention(Mixer):
         specs = {
             p + "uk": TensorSpec((self.H * self.d, self.Rc), init=init),
             p + "uv": TensorSpec((self.H * self.e, self.Rc), init=init),
-            p + "o": TensorSpec((self.width, self.H * self.e), init=init),
+            p + "o": TensorSpec((self.width, self.H * self.e), init=init, packs=True),
         }
         if self.Rq:
-            specs[p + "dq"] = TensorSpec((self.Rq, self.width), init=init)
+            specs[p + "dq"] = TensorSpec((self.Rq, self.width), init=init, packs=True)
             specs[p + "dq.norm"] = TensorSpec((self.Rq,), init=norm)
-            specs[p + "uq"] = TensorSpec((self.H * (self.d + self.r), self.Rq), init=init)
+            specs[p + "uq"] = TensorSpec((self.H * (self.d + self.r), self.Rq), init=init, packs=True)
         else:
-            specs[p + "q"] = TensorSpec((self.H * (self.d + self.r), self.width), init=init)
+            specs[p + "q"] = TensorSpec((self.H * (self.d + self.r), self.width), init=init, packs=True)
         if self.sink:
             specs[p + "sink"] = TensorSpec((self.H,), init=("normal", 1.0))
         if self.gate:
-            specs[p + "g"] = TensorSpec((self.H * self.e, self.width), init=init)
+            specs[p + "g"] = TensorSpec((self.H * self.e, self.width), init=init, packs=True)
         if not self.shares_latent:
-            specs[p + "dkv"] = TensorSpec((self.hd, self.width), init=init)
+            specs[p + "dkv"] = TensorSpec((self.hd, self.width), init=init, packs=True)
             specs[p + "dkv.norm"] = TensorSpec((self.Rc,), init=norm)
         return specs
 

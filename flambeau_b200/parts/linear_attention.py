@@ -48,7 +48,7 @@ class GatedLinearAttention(Mixer):
             p + "k": TensorSpec((self.qk, self.width), init=init),
             p + "v": TensorSpec((self.vw, self.width), init=init),
             p + "g": TensorSpec((self.vw, self.width), init=init),
-            p + "o": TensorSpec((self.width, self.vw), init=init),
+            p + "o": TensorSpec((self.width, self.vw), init=init, packs=True),
             p + "norm": TensorSpec((self.dv,), init=("one_plus_normal", 0.1)),
             p + "a1": TensorSpec((self.rank, self.width), init=init, free_axes=(0,)),
             p + "a2": TensorSpec((self.qk, self.rank), init=("normal", 0.5), free_axes=(1,)),

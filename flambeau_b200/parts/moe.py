@@ -102,15 +102,15 @@ class RoutedExperts(FeedForward):
         specs = {}
         for e in range(self.E):
             if self.gated:
-                specs[f"{p}e{e}.gate"] = TensorSpec((self.inner, self.width), init=init)
-            specs[f"{p}e{e}.up"] = TensorSpec((self.inner, self.width), init=init)
-            specs[f"{p}e{e}.down"] = TensorSpec((self.width, self.inner), init=init)
+                specs[f"{p}e{e}.gate"] = TensorSpec((self.inner, self.width), init=init, packs=True)
+            specs[f"{p}e{e}.up"] = TensorSpec((self.inner, self.width), init=init, packs=True)
+            specs[f"{p}e{e}.down"] = TensorSpec((self.width, self.inner), init=init, packs=True)
         specs[p + "router"] = TensorSpec((self.outputs, self.width), init=("normal", self.router_std))
         if self.router_bias:
             specs[p + self.bias_name] = TensorSpec((self.outputs,), init=("normal", 0.1))
         if self.shared_inner:
-            specs[p + "shared.up"] = TensorSpec((self.shared_inner, self.width), init=init)
-            specs[p + "shared.down"] = TensorSpec((self.width, self.shared_inner), init=init)
+            specs[p + "shared.up"] = TensorSpec((self.shared_inner, self.width), init=init, packs=True)
+            specs[p + "shared.down"] = TensorSpec((self.width, self.shared_inner), init=init, packs=True)
         if self.token_gate:
             specs[p + "shared.sg"] = TensorSpec((1, self.width), init=init)
         return specs

@@ -29,12 +29,14 @@ class TensorSpec:
     file does not have it (tied embeddings).
     free_axes: axes whose size the weight file decides (a size that no configuration key gives); `shape` holds what
     the random-weights mode draws there, and the part reads the real size from the tensor it is bound to.
+    packs: a large map, which the part holds in the runtime's weight format (parts.linear.held).
     """
     shape: tuple
     kind: str = "float"
     init: tuple = ("normal", 0.02)
     alias_of: Optional[str] = None
     free_axes: tuple = ()
+    packs: bool = False
 
 
 @dataclass(frozen=True)

@@ -78,13 +78,14 @@ class FolderTensors:
         """name -> device tensor for the given names."""
         out = {}
         rt = self.runtime
+        packed = {n for n in names if self.specs[n].packs} if getattr(rt, "weight_format", "stored") != "stored" else set()
         for name in names:
             src = self.source[name]
             t = self._shared.get(src)
             if t is None:
                 raw = self.files.tensor(src)
                 want = torch.int32 if self.specs[name].kind == "int" else rt.weight_dtype(raw.dtype)
-                if want == torch.float32 and not rt.full_precision and raw.dim() >= 2 and not self._warned:
+                if want == torch.float32 and not rt.full_precision and raw.dim() >= 2 and name not in packed and not self._warned:
                     self._warned = True
                     warnings.warn(f"'{src}' is stored in 32-bit and stays so in bfloat16 mode: products with it "
                                   f"run on the float32 FMA kernel, far below the tensor cores' rate; store linear "
