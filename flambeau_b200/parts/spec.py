@@ -29,7 +29,8 @@ class TensorSpec:
     file does not have it (tied embeddings).
     free_axes: axes whose size the weight file decides (a size that no configuration key gives); `shape` holds what
     the random-weights mode draws there, and the part reads the real size from the tensor it is bound to.
-    packs: a large map, which the part holds in the runtime's weight format (parts.linear.held).
+    packs: a large map, which the part holds in the runtime's weight format (parts.linear.held): where that is not the
+    stored one, the tensor comes with the bits that it is stored with, whatever the engine's dtype.
     """
     shape: tuple
     kind: str = "float"

@@ -70,21 +70,25 @@ class FolderTensors:
         counts: dict = {}
         for src in self.source.values():
             counts[src] = counts.get(src, 0) + 1
-        self._shared = {src: None for src, c in counts.items() if c > 1}
-        self._shared.update({self.source[name]: None for name in shared})
+        self._shared = {src: {} for src, c in counts.items() if c > 1}              # by the dtype that it is held in
+        self._shared.update({self.source[name]: {} for name in shared})
         self._warned = False
 
     def fetch(self, names) -> dict:
         """name -> device tensor for the given names."""
         out = {}
         rt = self.runtime
+        # maps that the runtime packs are quantised from the bits that they are stored with: from bfloat16 where all of a
+        # part's are stored so, else from float32 (a part may stack them)
         packed = {n for n in names if self.specs[n].packs} if getattr(rt, "weight_format", "stored") != "stored" else set()
+        narrow = not rt.full_precision and all(self.files.dtype(self.source[n]) == torch.bfloat16 for n in packed)
         for name in names:
             src = self.source[name]
-            t = self._shared.get(src)
+            want = torch.int32 if self.specs[name].kind == "int" else \
+                (torch.bfloat16 if narrow else torch.float32) if name in packed else rt.weight_dtype(self.files.dtype(src))
+            t = self._shared.get(src, {}).get(want)
             if t is None:
                 raw = self.files.tensor(src)
-                want = torch.int32 if self.specs[name].kind == "int" else rt.weight_dtype(raw.dtype)
                 if want == torch.float32 and not rt.full_precision and raw.dim() >= 2 and name not in packed and not self._warned:
                     self._warned = True
                     warnings.warn(f"'{src}' is stored in 32-bit and stays so in bfloat16 mode: products with it "
@@ -92,7 +96,7 @@ class FolderTensors:
                                   f"weights in bfloat16 (or float16) for serving")
                 t = raw.to(device=rt.device, dtype=want).contiguous()
                 if src in self._shared:
-                    self._shared[src] = t
+                    self._shared[src][want] = t
             out[name] = t
         return out
 
