@@ -36,6 +36,8 @@
 #include "tensor_map.cuh"
 #include "umma.cuh"
 
+#include <limits.h>
+
 namespace {
 
 constexpr int A_COLS = MX_COLS / 4;               // tensor-memory columns of a stage's weights, then of their scales
@@ -832,6 +834,13 @@ constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 6000;
 struct Cut { int grid, segments; };
 // What was last asked for in a place of a thread's table, and the answer to it (neither allocates nor locks).
 constexpr int REMEMBERED = 256;
+template <int N> constexpr uint32_t place_of(const int (&key)[N]) {
+    uint32_t h = 0;                              // (which may wrap; a constant expression, as below, may not overflow an int)
+    for (int i = 0; i < N; ++i) h = h * 37u + (uint32_t)key[i];
+    return h % REMEMBERED;
+}
+constexpr int FURTHEST[7] = {INT_MAX, ANY, -ANY, INT_MAX, INT_MIN, 1, INT_MAX};
+static_assert(place_of(FURTHEST) < REMEMBERED, "every question has a place");
 template <typename Value, int N> struct Remembered {
     int asked[N];
     Value value;
@@ -845,8 +854,9 @@ template <typename Value, int N> struct Remembered {
 };
 Cut cut_of(int tiles_n, int kb, int limit, bool join) {
     static thread_local Remembered<Cut, 4> known[REMEMBERED];                // (counting through the tiles takes microseconds)
-    Remembered<Cut, 4>& was = known[(uint32_t)(tiles_n + 37 * kb + 101 * limit + join) % REMEMBERED];
-    if (was.is({tiles_n, kb, join ? -limit : limit, fb_sm_count()})) return was.value;
+    const int key[4] = {tiles_n, kb, join ? -limit : limit, fb_sm_count()};
+    Remembered<Cut, 4>& was = known[place_of(key)];
+    if (was.is(key)) return was.value;
     const long most = ((long)tiles_n * kb + LEAST_ITEMS - 1) / LEAST_ITEMS, slots = fb_sm_count();
     long grid = most < slots ? most : slots;
     const long even = grid / tiles_n * tiles_n;
@@ -906,8 +916,9 @@ constexpr int MOST_SPLITS = 16;
 
 Plan plan_wide(int M, int N, int kb, int max_splits, int n_counters, bool slabs) {
     static thread_local Remembered<Plan, 7> known[REMEMBERED];                               // (looking for it takes microseconds)
-    Remembered<Plan, 7>& was = known[(uint32_t)(M + 37 * N + 101 * kb + 211 * max_splits + slabs) % REMEMBERED];
-    if (was.is({M, N, kb, max_splits, n_counters, slabs ? 1 : 0, fb_sm_count()})) return was.value;
+    const int key[7] = {M, N, kb, max_splits, n_counters, slabs ? 1 : 0, fb_sm_count()};
+    Remembered<Plan, 7>& was = known[place_of(key)];
+    if (was.is(key)) return was.value;
     return was.value = cheapest(M, N, kb, max_splits, SHARE_FLOATS, n_counters, slabs);
 }
 
@@ -971,7 +982,7 @@ int check_operands(const void* X, long long lda, const void* W, const void* out,
     FB_REQUIRE(!gate.act || (fb_gate_known(gate) && N % 2 == 0 && !plain_act),
                "gemm_mxfp4: a gate needs a known activation, an even number of stacked rows and no plain activation beside it");
     FB_REQUIRE(fb_plain_act_known(plain_act), "gemm_mxfp4: unknown activation code %d", plain_act);
-    FB_REQUIRE((long)((N + MX_ROWS - 1) / MX_ROWS) * ((K + MX_COLS - 1) / MX_COLS) < (1L << 24), "gemm_mxfp4: too many weights, %d x %d", N, K);
+    FB_REQUIRE(((long)N + MX_ROWS - 1) / MX_ROWS * (((long)K + MX_COLS - 1) / MX_COLS) < (1L << 24), "gemm_mxfp4: too many weights, %d x %d", N, K);
     FB_REQUIRE(lda >= K && ldo >= (gate.act ? N / 2 : N), "gemm_mxfp4: a row stride is shorter than its row");
     FB_REQUIRE(((uintptr_t)X & 1) == 0 && W && ((uintptr_t)W & 15) == 0 && status,
                "gemm_mxfp4: unaligned rows or weights, or no status word");

@@ -339,12 +339,12 @@ FB_API int fb_dequantize_mxfp4(const void* codes, const void* scales, long long 
 
 // Bytes of one matrix [N, K] in tiles.
 FB_API long long fb_mxfp4_tile_bytes(int N, int K) {
-    return (long long)((N + MX_ROWS - 1) / MX_ROWS) * ((K + MX_COLS - 1) / MX_COLS) * MX_TILE_BYTES;
+    return ((long long)N + MX_ROWS - 1) / MX_ROWS * (((long long)K + MX_COLS - 1) / MX_COLS) * MX_TILE_BYTES;
 }
 
 // `groups` matrices [N, K] from rows (codes, scales as fb_quantize_mxfp4 writes them) into tiles.
 FB_API int fb_mxfp4_tiles(const void* codes, const void* scales, int groups, int N, int K, void* tiles, cudaStream_t stream) {
-    FB_REQUIRE(groups > 0 && N > 0 && K > 0 && groups <= 65535 && N <= 65535 * MX_ROWS, "mxfp4_tiles: bad sizes");
+    FB_REQUIRE(groups > 0 && N > 0 && K > 0 && groups <= 65535 && N <= 65535 * MX_ROWS && K <= (1 << 30), "mxfp4_tiles: bad sizes");
     FB_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)tiles & 15) == 0, "mxfp4_tiles: operands must be 16-byte aligned");
     const int blocks = (K + MX_BLOCK - 1) / MX_BLOCK, tiles_k = (K + MX_COLS - 1) / MX_COLS;
     fb_launch(tiles_kernel, dim3(4 * tiles_k, (N + MX_ROWS - 1) / MX_ROWS, groups), dim3(128), 0, stream, (const uint8_t*)codes,
