@@ -1618,6 +1618,14 @@ def hc_step(streams: torch.Tensor, y, n_partials: int, partial_stride: int, mix,
 MXFP4_BLOCK = 32          # numbers that share a scale
 
 
+def _stream_on(device: int, what: str) -> int:
+    """torch's current stream, which has to be one of that device: a kernel of another one cannot follow its addresses."""
+    here = torch.cuda.current_device()
+    if here != device:
+        raise KernelError(f"{what}: the tensors are on cuda:{device}, the current device is cuda:{here}")
+    return _raw_stream(here) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
 def quantize_mxfp4(x: torch.Tensor) -> tuple:
     """(codes, scales) of x [..., columns], float32 or bfloat16 (a 2-d x may have rows apart, more dimensions are contiguous).
 
@@ -1637,8 +1645,8 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple:
     stride = _rows(flat) if rows > 1 or flat.stride(1) != 1 else columns
     blocks = -(-columns // MXFP4_BLOCK)
     codes, scales = x.new_empty((*lead, 16 * blocks), dtype=torch.uint8), x.new_empty((*lead, blocks), dtype=torch.uint8)
-    check(lib().fb_quantize_mxfp4(flat.data_ptr(), code, stride, rows, columns, codes.data_ptr(), scales.data_ptr(), _stream()),
-          "quantize_mxfp4")
+    check(lib().fb_quantize_mxfp4(flat.data_ptr(), code, stride, rows, columns, codes.data_ptr(), scales.data_ptr(),
+                                  _stream_on(x.get_device(), "quantize_mxfp4")), "quantize_mxfp4")
     return codes, scales
 
 
@@ -1650,6 +1658,8 @@ def _mxfp4_blocks(codes: torch.Tensor, scales: torch.Tensor, columns: int, what:
             or (*codes.shape[:-1], blocks) != tuple(scales.shape) or codes.shape[-1] != 16 * blocks:
         raise KernelError(f"{what}: uint8 codes [..., {16 * blocks}] and scales [..., {blocks}] wanted for {columns} columns, not "
                           f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+    if codes.device != scales.device:
+        raise KernelError(f"{what}: codes on {codes.device}, scales on {scales.device}")
     if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
         raise KernelError(f"{what}: codes and scales must be contiguous, codes on a 16-byte border")
     return blocks
@@ -1661,7 +1671,7 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, columns: int, dt
     out = codes.new_empty((*codes.shape[:-1], columns), dtype=dtype)
     code = dtype_code(out)
     check(lib().fb_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), scales.numel() // blocks, int(columns), out.data_ptr(), code,
-                                    int(columns), _stream()), "dequantize_mxfp4")
+                                    int(columns), _stream_on(codes.get_device(), "dequantize_mxfp4")), "dequantize_mxfp4")
     return out
 
 
@@ -1686,11 +1696,11 @@ class Mxfp4Weight(PackedWeight):
         self._outputs, self._inputs = int(outputs), int(inputs)
         if groups < 1 or outputs < 1:
             raise KernelError("mxfp4 weight: no outputs")
-        self.device = codes.device
+        self.device, self._index = codes.device, codes.get_device()
         self.tiles = torch.empty(groups * lib().fb_mxfp4_tile_bytes(outputs, int(inputs)), dtype=torch.uint8, device=codes.device)
         self._tiles, self._scratch = self.tiles.data_ptr(), {}
         check(lib().fb_mxfp4_tiles(codes.data_ptr(), scales.data_ptr(), groups, outputs, int(inputs), self.tiles.data_ptr(),
-                                   _stream()), "mxfp4_tiles")
+                                   _stream_on(self._index, "mxfp4 weight")), "mxfp4_tiles")
 
     @classmethod
     def from_dense(cls, weight: torch.Tensor) -> "Mxfp4Weight":
@@ -1717,7 +1727,7 @@ class Mxfp4Weight(PackedWeight):
             raise KernelError(f"{what}: shapes a{tuple(rows)} w{tuple(self.shape)} out{tuple(outs)} do not agree")
         if a.dtype is not torch.bfloat16:
             raise KernelError(f"{what}: four-bit weights multiply bfloat16 rows, not {a.dtype}")
-        if a.device != self.device or out.device != self.device:
+        if a.get_device() != self._index or out.get_device() != self._index:
             raise KernelError(f"{what}: the weight is on {self.device}, the rows on {a.device}, the output on {out.device}")
         dtype_code(out)
         return rows[0], N, K
@@ -1729,6 +1739,9 @@ class Mxfp4Weight(PackedWeight):
         if ws is None:
             raise KernelError(f"{what}: four-bit weights need the step's scratch (ctx)")
         counters = ws.counters
+        if counters.get_device() != self._index:
+            raise KernelError(f"{what}: the weight is on {self.device}, the step's scratch on {counters.device}")
+        stream = _stream_on(self._index, what)
         nbytes = self._scratch_bytes(M, counters.numel(), slabs is not None, 0)
         splits = ctypes.c_int(1) if slabs is not None else None
         mark = ws.mark()
@@ -1736,7 +1749,7 @@ class Mxfp4Weight(PackedWeight):
             check(lib().fb_gemm_mxfp4(a.data_ptr(), _rows(a), self._tiles, out.data_ptr(), _CODES[out.dtype], _rows(out),
                                       slabs.stride(0) if slabs is not None else 0, slabs.shape[0] if slabs is not None else 0,
                                       ctypes.byref(splits) if splits is not None else None, M, N, K, *gate, plain_act, accumulate, counters.data_ptr(), counters.numel(),
-                                      ws.reserve(nbytes) if nbytes else 0, nbytes, ctx.runtime.status.data_ptr(), _stream()),
+                                      ws.reserve(nbytes) if nbytes else 0, nbytes, ctx.runtime.status.data_ptr(), stream),
                   "gemm_mxfp4", (M, N, K))
         finally:
             ws.release(mark)
@@ -1808,6 +1821,10 @@ class Mxfp4Weight(PackedWeight):
         self._operands(a, out, N // 2 if gate is not None else N, what, indexed=row_index is not None)
         gate_args = gate_arguments(gate) if gate is not None else (0, 0.0, 0.0)
         ws = ctx.ws
+        for t in (tile_group, row_index, row_share, row_pair, ws.counters):
+            if t is not None and t.get_device() != self._index:
+                raise KernelError(f"{what}: the weight is on {self.device}, an index, shares or the step's scratch on {t.device}")
+        stream = _stream_on(self._index, what)
         nbytes = self._scratch_bytes(M, 0, False, int(tile))
         mark = ws.mark()
         try:
@@ -1815,6 +1832,6 @@ class Mxfp4Weight(PackedWeight):
                                               self._tiles, self.shape[0], tile_group.data_ptr(), int(tile), out.data_ptr(),
                                               dtype_code(out), _rows(out), M, N, K, *gate_args,
                                               plain_activation_code(activation_name), ws.reserve(nbytes), nbytes,
-                                              ctx.runtime.status.data_ptr(), _stream()), "gemm_mxfp4_grouped", (M, N, K))
+                                              ctx.runtime.status.data_ptr(), stream), "gemm_mxfp4_grouped", (M, N, K))
         finally:
             ws.release(mark)
