@@ -53,6 +53,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* st
     }
 }
 
+// Where a wait ran out, what the block has under way (copies into its shared memory, MMAs that read it) is given this long to end before
+// the block frees its tensor memory and returns.
+constexpr unsigned long long FB_SETTLE_NS = 10000000ull;         // 10 ms
+__device__ __forceinline__ void fb_settle() {
+    for (const unsigned long long t0 = global_ns(); global_ns() - t0 < FB_SETTLE_NS;) __nanosleep(1000);
+}
+
 // 4 or 16 bytes from global to shared memory (both aligned to as many) by a thread's own asynchronous copies, which are
 // counted in groups: cp_async_wait<LEFT> waits until all but the thread's LEFT newest groups have landed.
 __device__ __forceinline__ void cp_async4(void* dst, const void* src) {

@@ -809,6 +809,7 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     tmem_fence_before();
     __syncthreads();
     if (warp == 3) {
+        if (bailed()) fb_settle();
         tmem_fence_after();
         tmem_dealloc(tmem, TMEM);
     }
