@@ -825,7 +825,8 @@ int segments_of(long tiles_n, long kb, long grid) {           // the most stretc
     }
     return (int)most;
 }
-// CTAs, one an SM, each with a few tiles at least, and the most stretches that they cut a row tile into: as many CTAs as leave no
+// CTAs, one an SM, each with a few tiles at least or a row tile (32 x 2,048 x 128: 9.3 us where a CTA took four row tiles of one, 5.1
+// with one each), and the most stretches that they cut a row tile into: as many CTAs as leave no
 // more than `limit`, or fewer that cut every row tile alike, down to two thirds of them: a CTA then has one unit, and SMs are left for
 // the next kernel (32 x 4,096 x 14,336 to slabs: 148 stretches 16.0 us, 128 quarters 12.2; 8 rows 10.6 and 10.0, added 13.9 and 11.6;
 // 32 x 6,400 x 4,096 12.9 and 7.5 in 100 halves; with 80 of 148 one row of 10,240 x 8,192 took 13.8 us instead of 12.1).  Where shares have to meet (`join`), row tiles stay whole if they come out even and the longest stretch and the
@@ -858,8 +859,10 @@ Cut cut_of(int tiles_n, int kb, int limit, bool join) {
     const int key[4] = {tiles_n, kb, join ? -limit : limit, fb_sm_count()};
     Remembered<Cut, 4>& was = known[place_of(key)];
     if (was.is(key)) return was.value;
-    const long most = ((long)tiles_n * kb + LEAST_ITEMS - 1) / LEAST_ITEMS, slots = fb_sm_count();
-    long grid = most < slots ? most : slots;
+    const long slots = fb_sm_count();
+    long grid = ((long)tiles_n * kb + LEAST_ITEMS - 1) / LEAST_ITEMS;
+    if (grid < tiles_n) grid = tiles_n;
+    if (grid > slots) grid = slots;
     const long even = grid / tiles_n * tiles_n;
     if (even * 3 >= grid * 2) grid = even;
     int segments = segments_of(tiles_n, kb, grid);
