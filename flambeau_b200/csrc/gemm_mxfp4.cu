@@ -184,6 +184,7 @@ __device__ __forceinline__ float silu_times(float g, float u) {
 
 // The epilogue's code is walked a few times a tile only, so that its instructions come from far: every 128 bytes of them cost
 // about as much as ten of the instructions.  What is seldom wanted is kept out of its straight way.
+__device__ __noinline__ void let_end() { fb_settle(); }
 __device__ __noinline__ float gate_slowly(const FbGate& gate, float g, float u) { return fb_gate_times(gate, g, u); }
 __device__ __noinline__ float act_slowly(int act, float z) { return fb_plain_act(act, z); }
 template <int N> __device__ __forceinline__ void gate_all(const FbGate& gate, float (&g)[N], const float (&u)[N]) {
@@ -754,7 +755,10 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             tmem_fence_before();
             mbar_arrive(smem_u32(&acc_empty[b]));
             }
-            if (stop) break;
+            if (stop) {                          // (else the sums of every unit have come, and with them all copies)
+                let_end();
+                break;
+            }
             u = following;
         }
         if (WIDE && leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");        // the boxes it sent are in memory
@@ -809,7 +813,6 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     tmem_fence_before();
     __syncthreads();
     if (warp == 3) {
-        if (bailed()) fb_settle();
         tmem_fence_after();
         tmem_dealloc(tmem, TMEM);
     }

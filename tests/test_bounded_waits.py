@@ -5,12 +5,14 @@ from flambeau_b200.kernels.build import CSRC
 
 
 def test_the_product_with_four_bit_weights_lets_what_is_under_way_end():
-    """Copies and MMAs of a block that gives up still use its shared and tensor memory: it waits for them, with a limit, before it
-    frees the columns; the warp that frees them is the block's last to return."""
+    """Copies and MMAs of a block that gives up still use its shared and tensor memory.  The epilogue is the last to be told: it
+    either has had the sums of every unit, and so every copy, or it waits, with a limit, ahead of the block's last barrier, behind
+    which the columns are freed."""
     text = re.sub(r"//[^\n]*", "", (CSRC / "gemm_mxfp4.cu").read_text())
-    end = text[text.rindex("__syncthreads();", 0, text.index("tmem_dealloc(")):]
-    assert re.search(r"if \(bailed\(\)\) fb_settle\(\);.*?tmem_dealloc\(", end, re.S)
-    waits = text[text.index("gemm_mxfp4_kernel("):]
-    assert len(re.findall(r"\*bail = 1", waits)) >= 6, "every role says when it gives up"
-    settle = (CSRC / "async_copy.cuh").read_text()
-    assert re.search(r"global_ns\(\) - t0 < FB_SETTLE_NS", settle)
+    kernel = text[text.index("gemm_mxfp4_kernel("):]
+    assert len(re.findall(r"\*bail = 1", kernel)) >= 6, "every role says when it gives up"
+    stop, settled, freed = kernel.index("stop = *flag == 2;"), kernel.index("let_end();"), kernel.index("tmem_dealloc(")
+    assert re.search(r"if \(stop\) \{\s*let_end\(\);\s*break;", kernel)
+    assert stop < settled < kernel.rindex("__syncthreads();", 0, freed) < freed
+    assert "void let_end() { fb_settle(); }" in text
+    assert re.search(r"global_ns\(\) - t0 < FB_SETTLE_NS", (CSRC / "async_copy.cuh").read_text())
