@@ -3,6 +3,7 @@
 
     python bench.py [--gpus 1] [--steps K] [--warmup W] [--impl ours|reference]
                     [--shape 7b|nemo12b|small24b] [--only headline|mixed|shapes] [--batch B] [--context C] [--layers L]
+                    [--weights stored|mxfp4]
 
 The same program as `flambeau bench`; what it measures, how, and the keys of the line are described in
 flambeau_b200/measure/bench.py.  Default run: the Mistral-7B-v0.1 shape with random bfloat16 weights, decode at

@@ -28,6 +28,9 @@ A "step" is one decode step.  It prints ONE JSON line:
   shapes     the Mistral-Small-24B shape: decode at batch 1 / 8 / 64 with 4,096-token contexts and a 2,048-token
              prefill, each with its roofline fraction
 
+`--weights mxfp4` runs the headline, mixed and shapes parts with the large maps' weights in four bits (the line says so in its
+config; the table of kernels, whose classes are those of stored weights, is left out).
+
 `--only zedivik` is a line of its own (not part of the default run): the Zedivik design beside Mistral at equal
 size, decode and prefill tokens a second and the kernels that differ (flambeau_b200/measure/compare.py).
 `--only nodepel` likewise: the Nodepel design beside Mistral (flambeau_b200/measure/compare_nodepel.py; --sizes 1b,7b).
@@ -88,6 +91,7 @@ def main(argv=None) -> int:
     ap.add_argument("--context", type=int, default=None, help="tokens per sequence (default: the shape's)")
     ap.add_argument("--layers", type=int, default=None, help="fewer layers than the shape has (sizes unchanged)")
     ap.add_argument("--prefill-tokens", type=int, default=2048)
+    ap.add_argument("--weights", choices=["stored", "mxfp4"], default="stored", help="how the large maps hold their weights")
     ap.add_argument("--skip-points", action="store_true", help="do not measure batch 1 and 64")
     ap.add_argument("--only", choices=["all", "headline", "mixed", "shapes", "timeline", "mma-issue", "zedivik", "nodepel", "fegizen", "tubepel",
                                       "saropel", "sisadra"],
@@ -140,7 +144,8 @@ def main(argv=None) -> int:
         cache_tokens = max(max_batch * per_seq + 512, prefill_tokens + PAGE)
         engine = Engine.from_config(cfg, seed=0, options=EngineOptions(
             dtype="bfloat16", page_size=PAGE, cache_tokens=cache_tokens, max_requests=max_batch,
-            max_step_tokens=max(prefill_tokens, max_batch), max_seq_len=min(context + 4096, cfg.max_position_embeddings)))
+            max_step_tokens=max(prefill_tokens, max_batch), max_seq_len=min(context + 4096, cfg.max_position_embeddings),
+            weights=args.weights))
         workloads.randomise_cache(engine)
         return cfg, engine
 
@@ -303,7 +308,7 @@ def main(argv=None) -> int:
             say("attention check and kernel sections")
             check = workloads.attention_check(engine, args.batch, context, gen)
             kernels = {}
-            if args.only == "all":
+            if args.only == "all" and args.weights == "stored":
                 ids = workloads.seat(engine, [context] * args.batch)
                 entries = [Entry(r, [int(torch.randint(0, cfg.vocab_size, (1,), generator=gen))], [0]) for r in ids]
                 sections = workloads.kernel_sections(engine, entries, cfg)
@@ -340,6 +345,8 @@ def main(argv=None) -> int:
                              "frac": round(d["frac"], 4), "bytes_per_step": int(d["bytes"]), "peak_source": tag},
                 "points": points, "check": check, "kernels": kernels,
             }
+            if args.weights != "stored":
+                line["config"]["weights"] = args.weights
             engine = None
             free_device_memory()
 
@@ -354,7 +361,7 @@ def main(argv=None) -> int:
             say(f"building {nemo.name}, {ncfg.num_hidden_layers} layers")
             engine = Engine.from_config(ncfg, seed=0, options=EngineOptions(
                 dtype="bfloat16", page_size=PAGE, cache_tokens=int(0.75 * demand) // PAGE * PAGE, max_requests=n_req,
-                max_step_tokens=ubatch, max_seq_len=hi + new + PAGE))
+                max_step_tokens=ubatch, max_seq_len=hi + new + PAGE, weights=args.weights))
             say("mixed workload: warm-up")
             workloads.mixed_requests(engine, n_requests=4, prompt_range=(lo, 600), chunk=chunk, ubatch=ubatch,
                                      decode_tokens=8, temperature=0.7, seed=99)        # warm-up

@@ -81,3 +81,11 @@ def test_maps_of_one_part_come_in_one_dtype(tmp_path, kinds):
     for n, t in stored.items():
         if is_map(n):
             assert got[n].dtype == want and torch.equal(got[n].float(), t.float())
+
+
+def test_the_benchmark_takes_the_weight_format(capsys):
+    from flambeau_b200.cli import main
+    assert main(["bench", "--gpus", "4", "--weights", "mxfp4"]) == 2
+    assert "one GPU" in capsys.readouterr().out
+    with pytest.raises(SystemExit):
+        main(["bench", "--weights", "int4"])
