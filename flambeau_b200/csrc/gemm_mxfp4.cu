@@ -14,10 +14,10 @@
 // parts side by side), and decoding is moving bits (3 instructions for eight), since the scales go to the tensor core as they are.
 //
 // Layout.  A CTA owns 128 output features x a tile of tokens ("swap-AB": the weight is the 128-row operand, the tokens are N).  A stage
-// is 128 of K (256 up to 32 tokens): one bulk copy brings a weight tile as it lies in memory, groups of four warps take the stages in turn and decode, a
-// thread a feature, into tensor memory, where the MMA takes its A operand and both operands' scales from; the rows' parts, made
-// once for all CTAs by a kernel of their own, come by TMA (K-major, 128-byte swizzle), their scales by tcgen05.cp.  Up to 64 tokens the
-// two parts are N's two halves, which the epilogue adds; with more they are two instructions into one accumulator.
+// is 128 of K (256 up to 32 tokens): one bulk copy brings a weight tile as it lies in memory, groups of four warps take the stages in
+// turn and decode, a thread a feature, into tensor memory, where the MMA takes its A operand and both operands' scales from; the rows'
+// parts, made once for all CTAs by a kernel of their own, come by TMA (K-major, 128-byte swizzle), their scales by tcgen05.cp.  Up to
+// 64 tokens the two parts are N's two halves, which the epilogue adds; with more they are two instructions into one accumulator.
 //
 // Forms.  Few (up to 8 tokens, the CTA splits the rows itself) and narrow (up to 32): the tiles of all row tiles form one line that the
 // CTAs cut into equal stretches.  Wide: token tiles of up to 64 or 128, the output through shared memory.  Shares of K go to slabs
@@ -27,10 +27,11 @@
 // full[s]: a stage's rows (by bytes) and its decoded weights (by arrivals) are there; done[s]: its MMAs are.  Two accumulators, so that
 // the epilogue of one unit overlaps the products of the next.  Every mbarrier wait is bounded as in gemm_tc.cu.
 //
-// What bounds it.  A few rows: instructions.  Decoding a tile takes 150 of a scheduler's slots of the 370 cycles that HBM has it
-// under way, its barriers and the thread that issues MMAs another 100; before that a launch and the way from the first weights to the
-// first MMA, 3 to 4 us (8 x 28,672 x 4,096: 13.8 us in a graph, 69% of HBM's rate).  Many rows: the MMAs, 512 cycles for 128 x 128 x
-// 128 in two parts, at the clock that the power limit leaves (2,048 x 28,672 x 4,096: 353 us in bursts at 1.63 GHz, 413 at 1.35).
+// What bounds it.  A few rows: a stage's way through waits, decoding, barriers and MMAs.  A tile takes 166 of a scheduler's issue
+// slots in all, 40% of those of the SMs at work (profiled), where HBM has it under way for 370 cycles; before that a launch and the way
+// from the first weights to the first MMA, 3 to 4 us (8 x 28,672 x 4,096: 13.9 us in a graph, 69% of HBM's rate).  Many rows: the MMAs,
+// 512 cycles for 128 x 128 x 128 in two parts, at the clock that the power limit leaves (2,048 x 28,672 x 4,096: 355 us in bursts at
+// 1.63 GHz, 413 at 1.35).
 #include "group_units.cuh"
 #include "mxfp4.cuh"
 #include "tensor_map.cuh"
@@ -59,7 +60,7 @@ constexpr int TMEM = 512, SMEM = 227 * 1024;
 // the MMAs are short, instructions are the bound, and two tiles a stage spare half of its waits and barriers.
 // PAIR: a unit is two neighbouring feature tiles, which share the stages of rows; their accumulators are the two that are otherwise
 // those of successive units, and sixteen warps store them.  It halves the reading of rows, and one round of pairs can replace two
-// of single tiles (128 x 28,672 x 4,096: 30 us, 34 single; 64 rows 20.8 and 22.2); see plan_wide.
+// of single tiles (128 x 28,672 x 4,096: 30 us, 34 single; 64 rows 21.1 and 22.2); see plan_wide.
 template <int TOK, bool PAIR> struct Form {
     static constexpr bool WIDE = TOK > NARROW_TOKENS;                    // (the narrow forms cut the line of tiles, and store directly)
     static constexpr bool FEW = TOK <= FEW_TOKENS;
@@ -73,7 +74,7 @@ template <int TOK, bool PAIR> struct Form {
     static constexpr int ATOMS = TOK <= SIDE_BY_SIDE ? 1 : 2 * ((TOK + 127) / 128);
     static constexpr int ACC_COLS = TOK <= SIDE_BY_SIDE ? 2 * TOK : TOK;
     static constexpr int W_COLS = A_COLS + SFA_COLS;
-    static constexpr int TILE_COLS = (TILES * W_COLS + 4 * ATOMS + 7) / 8 * 8;         // [weights | their scales] a feature tile, the rows' scales
+    static constexpr int TILE_COLS = (TILES * W_COLS + 4 * ATOMS + 7) / 8 * 8;  // [weights | their scales] a feature tile, rows' scales
     static constexpr int TILE_BYTES = (TOK * 256 + ATOMS * ATOM + 1023) / 1024 * 1024; // the rows' parts, their scales
     static constexpr int RING_COLS = KT * TILE_COLS, STAGE_BYTES = KT * TILE_BYTES;
     static constexpr int OUT = WIDE ? EPI_GROUPS * OUT_BUFFERS * OUT_BYTES : 0;
@@ -109,7 +110,8 @@ struct MxArgs {
     int* status;
 };
 
-// What a CTA works on at a time: row tile nt (and the one behind it) of a group's matrix, tiles kb0 .. kb0 + n_kb along K, over n_tok rows from m0 on.
+// What a CTA works on at a time: row tile nt (and the one behind it) of a group's matrix, tiles kb0 .. kb0 + n_kb along K, over n_tok
+// rows from m0 on.
 struct Unit { int m0, n_tok, nt, group, kb0, n_kb, share, shares, id; };
 
 __device__ __forceinline__ void mma_mx(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
@@ -202,7 +204,7 @@ __device__ __forceinline__ void st_shared(uint32_t addr, __nv_bfloat16 v) {
 }
 
 // The shares of a row tile, `step` float4 apart, added in order; a thread has four neighbouring features of a token, n .. n + 3 of row
-// m0 + e / 32.  (What it needs comes by value: read through a reference again and again, behind every store, it made this ten times as long.)
+// m0 + e / 32.  (What it needs comes by value: read through a reference behind every store, it made this ten times as long.)
 template <int EPI>
 __device__ __noinline__ void join_shares(const float4* __restrict__ base, size_t step, int shares, int all, int tid, void* out,
                                          long ldo, int m0, int n0, int N, int act, float limit, float slope, int plain_act, int o_bf16,
@@ -359,8 +361,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         return w;
     };
-    // CTAs of neighbouring row tiles of a group want the same rows: each begins at another place along K, or they would all ask for the same
-    // few lines of L2 at once (8 tokens on 6 of 64 experts, 3,584 x 4,096: 68 us, like this 64).
+    // CTAs of neighbouring row tiles of a group want the same rows: each begins at another place along K, or they would all ask for the
+    // same few lines of L2 at once (8 tokens on 6 of 64 experts, 3,584 x 4,096: 68 us, like this 64).
     auto first_tile = [&](const Unit& w) { return GROUPED ? w.nt % w.n_kb : 0; };
     auto stages_of = [&](const Unit& w) { return (w.n_kb + KT - 1) / KT; };
     auto after = [&](uint32_t item, const Unit& w) { return LINE ? item + w.n_kb : item + gridDim.x; };
@@ -384,8 +386,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                     // (a stage's second tile that is none of the unit is the first one again: nothing is multiplied with it)
                     const int k = begin + min(i / TILES, w.n_kb - 1);
                     mbar_expect_tx(smem_u32(&w_full[s]), MX_TILE_BYTES);
-                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES),
-                                  src + (size_t)(k < w.n_kb ? k : k - w.n_kb) * MX_TILE_BYTES + (i % TILES) * next, MX_TILE_BYTES, smem_u32(&w_full[s]));
+                    const uint8_t* from = src + (size_t)(k < w.n_kb ? k : k - w.n_kb) * MX_TILE_BYTES + (i % TILES) * next;
+                    bulk_copy_g2s(smem_u32(w_base + (size_t)s * MX_TILE_BYTES), from, MX_TILE_BYTES, smem_u32(&w_full[s]));
                     if ((s += F::PRODUCERS) >= WS) { s -= WS; phase ^= 1u; }
                 }
                 if (!ok) *bail = 1;
@@ -495,7 +497,8 @@ gemm_mxfp4_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
                 int i = 0;
                 const int stages = stages_of(w), whole = w.n_kb / KT;
                 if constexpr (PAIR) {
-                    // the first tile's products of the stages that the ring holds run ahead, while the epilogue still has the other accumulator
+                    // the first tile's products of the stages that the ring holds run ahead, while the epilogue still has the other
+                    // accumulator
                     const int s0 = s, ahead = w.n_kb < R ? w.n_kb : R;
                     const uint32_t phase0 = phase;
                     for (; i < ahead && ok; ++i) {
@@ -829,12 +832,12 @@ int segments_of(long tiles_n, long kb, long grid) {           // the most stretc
     return (int)most;
 }
 // CTAs, one an SM, each with a few tiles at least or a row tile (32 x 2,048 x 128: 9.3 us where a CTA took four row tiles of one, 5.1
-// with one each), and the most stretches that they cut a row tile into: as many CTAs as leave no
-// more than `limit`, or fewer that cut every row tile alike, down to two thirds of them: a CTA then has one unit, and SMs are left for
-// the next kernel (32 x 4,096 x 14,336 to slabs: 148 stretches 16.0 us, 128 quarters 12.2; 8 rows 10.6 and 10.0, added 13.9 and 11.6;
-// 32 x 6,400 x 4,096 12.9 and 7.5 in 100 halves; with 80 of 148 one row of 10,240 x 8,192 took 13.8 us instead of 12.1).  Where shares have to meet (`join`), row tiles stay whole if they come out even and the longest stretch and the
-// meeting take longer (16 x 28,672 x 4,096 gated: 23.0 us in 148 stretches, 16.7 in 112 of two whole tiles).  In cycles: STAGE for a
-// tile of an SM, JOIN for the partial sums' way through L2 and back.
+// with one each), and the most stretches that they cut a row tile into: as many CTAs as leave no more than `limit`, or fewer that cut
+// every row tile alike, down to two thirds of them: a CTA then has one unit, and SMs are left for the next kernel (32 x 4,096 x 14,336
+// to slabs: 148 stretches 16.0 us, 128 quarters 12.2; 8 rows 10.6 and 10.0, added 13.9 and 11.6; 32 x 6,400 x 4,096 12.9 and 7.5 in 100
+// halves; with 80 of 148 one row of 10,240 x 8,192 took 13.8 us instead of 12.1).  Where shares have to meet (`join`), row tiles stay
+// whole if they come out even and the longest stretch and the meeting take longer (16 x 28,672 x 4,096 gated: 23.0 us in 148 stretches,
+// 16.7 in 112 of two whole tiles).  In cycles: STAGE for a tile of an SM, JOIN for the partial sums' way through L2 and back.
 constexpr int ANY = 1 << 30, LEAST_ITEMS = 4, STAGE = 370, JOIN = 6000;
 struct Cut { int grid, segments; };
 // What was last asked for in a place of a thread's table, and the answer to it (neither allocates nor locks).
@@ -884,14 +887,16 @@ struct Plan { int bn, splits; bool pair; };
 constexpr int MORE_TILES = 2;
 constexpr double L2_BYTES = 62.0;                 // what an SM gets from L2 a cycle when all of them ask
 // The cheapest of the choices in cycles of an SM.  A stage costs its MMAs (2 cycles a column, twice for two parts of more than 64
-// tokens), its way from L2 or its decoding, whichever is most; all CTAs together no less than the weights from HBM.  Decoding's
-// cost grows with the CTAs: products that follow one another overlap on the SMs that the first leaves free (67 x 6,144 x 5,120 one after the
-// other: 96 CTAs 12.9 us, 144 of fewer tokens 17.2; each by itself about 19.5).  A pair's epilogue overlaps little of the next
-// one's products (100 cycles a token for both tiles), of a single tile's only the last one's shows.  Shares of K cost a copy of the output,
-// written and read, and where they meet the adding, which nothing overlaps (67 x 6,144 x 5,120: three shares 21 us, whole 15.6 with
-// the same tiles).  Where it decides for or against pairs: 301 x 28,672 x 4,096 68 us single, 80 in pairs; 128 x 28,672 x 4,096
-// 34 single, 30 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.  (Pairs of up to 64 tokens have three stages in flight for the
-// way to L2 and back, 690 cycles: 64 x 28,672 x 4,096 22.2 single, 20.8 in pairs, 301 in tiles of 64 74.)
+// tokens), its way from L2 or its decoding, whichever is most; all CTAs together no less than the weights from HBM.  Decoding's cost
+// grows with the CTAs: products that follow one another overlap on the SMs that the first leaves free (67 x 6,144 x 5,120 one after the
+// other: 96 CTAs 12.9 us, 144 of fewer tokens 17.2; each by itself about 19.5).  A pair's epilogue overlaps little of the next one's
+// products (100 cycles a token for both tiles), of a single tile's only the last one's shows.  Shares of K cost a copy of the output,
+// written and read, and where they meet the adding, which nothing overlaps (67 x 6,144 x 5,120: three shares 21 us, whole 15.6 with the
+// same tiles).  Where it decides for or against pairs: 301 x 28,672 x 4,096 68 us single, 80 in pairs; 128 x 28,672 x 4,096 34 single,
+// 30 in pairs; 1,024 x 6,144 x 4,096 47 single, 55 in pairs.  (Pairs of up to 64 tokens have three stages in flight for the way to L2
+// and back, 690 cycles: 64 x 28,672 x 4,096 22.2 single, 21.1 in pairs, 301 in tiles of 64 74.)  What the meeting of shares costs is
+// counted as if there were few of them; where there are more than eight, plans come out up to half as long again as the best of their
+// neighbours (33 x 1,024 x 14,336: 23.8 us, 64 rows 16.1).
 Plan cheapest(long M, long N, int kb, int max_splits, long partial_floats, int n_counters, bool slabs) {
     const long sms = fb_sm_count(), tiles_n = (N + MX_ROWS - 1) / MX_ROWS;
     Plan best = {WIDE_TOKENS, 1, false};
@@ -906,7 +911,8 @@ Plan cheapest(long M, long N, int kb, int max_splits, long partial_floats, int n
             for (int splits = 1; splits <= max_splits && splits <= kb; ++splits) {
                 if (!slabs && splits > 1 && (tiles * tiles_n > n_counters || tiles * tiles_n * splits * bn * MX_ROWS > partial_floats)) break;
                 const long units = tiles * units_n * splits, rounds = (units + sms - 1) / sms;
-                const double stage = fmax(fmax((pair ? 8.0 : 4.0) * bn, l2), pair ? (bn <= SIDE_BY_SIDE ? 690.0 : 490.0) : 300.0 + (double)(units < sms ? units : sms)) + 30.0;
+                const double decode = pair ? (bn <= SIDE_BY_SIDE ? 690.0 : 490.0) : 300.0 + (double)(units < sms ? units : sms);
+                const double stage = fmax(fmax((pair ? 8.0 : 4.0) * bn, l2), decode) + 30.0;
                 double cost = fmax((double)rounds * ((kb + splits - 1) / splits * stage + (pair ? 100.0 * bn : 500.0)) + (pair ? 0.0 : 45.0 * bn),
                                    (double)tiles_n * kb * MX_TILE_BYTES / (23.0 * sms));
                 cost += (splits - 1) * (double)M * N * 8.0 / (24.0 * sms);
@@ -929,7 +935,8 @@ Plan plan_wide(int M, int N, int kb, int max_splits, int n_counters, bool slabs)
     return was.value = cheapest(M, N, kb, max_splits, SHARE_FLOATS, n_counters, slabs);
 }
 
-template <int TOK, bool GROUPED, bool PAIR> int launch(const MxArgs& a, const CUtensorMap& mx, const CUtensorMap& mo, long grid, cudaStream_t stream) {
+template <int TOK, bool GROUPED, bool PAIR>
+int launch(const MxArgs& a, const CUtensorMap& mx, const CUtensorMap& mo, long grid, cudaStream_t stream) {
     auto kernel = gemm_mxfp4_kernel<TOK, GROUPED, PAIR>;
     static bool configured[FB_MAX_DEVICES] = {};
     if (fb_needs_setup(configured)) {
@@ -937,15 +944,16 @@ template <int TOK, bool GROUPED, bool PAIR> int launch(const MxArgs& a, const CU
         if (e != cudaSuccess) return fb_fail(-2, "gemm_mxfp4: cannot reserve shared memory: %s", cudaGetErrorString(e));
         fb_setup_done(configured);
     }
-    fb_launch_class(a.M > 128 && Form<TOK, PAIR>::WIDE ? FB_LAUNCH_GEMM_WIDE : FB_LAUNCH_OTHER, kernel, dim3((unsigned)grid), dim3(Form<TOK, PAIR>::THREADS), SMEM, stream, mx, mo, a);
+    fb_launch_class(a.M > 128 && Form<TOK, PAIR>::WIDE ? FB_LAUNCH_GEMM_WIDE : FB_LAUNCH_OTHER, kernel, dim3((unsigned)grid),
+                    dim3(Form<TOK, PAIR>::THREADS), SMEM, stream, mx, mo, a);
     return fb_check_launch("gemm_mxfp4");
 }
 
-// Whether the form of few rows takes the product (tile: the grouped form's row tile, 0: not grouped).  A CTA splits what it multiplies: that
-// spares a kernel that 8 rows spent 4 to 8 us in, behind the weights that the product had on their way by then, and one until the
-// first MMA (shares to slabs, 8 x 4,096 x 14,336, 24 stages a CTA: 17.3 us with that kernel, 11.9 without; 8 x 7,168 x 18,432, 55: 21.7 and
-// 18.2).  But its warps share the issue slots with the decoding: longer stretches are faster with the kernel (8 x 28,672 x 4,096 gated,
-// 64 stages: 14.9 us, 17.5), and so are 16 rows (15.1 us, 30.8) and products whose row tiles share a group's rows (65 us, 93).
+// Whether the form of few rows takes the product (tile: the grouped form's row tile, 0: not grouped).  A CTA splits what it multiplies:
+// that spares a kernel that 8 rows spent 4 to 8 us in, behind the weights that the product had on their way by then, and one until the
+// first MMA (shares to slabs, 8 x 4,096 x 14,336, 24 stages a CTA: 17.3 us with that kernel, 11.9 without; 8 x 7,168 x 18,432, 55: 21.7
+// and 18.2).  But its warps share the issue slots with the decoding: longer stretches are faster with the kernel (8 x 28,672 x 4,096
+// gated, 64 stages: 14.9 us, 17.5), and so are 16 rows (15.1 us, 30.8) and products whose row tiles share a group's rows (65 us, 93).
 constexpr int FEW_STAGES = 60;
 bool few_rows(int M, int N, int K, int tile, bool slabs) {
     if (tile || M > FEW_TOKENS) return false;
@@ -954,7 +962,8 @@ bool few_rows(int M, int N, int K, int tile, bool slabs) {
     return tiles_n * kb <= FEW_STAGES * grid;
 }
 
-// Bytes of the rows' scales.  (Token tiles are at most MORE_TILES more than the rows need; the grouped form has a place for every row tile.)
+// Bytes of the rows' scales.  (Token tiles are at most MORE_TILES more than the rows need; the grouped form has a place for every row
+// tile.)
 long long scale_bytes_of(int M, int kb, int tile) {
     const long long tiles = tile ? M / tile : (M + WIDE_TOKENS - 1) / WIDE_TOKENS + MORE_TILES;
     return kb * tiles * ATOM * (tile == 16 || (!tile && M <= SIDE_BY_SIDE) ? 1 : 2);
@@ -1036,7 +1045,8 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
                          long long scratch_bytes, int* status, cudaStream_t stream) {
     const FbGate gate = {act, limit, slope};
     if (const int rc = check_operands(X, lda, W, out, o_dtype, ldo, M, N, K, gate, plain_act, status)) return rc;
-    FB_REQUIRE(slab_stride == 0 || (o_dtype == FB_F32 && max_slabs >= 1 && slab_stride >= (long long)M * ldo && !act && !plain_act && !accumulate),
+    FB_REQUIRE(slab_stride == 0 || (o_dtype == FB_F32 && max_slabs >= 1 && slab_stride >= (long long)M * ldo && !act && !plain_act &&
+                                    !accumulate),
                "gemm_mxfp4: slabs must be float32, at least one, not overlap, and hold plain shares");
     FB_REQUIRE(!accumulate || (o_dtype == FB_F32 && !act && !plain_act), "gemm_mxfp4: only a float32 product can be added to its output");
     if (splits_used) *splits_used = 1;
@@ -1064,7 +1074,8 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
             if (splits_used) *splits_used = cut.segments;
         }
         if (const int rc = prepare(a, mx, mo, scratch, a.bn, stream)) return rc;
-        return few_rows(M, N, K, 0, slabs) ? launch<FEW_TOKENS, false, false>(a, mx, mo, cut.grid, stream) : launch<32, false, false>(a, mx, mo, cut.grid, stream);
+        return few_rows(M, N, K, 0, slabs) ? launch<FEW_TOKENS, false, false>(a, mx, mo, cut.grid, stream)
+                                           : launch<32, false, false>(a, mx, mo, cut.grid, stream);
     }
     const Plan plan = plan_wide(M, N, a.kb, slabs ? (max_slabs < MOST_SPLITS ? max_slabs : MOST_SPLITS) : join ? MOST_SPLITS : 1, n_counters,
                                 slabs);
@@ -1085,10 +1096,10 @@ FB_API int fb_gemm_mxfp4(const void* X, long long lda, const void* W, void* out,
     return a.bn <= 64 ? launch<64, false, false>(a, mx, mo, grid, stream) : launch<128, false, false>(a, mx, mo, grid, stream);
 }
 
-// The grouped form: W holds `groups` matrices [N, K] in tiles; the M rows of `out` come in tiles of `tile` (a
-// multiple of 16 up to 128) rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are; beyond the last:
-// its products are NaN, and what the activation makes of that).  Row m is
-// X[m], or with row_index X[row_index[m]] (zeros where that is none of the x_rows), with row_share times row_share[row_pair[m]].  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
+// The grouped form: W holds `groups` matrices [N, K] in tiles; the M rows of `out` come in tiles of `tile` (a multiple of 16 up to 128)
+// rows of one group each (tile_group, negative: skipped, its rows of `out` stay as they are; beyond the last: its products are NaN, and
+// what the activation makes of that).  Row m is X[m], or with row_index X[row_index[m]] (zeros where that is none of the x_rows), with
+// row_share times row_share[row_pair[m]].  `scratch`: at least fb_gemm_mxfp4_scratch_bytes on a 128-byte border.
 FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, int x_rows, const int* row_index, const float* row_share, const int* row_pair,
                                  const void* W, int groups, const int* tile_group, int tile, void* out, int o_dtype,
                                  long long ldo, int M, int N, int K, int act, float limit, float slope, int plain_act, void* scratch,
@@ -1111,8 +1122,9 @@ FB_API int fb_gemm_mxfp4_grouped(const void* X, long long lda, int x_rows, const
     a.o_bf16 = o_dtype == FB_BF16; a.M = M; a.N = N; a.K = K; a.tiles_m = 1; a.splits = a.max_segments = 1;
     a.gate = gate; a.plain_act = plain_act; a.status = status;
     a.tile_group = tile_group; a.tile = tile; a.n_tiles = M / tile;
-    // Tiles of 16 are few rows a group, seldom two tiles.  Groups of at most 64 rows have units of 64 (180 tokens on 6 of 64 experts, 3,584 x
-    // 4,096: 116 us, in units of 128 131), larger ones of 128 (1,024 tokens: 214 us, in units of 64 264).
+    // Tiles of 16 are few rows a group, and stay by themselves: six of one group take as long as six of as many groups (20.5 us, 3,584
+    // x 4,096; six tiles of 32 of one group, which are joined, 17.7).  Groups of at most 64 rows have units of 64 (180 tokens on 6 of 64
+    // experts, 3,584 x 4,096: 116 us, in units of 128 131), larger ones of 128 (1,024 tokens: 214 us, in units of 64 264).
     const bool narrow = tile == 16, small = M <= (long)SIDE_BY_SIDE * groups && tile <= SIDE_BY_SIDE;
     a.units_n = a.tiles_n;
     const long units = (long)a.n_tiles * a.units_n;

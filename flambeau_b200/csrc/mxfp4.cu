@@ -1,10 +1,10 @@
 // Rows into four bits and back, and the tiles that the product reads (formats in mxfp4.cuh).
 //
 // A block's scale is the smallest power of two, not below 2^-127, under which its largest magnitude stays below 7, where rounding
-// still ends at 6: with amax = m 2^e, 1 <= m < 2, it is 2^(e - 2), or 2^(e - 1) where m >= 1.75.  Codes are the nearest of the grid,
-// ties to the even code (of 6 and less: scales end at 2^125,
-// so that every number of a block is a finite float32, and magnitudes above 6 times that become it); both follow from bits and from products with powers of two, so they are the same on any machine.  A block
-// with an infinity or a NaN gets scale 255 and decodes to NaN.
+// still ends at 6: with amax = m 2^e, 1 <= m < 2, it is 2^(e - 2), or 2^(e - 1) where m >= 1.75.  Scales end at 2^125, so that every
+// number of a block is a finite float32; magnitudes above 6 times that become it.  Codes are the nearest of the grid, ties to the even
+// code.  Both follow from bits and from products with powers of two, so they are the same on any machine.  A block with an infinity or
+// a NaN gets scale 255 and decodes to NaN.
 //
 // Bound by memory: 2 or 4 bytes in, 17/32 out.  Four threads share a block, eight numbers each; a warp reads 512 bytes (bfloat16) in
 // a row.

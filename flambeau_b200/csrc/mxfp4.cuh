@@ -99,8 +99,8 @@ __device__ __forceinline__ uint32_t mx_split_block(const uint4 (&v)[4], uint2 (&
 // Where a row's word of scales lies among those of a tile.
 __device__ __forceinline__ int mx_scale_place(int row) { return (row >> 7) * 512 + (row & 31) * 16 + (row >> 5 & 3) * 4; }
 
-// Rows that a product reads: row m is x[m], or x[index[m]] (zeros where that is none of x's `count`), times share[pair[m]] (rounded to bfloat16) where
-// there are shares.
+// Rows that a product reads: row m is x[m], or x[index[m]] (zeros where that is none of x's `count`), times share[pair[m]] (rounded
+// to bfloat16) where there are shares.
 struct MxRows {
     const __nv_bfloat16* x; long ld; int count, aligned;
     const int* index; const float* share; const int* pair;
