@@ -1,8 +1,17 @@
 """Rows and four-bit weights of whole numbers: every sum of a product with them is a float32 number whatever the order of its
 terms, so that a product is right when it is equal.  Used by the tests of four-bit weights; runs on any device."""
+from types import SimpleNamespace
+
 import torch
 
 GRID = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def step():
+    """What a product wants of a step: the runtime and its arena."""
+    from flambeau_b200.engine.runtime import Runtime
+    rt = Runtime("cuda:0", "bfloat16")
+    return SimpleNamespace(runtime=rt, ws=rt.ws)
 
 
 def numbers(codes, scales):

@@ -1,16 +1,10 @@
 """SiLU gates in the epilogue of products with four-bit weights, over the whole range of the gate."""
-from types import SimpleNamespace
-
 import pytest
 import torch
 
+from mxfp4_whole import step
+
 pytestmark = pytest.mark.gpu
-
-
-def step():
-    from flambeau_b200.engine.runtime import Runtime
-    rt = Runtime("cuda:0", "bfloat16")
-    return SimpleNamespace(runtime=rt, ws=rt.ws)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

@@ -1,20 +1,14 @@
 """What four-bit weights multiply: rows as two e4m3 numbers under their block's power of two.  Rows with numbers far above their
 block's others, rows at both ends of bfloat16's range, and rows with an infinity or a NaN, in every form."""
 import math
-from types import SimpleNamespace
 
 import pytest
 import torch
 
 import mxfp4_whole as whole
+from mxfp4_whole import step
 
 pytestmark = pytest.mark.gpu
-
-
-def step():
-    from flambeau_b200.engine.runtime import Runtime
-    rt = Runtime("cuda:0", "bfloat16")
-    return SimpleNamespace(runtime=rt, ws=rt.ws)
 
 
 # (rows, outputs, inputs): split by the product itself, ahead of a narrow one (few rows of a long stretch, and more), wide, in pairs

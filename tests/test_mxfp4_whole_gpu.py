@@ -1,19 +1,12 @@
 """Products of whole numbers with four-bit weights are equal to the formula's, in every form: a tile along K, a share, a scale or a
 second part that is lost, repeated or taken from elsewhere shows however long the sums are."""
-from types import SimpleNamespace
-
 import pytest
 import torch
 
 import mxfp4_whole as whole
+from mxfp4_whole import step
 
 pytestmark = pytest.mark.gpu
-
-
-def step():
-    from flambeau_b200.engine.runtime import Runtime
-    rt = Runtime("cuda:0", "bfloat16")
-    return SimpleNamespace(runtime=rt, ws=rt.ws)
 
 
 def weight(shape, K, seed):
@@ -161,3 +154,54 @@ def test_groups(pattern, tile, groups):
         ops.grouped_linear(x, index, w, tiles, tile, act, "relu_squared", ctx, **more)
         assert torch.equal(act[kept], want[kept].float().clamp(min=0).square().bfloat16()) and bool((act[~kept] == 7.0).all())
     ctx.runtime.check_status()
+
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128])
+def test_more_units_than_are_listed(tile):
+    """Thousands of runs of one to five tiles, skipped tiles among them: units behind the first 512 are counted on."""
+    from flambeau_b200.kernels import ops
+    N, K, groups = 200, 96, 7
+    g = torch.Generator().manual_seed(tile)
+    order = torch.repeat_interleave(torch.randint(-1, groups, (1500,), generator=g), torch.randint(1, 6, (1500,), generator=g))
+    tiles = order.int().cuda()
+    M = tile * len(order)
+    w, dense = weight((groups, N), K, 14)
+    x = whole.rows(M, K, 15)
+    of = tiles.repeat_interleave(tile)
+    want = torch.zeros(M, N, dtype=torch.float64, device="cuda")
+    for e in range(groups):
+        want[of == e] = whole.product(x[of == e], dense[e])
+    ctx = step()
+    out = torch.full((M, N), 7.0, device="cuda")
+    ops.grouped_linear(x, None, w, tiles, tile, out, None, ctx)
+    assert torch.equal(out[of >= 0].double(), want[of >= 0]) and bool((out[of < 0] == 7.0).all())
+    ctx.runtime.check_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(70001, 130, 96), (300000, 8, 32)])
+def test_many_rows(M, N, K):
+    from flambeau_b200.kernels import ops
+    w, dense = weight((N,), K, 16)
+    a = whole.rows(M, K, 17)
+    ctx = step()
+    linear_is_equal(a, w, whole.product(a, dense), ctx)
+    finished(ctx)
+
+
+def test_slabs_of_any_number_and_stride():
+    """As many slabs as are given, apart by more than their rows, in rows apart; what lies between is not touched."""
+    from flambeau_b200.kernels import ops
+    N, K = 130, 14336
+    w, dense = weight((N,), K, 18)
+    ctx = step()
+    for M in (1, 8, 20, 40, 130):
+        a = whole.rows(M, K, 19)
+        want = whole.product(a, dense)
+        for most in (2, 5, 40):
+            for pad in (2, 6):
+                room = torch.full((most, M + 1, N + pad), 7.0, device="cuda")
+                slabs = room[:, :M, :N]
+                k = ops.linear_slabs(a, w, slabs, ctx)
+                assert 1 <= k <= most and torch.equal(slabs[:k].sum(0).double(), want)
+                assert bool((room[:, M:] == 7.0).all()) and bool((room[:, :, N:] == 7.0).all()) and bool((room[k:] == 7.0).all())
+    finished(ctx)
